@@ -6,7 +6,8 @@ Importing this package loads two in-tree shared libraries
 * ``lib/libtbe_b200_torch.so`` -- the ``torch.ops.fbgemm.*`` registrations
   (``int_nbit_split_embedding_codegen_lookup_function``,
   ``FloatToFused8BitRowwiseQuantized`` / ``Fused8BitRowwiseQuantizedToFloat``,
-  ``permute_pooled_embs`` and relatives) for the CUDA dispatch key,
+  ``permute_pooled_embs`` and relatives) for the CUDA dispatch key, and ``torch.ops.tbe_b200.*`` for what has no
+  upstream counterpart (token tables in training, 4-bit rows with group scales and products with them),
 
 which is what ``import fbgemm_ascend`` does for the reference through chip detection
 and ``torch.ops.load_library`` (fbgemm_ascend/__init__.py:189-231).  There is one
@@ -41,7 +42,8 @@ def _load():
 cabi_lib = _load()
 
 from . import cabi  # noqa: E402,F401
-from .modules import IntNBitTableBatchedEmbeddingBags, PermutePooledEmbeddings, TableSpec  # noqa: E402,F401
+from .modules import (GroupRowTable, IntNBitTableBatchedEmbeddingBags, PermutePooledEmbeddings, TableSpec,  # noqa: E402,F401
+                      TokenEmbedding)
 
 __all__ = ["PoolingMode", "SparseType", "cabi", "cabi_lib", "IntNBitTableBatchedEmbeddingBags",
-           "PermutePooledEmbeddings", "TableSpec", "CABI_LIB_PATH", "TORCH_LIB_PATH"]
+           "PermutePooledEmbeddings", "TableSpec", "GroupRowTable", "TokenEmbedding", "CABI_LIB_PATH", "TORCH_LIB_PATH"]

@@ -28,7 +28,9 @@ INCLUDE = os.path.join(ROOT, "include")
 CABI_LIB = os.path.join(LIB_DIR, "libtbe_b200.so")
 TORCH_LIB = os.path.join(LIB_DIR, "libtbe_b200_torch.so")
 
-CUDA_SOURCES = ["tbe_common.cu", "tbe_lookup.cu", "tbe_quant.cu", "tbe_permute.cu", "tbe_sparse.cu", "tbe_exchange.cu"]
+CUDA_SOURCES = ["tbe_common.cu", "tbe_lookup.cu", "tbe_quant.cu", "tbe_permute.cu", "tbe_sparse.cu", "tbe_exchange.cu",
+                "tbe_token.cu", "tbe_group_rows.cu", "tbe_group_linear.cu"]
+TORCH_SOURCES = ["torch_ops.cpp", "token_ops.cpp"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
               "-Xcompiler", "-fPIC", "-I" + INCLUDE]
 
@@ -59,7 +61,7 @@ def _run(cmd, verbose):
 def build_cabi(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
-    headers = [os.path.join(CSRC, "tbe_common.cuh"), os.path.join(INCLUDE, "tbe_b200.h")]
+    headers = [os.path.join(CSRC, "tbe_common.cuh"), os.path.join(CSRC, "tbe_elements.cuh"), os.path.join(INCLUDE, "tbe_b200.h")]
     nvcc = _nvcc()
     jobs, objs = [], []
     for src in CUDA_SOURCES:
@@ -76,17 +78,25 @@ def build_cabi(force: bool = False, verbose: bool = False, extra_flags=()) -> st
 
 
 def build_torch(force: bool = False, verbose: bool = False) -> str:
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    if not (force or _newer(TORCH_LIB, [src, os.path.join(INCLUDE, "tbe_b200.h"), CABI_LIB])):
+    header = os.path.join(INCLUDE, "tbe_b200.h")
+    srcs = [os.path.join(CSRC, s) for s in TORCH_SOURCES]
+    if not (force or _newer(TORCH_LIB, srcs + [header, CABI_LIB])):
         return TORCH_LIB
     torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
     cuda_home = os.path.dirname(os.path.dirname(_nvcc()))
     cxx = shutil.which("g++") or "g++"
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=1",
-           "-I" + INCLUDE, "-I" + os.path.join(torch_dir, "include"),
-           "-I" + os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
-           "-I" + os.path.join(cuda_home, "include"),
-           src, "-o", TORCH_LIB,
+    objs, jobs = [], []
+    for s in srcs:
+        o = os.path.join(OBJ_DIR, os.path.basename(s).replace(".cpp", ".torch.o"))
+        objs.append(o)
+        if force or _newer(o, [s, header]):
+            jobs.append([cxx, "-O2", "-std=c++17", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1",
+                         "-I" + INCLUDE, "-I" + os.path.join(torch_dir, "include"),
+                         "-I" + os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+                         "-I" + os.path.join(cuda_home, "include"), "-c", s, "-o", o])
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        list(ex.map(lambda c: _run(c, verbose), jobs))
+    cmd = [cxx, "-shared", "-o", TORCH_LIB] + objs + [
            "-L" + LIB_DIR, "-ltbe_b200", "-L" + os.path.join(torch_dir, "lib"),
            "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda",
            "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(torch_dir, "lib")]

@@ -13,7 +13,7 @@ import torch
 
 from .types import PoolingMode, SparseType
 
-_vp, _i64, _i32 = C.c_void_p, C.c_int64, C.c_int32
+_vp, _i64, _i32, _f32 = C.c_void_p, C.c_int64, C.c_int32, C.c_float
 
 
 class LookupArgs(C.Structure):
@@ -49,6 +49,13 @@ EXPORTS = {
     "tbe_b200_permute_2d_sparse_copy_to_dests": (_i32, [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
     "tbe_b200_signal_peers": (_i32, [_vp, _i32, _i32, _i64, _vp]),
     "tbe_b200_wait_flags": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp]),
+    "tbe_b200_token_embedding": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _i64, _f32, _vp, _i32, _i64, _vp, _vp]),
+    "tbe_b200_token_embedding_grad_scratch_bytes": (_i64, [_i64, _i64, _i64]),
+    "tbe_b200_token_embedding_grad": (_i32, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _f32, _i64, _i32, _vp, _i32, _i64, _vp, _i64,
+                                             _vp]),
+    "tbe_b200_quantize_to_group_rows": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _i64, _vp, _vp]),
+    "tbe_b200_group_row_embedding": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _i32, _i64, _f32, _vp, _i32, _i64, _vp, _vp]),
+    "tbe_b200_group_row_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _i32, _i64, _vp]),
     "tbe_b200_last_error": (C.c_char_p, []),
     "tbe_b200_version": (_i32, []),
 }
@@ -156,6 +163,35 @@ def quantize_to_table_rows(x: torch.Tensor, weight_ty: int, row_bytes_: int, row
     check(lib().tbe_b200_quantize_to_table_rows(int(weight_ty), _ptr(x), x.shape[0], x.shape[1], row_bytes_,
                                                 _ptr(rows_out), _stream()), "tbe_b200_quantize_to_table_rows")
     return rows_out
+
+
+def quantize_to_group_rows(x: torch.Tensor, group_size: int, rows_out: torch.Tensor) -> torch.Tensor:
+    """fp32 / fp16 / bf16 [E, D] -> 4-bit rows with group scales, written in place into ``rows_out`` (uint8 [E, row_bytes])."""
+    assert x.is_contiguous() and rows_out.dtype == torch.uint8 and rows_out.is_contiguous() and rows_out.shape[0] == x.shape[0]
+    check(lib().tbe_b200_quantize_to_group_rows(_ptr(x), int(_OUT_DTYPE[x.dtype]), x.shape[1], x.shape[0], x.shape[1], group_size,
+                                                rows_out.shape[1], _ptr(rows_out), _stream()), "tbe_b200_quantize_to_group_rows")
+    return rows_out
+
+
+def token_embedding(weight: torch.Tensor, tokens: torch.Tensor, output: torch.Tensor, scale: float = 1.0,
+                    error_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``tbe_b200_token_embedding`` on the current stream, into ``output`` [n, D] (rows may lie apart)."""
+    assert tokens.is_contiguous() and weight.stride(1) == 1 and output.stride(1) == 1
+    check(lib().tbe_b200_token_embedding(_ptr(weight), int(_OUT_DTYPE[weight.dtype]), weight.shape[0], weight.shape[1], weight.stride(0),
+                                         _ptr(tokens), tokens.element_size() * 8, tokens.numel(), scale, _ptr(output),
+                                         int(_OUT_DTYPE[output.dtype]), output.stride(0), _ptr(error_flag), _stream()),
+          "tbe_b200_token_embedding")
+    return output
+
+
+def group_row_embedding(rows: torch.Tensor, D: int, group_size: int, tokens: torch.Tensor, output: torch.Tensor, scale: float = 1.0,
+                        error_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``tbe_b200_group_row_embedding`` on the current stream, into ``output`` [n, D] (rows may lie apart)."""
+    assert tokens.is_contiguous() and rows.is_contiguous() and output.stride(1) == 1
+    check(lib().tbe_b200_group_row_embedding(_ptr(rows), rows.shape[0], rows.shape[1], D, group_size, _ptr(tokens), tokens.element_size() * 8,
+                                             tokens.numel(), scale, _ptr(output), int(_OUT_DTYPE[output.dtype]), output.stride(0),
+                                             _ptr(error_flag), _stream()), "tbe_b200_group_row_embedding")
+    return output
 
 
 def permute_pooled_embs_blocked(blocks: torch.Tensor, offset_dim_list: torch.Tensor, permute_list: torch.Tensor,

@@ -1,0 +1,124 @@
+// Rows of fp32 / fp16 / bf16 elements, moved in pieces of VEC elements: shared by the token-table kernels.
+#pragma once
+
+#include <type_traits>
+
+#include "tbe_common.cuh"
+
+namespace tbe {
+
+// VEC consecutive elements of type T as they lie in memory (at most 32 bytes).
+template <typename T, int VEC>
+struct Piece {
+    static constexpr int kBytes = VEC * static_cast<int>(sizeof(T));
+    static constexpr int kWords = (kBytes + 3) / 4;
+    uint32_t w[kWords];
+};
+
+// CONSTANT: nothing writes this memory while the kernel runs (read-only loads).
+template <typename U, bool CONSTANT>
+__device__ __forceinline__ U load_as(const void* p)
+{
+    if constexpr (CONSTANT) return __ldg(static_cast<const U*>(p));
+    else return *static_cast<const U*>(p);
+}
+
+template <typename T, int VEC, bool CONSTANT = true>
+__device__ __forceinline__ void load_piece(Piece<T, VEC>& r, const T* p)
+{
+    constexpr int B = Piece<T, VEC>::kBytes;
+    if constexpr (B >= 16) {
+#pragma unroll
+        for (int i = 0; i < B / 16; ++i) {
+            const uint4 q = load_as<uint4, CONSTANT>(reinterpret_cast<const char*>(p) + 16 * i);
+            r.w[4 * i] = q.x; r.w[4 * i + 1] = q.y; r.w[4 * i + 2] = q.z; r.w[4 * i + 3] = q.w;
+        }
+    } else if constexpr (B == 8) {
+        const uint2 q = load_as<uint2, CONSTANT>(p);
+        r.w[0] = q.x; r.w[1] = q.y;
+    } else if constexpr (B == 4) {
+        r.w[0] = load_as<uint32_t, CONSTANT>(p);
+    } else {
+        r.w[0] = load_as<unsigned short, CONSTANT>(p);
+    }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void clear_piece(Piece<T, VEC>& r)
+{
+#pragma unroll
+    for (int i = 0; i < Piece<T, VEC>::kWords; ++i) r.w[i] = 0u;
+}
+
+// 16-bit types come two to a word; bf16 is the upper half of an fp32.
+template <typename T, int VEC>
+__device__ __forceinline__ float element(const Piece<T, VEC>& r, int i)
+{
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[i]);
+    else {
+        const uint32_t w = r.w[i / 2];
+        if constexpr (std::is_same<T, __half>::value) return half_bits_to_float((i & 1) ? w >> 16 : w & 0xffffu);
+        else return __uint_as_float((i & 1) ? w & 0xffff0000u : w << 16);
+    }
+}
+
+// Rounds VEC fp32 numbers to T (to nearest even) and stores them; streaming, since a result is not read again here.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_piece(T* p, const float (&v)[VEC])
+{
+    if constexpr (VEC == 1) {
+        if constexpr (sizeof(T) == 4) *p = v[0];
+        else if constexpr (std::is_same<T, __half>::value) *p = __float2half_rn(v[0]);
+        else *p = __float2bfloat16_rn(v[0]);
+    } else {
+        constexpr int W = Piece<T, VEC>::kWords;
+        uint32_t w[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+            else if constexpr (std::is_same<T, __half>::value) {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        if constexpr (W >= 4) {
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i)
+                st_stream16(reinterpret_cast<char*>(p) + 16 * i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+        } else if constexpr (W == 2) {
+            st_stream8(p, make_uint2(w[0], w[1]));
+        } else {
+            st_stream4(p, w[0]);
+        }
+    }
+}
+
+inline int element_bytes(int dtype) { return dtype == TBE_B200_FP32 ? 4 : (dtype == TBE_B200_FP16 || dtype == TBE_B200_BF16) ? 2 : 0; }
+
+// Whether rows that start at p, stride elements apart, can be moved in pieces of vec elements.
+inline bool rows_aligned(const void* p, int64_t stride, int elem_bytes, int vec)
+{
+    const int64_t b = static_cast<int64_t>(vec) * elem_bytes < 16 ? static_cast<int64_t>(vec) * elem_bytes : 16;
+    return reinterpret_cast<uintptr_t>(p) % b == 0 && (stride * elem_bytes) % b == 0;
+}
+
+// Calls f with a null pointer to the element type that `dtype` (checked before) names.
+template <typename F>
+int with_element(int dtype, F&& f)
+{
+    switch (dtype) {
+        case TBE_B200_FP32: return f(static_cast<float*>(nullptr));
+        case TBE_B200_FP16: return f(static_cast<__half*>(nullptr));
+        default: return f(static_cast<__nv_bfloat16*>(nullptr));
+    }
+}
+
+// 4-bit rows with group scales (tbe_group_rows.cu): log2 of a group size, -1 if it is none; and the argument checks that every
+// entry point over such rows makes.
+int group_log2_of(int group_size);
+int check_group_rows(const char* op, int64_t D, int group_size, int64_t row_bytes, const void* rows, int64_t nrows);
+
+}  // namespace tbe

@@ -16,7 +16,7 @@ from typing import Callable, List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import cabi
-from .types import PoolingMode, SparseType, row_bytes
+from .types import PoolingMode, SparseType, group_row_bytes, row_bytes
 
 
 @dataclass
@@ -142,6 +142,84 @@ class IntNBitTableBatchedEmbeddingBags:
             fp8_exponent_bias=self.fp8_exponent_bias)
 
     __call__ = forward
+
+
+class TokenEmbedding(torch.nn.Module):
+    """A trainable token table: ``scale * weight[tokens]`` and the table's gradient, both by this package's kernels.
+
+    ``weight`` is fp32, fp16 or bf16; a token outside the table (-1 among them) looks up zeros and gets no gradient, a
+    ``padding_idx`` looks up its row and gets none.  The gradient is dense and of the table's type; a program that keeps
+    gradients in a buffer of its own (in fp32, over several micro-batches) calls :meth:`add_gradient_` instead, which
+    touches the rows met only.  No counterpart in the reference, which serves tables and does not train them.
+
+    A step captured into a CUDA graph needs outputs of earlier eager steps released first, unless those ran on a side
+    stream; the lookup refuses the capture otherwise.
+    """
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, scale: float = 1.0,
+                 dtype: torch.dtype = torch.float32, device: Union[str, torch.device] = "cuda",
+                 output_dtype: Optional[SparseType] = None) -> None:
+        super().__init__()
+        if torch.device(device).type != "cuda":
+            raise RuntimeError("TokenEmbedding needs a CUDA device: there is no CPU path")
+        self.num_embeddings, self.embedding_dim = int(num_embeddings), int(embedding_dim)
+        self.padding_idx, self.scale = padding_idx, float(scale)
+        self.output_dtype = None if output_dtype is None else int(output_dtype)
+        self.weight = torch.nn.Parameter(torch.empty(self.num_embeddings, self.embedding_dim, dtype=dtype, device=device))
+        torch.nn.init.normal_(self.weight, std=self.embedding_dim ** -0.5)
+
+    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+        return torch.ops.tbe_b200.token_embedding(self.weight, tokens, scale=self.scale, padding_idx=self.padding_idx,
+                                                  output_dtype=self.output_dtype)
+
+    def add_gradient_(self, into: torch.Tensor, grad: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
+        """``into[v] += scale * sum of grad over the tokens v``, in place."""
+        with torch.no_grad():
+            return torch.ops.tbe_b200.token_embedding_grad_(into, grad, tokens, scale=self.scale, padding_idx=self.padding_idx)
+
+
+class GroupRowTable:
+    """A table or weight matrix in 4 bits, one fp16 scale and bias per ``group_size`` elements of a row.
+
+    ``rows`` is uint8 ``[num_embeddings, group_row_bytes(D, group_size)]``; the same bytes serve the lookup of tokens
+    (:meth:`forward`) and products with all rows (:meth:`linear`: a layer, or scores over a vocabulary).
+    """
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, group_size: int = 128, device: Union[str, torch.device] = "cuda",
+                 output_dtype: SparseType = SparseType.BF16) -> None:
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError("GroupRowTable needs a CUDA device: there is no CPU path")
+        if group_size not in (32, 64, 128, 256):
+            raise ValueError(f"group_size must be 32, 64, 128 or 256, got {group_size}")
+        if embedding_dim <= 0 or embedding_dim % SparseType.INT4.align_size() != 0:
+            raise ValueError(f"D={embedding_dim} must be a positive multiple of {SparseType.INT4.align_size()}")
+        self.num_embeddings, self.embedding_dim, self.group_size = int(num_embeddings), int(embedding_dim), int(group_size)
+        self.output_dtype = int(output_dtype)
+        self.rows = torch.zeros(self.num_embeddings, group_row_bytes(self.embedding_dim, self.group_size), dtype=torch.uint8, device=self.device)
+
+    def assign_rows_from_float(self, x: torch.Tensor, row_start: int = 0) -> None:
+        """Quantize fp32, fp16 or bf16 ``x`` [n, D] into rows ``row_start .. row_start + n``."""
+        n = x.shape[0]
+        if x.dim() != 2 or x.shape[1] != self.embedding_dim or row_start < 0 or row_start + n > self.num_embeddings:
+            raise ValueError(f"rows {row_start} .. {row_start + n} of {tuple(x.shape)} do not fit a table of "
+                             f"[{self.num_embeddings}, {self.embedding_dim}]")
+        with torch.cuda.device(self.device):
+            cabi.quantize_to_group_rows(x.detach().to(self.device).contiguous(), self.group_size, self.rows[row_start:row_start + n])
+
+    def to_float(self) -> torch.Tensor:
+        return torch.ops.tbe_b200.group_rows_to_float(self.rows, self.embedding_dim, self.group_size, output_dtype=int(SparseType.FP32))
+
+    def forward(self, tokens: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+        return torch.ops.tbe_b200.group_row_embedding(self.rows, tokens, self.embedding_dim, self.group_size, scale=scale,
+                                                      output_dtype=self.output_dtype)
+
+    __call__ = forward
+
+    def linear(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None, output_dtype: Optional[SparseType] = None) -> torch.Tensor:
+        """``x @ rows.T (+ bias)``: [..., D] -> [..., num_embeddings]; made for up to 16 vectors."""
+        return torch.ops.tbe_b200.group_row_linear(x, self.rows, self.group_size, bias=bias,
+                                                   output_dtype=None if output_dtype is None else int(output_dtype))
 
 
 class PermutePooledEmbeddings:

@@ -44,3 +44,8 @@ def row_bytes(ty: int, D: int, row_alignment: int = 16) -> int:
     if row_alignment > 1:
         b = (b + row_alignment - 1) // row_alignment * row_alignment
     return b
+
+
+def group_row_bytes(D: int, group_size: int) -> int:
+    """Bytes of one 4-bit row with group scales: D / 2 bytes of codes, 4 bytes per group, padded to 16."""
+    return (D // 2 + 4 * (-(-D // group_size)) + 15) // 16 * 16

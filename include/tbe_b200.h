@@ -267,6 +267,56 @@ int tbe_b200_signal_peers(int64_t* const* peer_flags, int32_t world, int32_t my_
 int tbe_b200_wait_flags(const int64_t* flags, int32_t world, int64_t value, int64_t max_polls, int32_t* error_flag,
                         tbe_b200_stream_t stream);
 
+/* ---- token tables: trained rows, 4-bit rows with group scales, products with them ----------------
+ *
+ * No counterparts in the reference.  Element types are given as TBE_B200_FP32, _FP16 or _BF16; strides count elements
+ * between consecutive rows (at least D); `tokens` is a contiguous array of token_bits (32 or 64) bits per entry.  A token
+ * outside [0, num_embeddings) names no row: it looks up zeros and takes part in no gradient; entries other than -1 that
+ * do so set bit 4 of *error_flag (if given), like an index past its table's end in the lookup above. */
+
+/* output[i, :] = scale * weight[tokens[i], :], the product rounded once to the output's type. */
+int tbe_b200_token_embedding(const void* weight, int32_t weight_dtype, int64_t num_embeddings, int64_t D, int64_t weight_stride,
+                             const void* tokens, int32_t token_bits, int64_t n, float scale, void* output, int32_t output_dtype,
+                             int64_t output_stride, int32_t* error_flag, tbe_b200_stream_t stream);
+
+/* The gradient of tbe_b200_token_embedding by its table:
+ *   grad_weight[v, :] = [grad_weight[v, :] if accumulate] + scale * sum of grad[i, :] over the i with tokens[i] == v
+ * Tokens are sorted first, so every row's sum has one fixed order: a call gives the same bits every time.  Sums are held
+ * in fp32 and rounded once.  accumulate 0: every row is written, zeros where no token names it; 1: only rows that
+ * tokens name are read and written.  Tokens equal to padding_idx (-1: none) take part in no gradient.
+ * scratch: tbe_b200_token_embedding_grad_scratch_bytes(n, num_embeddings, D) bytes of device memory, 16-byte aligned,
+ * overwritten by the call; two calls that may overlap need separate scratch.  The function returns -1 for sizes that
+ * the call refuses.  n and num_embeddings are below 2^31. */
+int64_t tbe_b200_token_embedding_grad_scratch_bytes(int64_t n, int64_t num_embeddings, int64_t D);
+int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtype, int64_t grad_stride, const void* tokens, int32_t token_bits,
+                                  int64_t n, int64_t num_embeddings, int64_t D, float scale, int64_t padding_idx,
+                                  int32_t accumulate, void* grad_weight, int32_t grad_weight_dtype, int64_t grad_weight_stride,
+                                  void* scratch, int64_t scratch_bytes, tbe_b200_stream_t stream);
+
+/* 4-bit rows with group scales: a row of D elements (D a multiple of 8) in groups of group_size (32, 64, 128 or 256; the
+ * last group may be shorter) is
+ *   [D / 2 bytes of codes, low nibble first][fp16 scale, fp16 bias of every group][zeros up to row_bytes]
+ * with row_bytes a multiple of 16, and element c stands for code * scale + bias of group c / group_size.  With one group
+ * these are the bytes of tbe_b200_quantize_nbit_rowwise_sbhalf(4, ...), padded; the arithmetic is the same group by group.
+ * `rows` is 16-byte aligned.  Rows with a non-finite element get codes without a meaning. */
+int tbe_b200_quantize_to_group_rows(const void* input, int32_t input_dtype, int64_t input_stride, int64_t nrows, int64_t D,
+                                    int32_t group_size, int64_t row_bytes, uint8_t* rows, tbe_b200_stream_t stream);
+
+/* output[i, :] = scale * the numbers of row tokens[i], rounded once (num_embeddings rows).  tokens NULL: row i itself
+ * (n <= num_embeddings), which reads a table back. */
+int tbe_b200_group_row_embedding(const uint8_t* rows, int64_t num_embeddings, int64_t row_bytes, int64_t D, int32_t group_size,
+                                 const void* tokens, int32_t token_bits, int64_t n, float scale, void* output, int32_t output_dtype,
+                                 int64_t output_stride, int32_t* error_flag, tbe_b200_stream_t stream);
+
+/* Products of a few vectors with every row: output[i, r] = sum over c of input[i, c] * (number c of row r) + bias[r], for
+ * m vectors of D elements and num_rows rows; fp32 accumulation, one rounding.  bias (num_rows entries) may be NULL.
+ * `input` is 16-byte aligned and input_stride a multiple of 8 elements.  Made for m up to 16 (a decoding step's states): every
+ * 16 vectors read the rows once more. */
+int tbe_b200_group_row_linear(const void* input, int32_t input_dtype, int64_t input_stride, int64_t m, const uint8_t* rows,
+                              int64_t num_rows, int64_t row_bytes, int64_t D, int32_t group_size, const void* bias,
+                              int32_t bias_dtype, void* output, int32_t output_dtype, int64_t output_stride,
+                              tbe_b200_stream_t stream);
+
 /* Message of the last failure on the calling thread ("" if none).  Host pointer,
  * valid until the next failing call on the same thread. */
 const char* tbe_b200_last_error(void);
