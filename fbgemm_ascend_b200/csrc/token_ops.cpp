@@ -351,7 +351,7 @@ Tensor group_row_linear(const Tensor& input, const Tensor& rows, int64_t group_s
     Tensor out = at::empty(shape, x.options().dtype(type));
     check_status(tbe_b200_group_row_linear(x.data_ptr(), it, row_stride(x), m, r.data_ptr<uint8_t>(), N, r.size(1), D, static_cast<int32_t>(group_size),
                                            b.defined() ? b.data_ptr() : nullptr, b.defined() ? element_type(b, op, "bias") : 0, out.data_ptr(),
-                                           static_cast<int32_t>(out_type), N, current_stream()), op);
+                                           static_cast<int32_t>(out_type), N, nullptr, current_stream()), op);
     return out;
 }
 
