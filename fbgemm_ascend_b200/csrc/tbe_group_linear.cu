@@ -37,81 +37,115 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// How states of type T meet the codes: the operand type, and into how many pieces a state's element is cut.  fp32 has 24
-// significant bits, which three bf16 pieces hold exactly over the whole range.
-template <typename T> struct Operand { static constexpr int kPieces = 1; static constexpr bool kHalf = std::is_same<T, __half>::value; };
-template <> struct Operand<float> { static constexpr int kPieces = 3; static constexpr bool kHalf = false; };
-
-// One word of codes (elements 0 .. 7, low nibble first) as four pairs (0,4) (1,5) (2,6) (3,7) of code - 8.  A nibble or'ed into
-// the low bits of 1024 (fp16: 16 steps apart for the upper nibble of a byte) or 128 (bf16) makes that number plus the
-// code; what is taken off again leaves it exact.
-template <bool HALF>
+// One word of codes (elements 0 .. 7, low nibble first) as four pairs (0,4) (1,5) (2,6) (3,7) of code - 8 in fp16.  A nibble
+// or'ed into the low bits of 1024 (16 steps apart for the upper nibble of a byte) makes that number plus the code; what is
+// taken off again leaves it exact.
 __device__ __forceinline__ void decode(uint32_t w, uint32_t (&p)[4])
 {
-    if constexpr (HALF) {
-        const uint32_t v = w >> 8;
-        const uint32_t lo[4] = {(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x64006400u, (v & 0x000f000fu) | 0x64006400u, (v & 0x00f000f0u) | 0x64006400u};
-        const __half2 even = __float2half2_rn(1032.0f), sixteenth = __float2half2_rn(0.0625f), odd = __float2half2_rn(-72.0f);
+    const uint32_t v = w >> 8;
+    const uint32_t in[4] = {(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x64006400u, (v & 0x000f000fu) | 0x64006400u, (v & 0x00f000f0u) | 0x64006400u};
+    const __half2 even = __float2half2_rn(1032.0f), sixteenth = __float2half2_rn(0.0625f), odd = __float2half2_rn(-72.0f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 h = *reinterpret_cast<const __half2*>(&lo[i]);
-            const __half2 r = (i & 1) ? __hfma2(h, sixteenth, odd) : __hsub2(h, even);
-            p[i] = *reinterpret_cast<const uint32_t*>(&r);
-        }
-    } else {
-        const __nv_bfloat162 off = __float2bfloat162_rn(136.0f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t b = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-            const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), off);
-            p[i] = *reinterpret_cast<const uint32_t*>(&r);
-        }
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = *reinterpret_cast<const __half2*>(&in[i]);
+        const __half2 r = (i & 1) ? __hfma2(h, sixteenth, odd) : __hsub2(h, even);
+        p[i] = *reinterpret_cast<const uint32_t*>(&r);
     }
 }
 
-template <bool HALF>
+// c = a * b, or c += a * b.
+template <bool FIRST>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    if constexpr (HALF)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if constexpr (FIRST)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
     else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Eight elements of a state as pairs (0,4) (1,5) (2,6) (3,7), one set per piece; zeros where `live` is false.
+// ---- the states, in the order that the matrix instructions take them --------------------------------------------
+//
+// A state's elements become fp16: as they are, or times the power of two that brings the state's largest into 2^14 .. 2^15
+// (bf16 keeps its 8 bits then, but for elements below 2^-28 of the largest, which are off by 2^-40 of it at most); fp32 in
+// two pieces, 22 bits and a sign, off by 2^-23 at most.  The sums are scaled back.
+// For NT * 8 states and a unit of 128 elements: four steps of NT sets of P pieces of 512 bytes, 16 to each lane, then the
+// sums of the states over every group of the unit.
+template <typename T> constexpr int kPieces = sizeof(T) == 4 ? 2 : 1;
+
+__host__ __device__ constexpr int sums_bytes(int NT, int steps) { return 4 / steps * NT * 32; }
+__host__ __device__ constexpr int unit_bytes(int NT, int P, int steps) { return P * NT * 2048 + sums_bytes(NT, steps); }
+
+constexpr int kStateThreads = 512;
+
+// One block per state.
 template <typename T>
-__device__ __forceinline__ void state_pairs(const T* p, bool live, uint4 (&out)[Operand<T>::kPieces])
+__global__ void __launch_bounds__(kStateThreads)
+arrange_states_kernel(const T* __restrict__ x, int64_t x_stride, int D, int NT, int steps, unsigned char* __restrict__ arranged, float* __restrict__ back)
 {
-    Piece<T, 8> r;
-    if (live) load_piece<T, 8>(r, p);
-    else clear_piece(r);
-    if constexpr (sizeof(T) == 2) {
-        out[0] = make_uint4(__byte_perm(r.w[0], r.w[2], 0x5410), __byte_perm(r.w[0], r.w[2], 0x7632), __byte_perm(r.w[1], r.w[3], 0x5410),
-                            __byte_perm(r.w[1], r.w[3], 0x7632));
-    } else {
-        // cut off, not rounded: fp32's largest numbers stay finite, and the remainders are exact
-        uint32_t top[3][8];
+    constexpr int P = kPieces<T>;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int m = blockIdx.x, units = (D + kUnit - 1) / kUnit, words = units * (kUnit / 8);
+    const T* row = x + m * x_stride;
+    float scale = 1.0f;
+    if constexpr (!std::is_same<T, __half>::value) {
+        __shared__ int largest;
+        if (threadIdx.x == 0) largest = 0;
+        __syncthreads();
+        int most = 0;      // magnitudes order like their bits
+        for (int i = threadIdx.x; i < D / 8; i += kStateThreads) {
+            Piece<T, 8> r;
+            load_piece<T, 8>(r, row + i * 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = max(most, static_cast<int>(__float_as_uint(element(r, e)) & 0x7fffffffu));
+        }
+        most = __reduce_max_sync(kFull, most);
+        if ((threadIdx.x & 31) == 0) atomicMax(&largest, most);
+        __syncthreads();
+        // 2^e, 14 - e the largest's exponent; both ways within fp32's normal numbers
+        const int e = min(126, 14 - ((largest >> 23) - 127));
+        scale = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        if (threadIdx.x == 0) back[m] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    } else if (threadIdx.x == 0) {
+        back[m] = 1.0f;
+    }
+    const int n = (m % (NT * 8)) / 8, col = m % 8, unit_size = unit_bytes(NT, P, steps);
+    unsigned char* to = arranged + static_cast<int64_t>(m / (NT * 8)) * units * unit_size;
+    for (int i = threadIdx.x; i < (words + 31) / 32 * 32; i += kStateThreads) {      // whole warps go round
+        Piece<T, 8> r;
+        if (i * 8 < D) load_piece<T, 8>(r, row + i * 8);
+        else clear_piece(r);
+        const int u = i / 16, q = i % 16, step = steps < 4 ? q / 4 : q % 4, t = steps < 4 ? q % 4 : q / 4;
+        unsigned char* unit = to + static_cast<int64_t>(u) * unit_size;
+        __half h[P][8];
+        float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float v = __uint_as_float(r.w[e]);
-            const bool finite = (r.w[e] & 0x7f800000u) != 0x7f800000u;
-            const float hi = __uint_as_float(r.w[e] & 0xffff0000u), rest = v - hi;
-            const float mid = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-            top[0][e] = (v != v) ? 0x7fc0u : r.w[e] >> 16;
-            top[1][e] = finite ? __float_as_uint(mid) >> 16 : 0u;
-            top[2][e] = finite ? __float_as_uint(rest - mid) >> 16 : 0u;
+            const float v = element(r, e) * scale;
+            h[0][e] = __float2half_rn(v);
+            if constexpr (P == 2) {
+                const float rest = v - __half2float(h[0][e]);
+                h[1][e] = __float2half_rn(isfinite(rest) ? rest : 0.0f);      // of an infinite element nothing is left
+                sum += __half2float(h[1][e]);
+            }
+            sum += __half2float(h[0][e]);
         }
+        for (int d = 1; d < 4 * steps; d <<= 1) sum += __shfl_xor_sync(kFull, sum, d);
+        if (i >= words) continue;
 #pragma unroll
-        for (int q = 0; q < 3; ++q)
-            out[q] = make_uint4(top[q][0] | (top[q][4] << 16), top[q][1] | (top[q][5] << 16), top[q][2] | (top[q][6] << 16), top[q][3] | (top[q][7] << 16));
+        for (int p = 0; p < P; ++p) {
+            const __half2 pair[4] = {__halves2half2(h[p][0], h[p][4]), __halves2half2(h[p][1], h[p][5]), __halves2half2(h[p][2], h[p][6]), __halves2half2(h[p][3], h[p][7])};
+            *reinterpret_cast<uint4*>(unit + ((step * NT + n) * P + p) * 512 + (col * 4 + t) * 16) = *reinterpret_cast<const uint4*>(pair);
+        }
+        if (q % (4 * steps) == 0) *reinterpret_cast<float*>(unit + P * NT * 2048 + (q / (4 * steps) * NT * 8 + n * 8 + col) * 4) = sum;
     }
 }
 
 struct LinearArgs {
-    const void* x;
-    int64_t x_stride, m;
+    const unsigned char* arranged;              // states as arrange_states_kernel leaves them, and what undoes their scales
+    const float* back;
+    int64_t m;
     const uint8_t* rows;
     int64_t num_rows, row_bytes;
     int D, group_log2;
@@ -158,14 +192,25 @@ __device__ __forceinline__ void box_copy(uint32_t to, const CUtensorMap* map, in
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x),
                  "r"(y), "r"(bar) : "memory");
 }
+// A run of bytes, all 16-byte aligned.
+__device__ __forceinline__ void bulk_copy(uint32_t to, const void* from, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
 __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
-// Bytes of a row's scales and biases that `units` units of it need, as they are fetched: from a 16-byte border on, in whole
-// 16-byte pieces, an odd number of them (so that eight rows' words lie in different banks).
-int head_window(int units, int group_log2)
+// Bytes of a row's scales and biases that a chunk of `slices` (at least 2) units needs, as they are fetched: from the 16-byte
+// border in front of them on, in whole 16-byte pieces, an odd number of them (so that eight rows' words lie in different
+// banks).  A chunk begins with a group, and where in 16 bytes repeats after four chunks at most.
+int head_window(int D, int slices, int group_log2)
 {
-    const int groups = ((units * kUnit - 1) >> group_log2) + 2;
-    return (((groups * 4 + 15) / 16 + 1) | 1) * 16;
+    const int bytes = 4 * (slices * kUnit >> group_log2);
+    int most = 0;
+    for (int c = 0; c < 4; ++c) {
+        const int pieces = ((D / 2 + c * bytes) % 16 + bytes + 15) / 16;
+        most = pieces > most ? pieces : most;
+    }
+    return (most | 1) * 16;
 }
 
 // The row that lane group g stands for among eight.  Copies put 16-byte piece p of row r at place p ^ (r % 8) of its 128 bytes:
@@ -178,26 +223,26 @@ __device__ __forceinline__ int row_of(int g) { return (g >> 1) | ((g & 1) << 2);
 // scales and biases of their groups.
 //
 // In a unit lane (g, t) = (lane / 4, lane % 4) takes two rows of every 16.  One matrix instruction takes 4 elements of each lane,
-// and one group: where a group is at least a unit, lane t takes elements 32 t .. 32 t + 31 with one 16-byte load; SMALL
+// and one group: where a group is at least a unit, lane t takes elements 32 t .. 32 t + 31 with one 16-byte load; small
 // groups (32 and 64) need an instruction's elements side by side, so that lane t takes elements 32 s + 8 t .. + 7 in step
 // s, a word at a time.
-// SHARED: the states lie in shared memory in the order that the instructions take them, else they are read as they are.
-template <typename T, int RT, int NT, bool SMALL, bool SHARED>
+// STEPS: how many steps of a unit a group spans.  P: pieces of a state's element.
+template <int RT, int NT, int P, int STEPS>
 __global__ void __launch_bounds__(kThreads, 1)
 group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap head_map)
 {
-    constexpr int P = Operand<T>::kPieces;
-    constexpr bool HALF = Operand<T>::kHalf;
     constexpr int kPitch = RT * 16 + 4;         // of a state's sums in shared memory: a warp's stores meet no bank twice
     constexpr int kPart = NT * 8 * kPitch;      // one warp's sums
+    constexpr int kStates = unit_bytes(NT, P, STEPS);
     extern __shared__ __align__(1024) unsigned char smem[];
     const int bands = kWarps >> a.slices_log2, slices = 1 << a.slices_log2, tile_rows = bands * RT * 16;
-    const int code_bytes = tile_rows * slices * (kUnit / 2), head_bytes = tile_rows * a.head_bytes;
-    // boxes of codes first (1024-byte aligned), then those of heads, sums, states, barriers
-    unsigned char* heads_at = smem + a.stages * code_bytes;
-    float* red = reinterpret_cast<float*>(heads_at + a.stages * head_bytes);
+    constexpr int kCodeBytes = kWarps * RT * 16 * (kUnit / 2);
+    const int head_bytes = tile_rows * a.head_bytes;
+    // boxes of codes first (1024-byte aligned), then those of heads, the states, sums, barriers
+    unsigned char* heads_at = smem + a.stages * kCodeBytes;
+    unsigned char* states_at = heads_at + a.stages * head_bytes;
+    float* red = reinterpret_cast<float*>(states_at + a.stages * slices * kStates);
     const uint32_t full = shared_address(red + kParts * kPart), empty = full + 8 * kMostStages;
-    uint4* xs = reinterpret_cast<uint4*>(red + kParts * kPart + 4 * kMostStages);
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int units = (a.D + kUnit - 1) / kUnit, groups = (a.D + (1 << a.group_log2) - 1) >> a.group_log2;
@@ -217,46 +262,64 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     if (warp == kWarps) {
         // ---- the warp that fetches ------------------------------------------------------------------------------------
         if (lane != 0) return;
+        const unsigned char* arranged = a.arranged + static_cast<int64_t>(blockIdx.y) * units * kStates;
+        int64_t tile = blockIdx.x;
+        int chunk = 0;
+        auto next = [&] {
+            if (++chunk == chunks) {
+                chunk = 0;
+                tile += gridDim.x;
+            }
+        };
+        auto states_of = [&](int c) { return (units - (c << a.slices_log2) < slices ? units - (c << a.slices_log2) : slices) * kStates; };
+        auto fetch_rows = [&](int stage) {
+            const uint32_t bar = full + 8 * stage;
+            const int first = static_cast<int>(tile * tile_rows);
+            barrier_expect(bar, kCodeBytes + head_bytes + states_of(chunk));
+            // what lies outside the matrix arrives as zeros
+            for (int k = 0; k < slices / 2; ++k)
+                box_copy(shared_address(smem + stage * kCodeBytes + k * (tile_rows * 128)), &code_map, (chunk * (slices / 2) + k) * 32, first, bar);
+            const int g0 = (chunk * slices * kUnit) >> a.group_log2;
+            box_copy(shared_address(heads_at + stage * head_bytes), &head_map, ((a.D / 2 + 4 * g0) & ~15) / 4, first, bar);
+        };
+        auto fetch_states = [&](int stage) {
+            bulk_copy(shared_address(states_at + stage * slices * kStates), arranged + static_cast<int64_t>(chunk << a.slices_log2) * kStates, states_of(chunk),
+                      full + 8 * stage);
+        };
+        // The first stages' rows are on their way before the states are ready.
+        int filled = 0;
+        for (; filled < a.stages && tile < a.tiles; ++filled) {
+            fetch_rows(filled);
+            next();
+        }
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        tile = blockIdx.x;
+        chunk = 0;
+        for (int i = 0; i < filled; ++i) {
+            fetch_states(i);
+            next();
+        }
         int stage = 0;
         uint32_t round = 0;
-        for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-            const int first = static_cast<int>(tile * tile_rows);
-            for (int c = 0; c < chunks; ++c) {
-                if (round > 0 && !barrier_wait(empty + 8 * stage, (round - 1) & 1)) {
-                    if (a.error_flag) atomicOr(a.error_flag, 16);
-                    return;
-                }
-                const uint32_t bar = full + 8 * stage;
-                barrier_expect(bar, code_bytes + head_bytes);
-                // what lies outside the matrix arrives as zeros
-                for (int k = 0; k < slices / 2; ++k)
-                    box_copy(shared_address(smem + stage * code_bytes + k * (tile_rows * 128)), &code_map, (c * (slices / 2) + k) * 32, first, bar);
-                const int g0 = (c * slices * kUnit) >> a.group_log2;
-                box_copy(shared_address(heads_at + stage * head_bytes), &head_map, ((a.D / 2 + 4 * g0) & ~15) / 4, first, bar);
-                if (++stage == a.stages) {
-                    stage = 0;
-                    ++round;
-                }
+        while (tile < a.tiles) {
+            if (!barrier_wait(empty + 8 * stage, round & 1)) {
+                if (a.error_flag) atomicOr(a.error_flag, 16);
+                return;
+            }
+            fetch_rows(stage);
+            fetch_states(stage);
+            next();
+            if (++stage == a.stages) {
+                stage = 0;
+                ++round;
             }
         }
         return;      // the workers wait for every copy
     }
 
     // ---- the warps that work ---------------------------------------------------------------------------------------
+    asm volatile("griddepcontrol.wait;" ::: "memory");      // `back` is read at a tile's end
     const int g = row_of(lane >> 2), t = lane & 3, slice = warp & (slices - 1), band = warp >> a.slices_log2;
-    const T* x = static_cast<const T*>(a.x) + m0 * a.x_stride;
-    const int words = units * (kUnit / 8);
-    if constexpr (SHARED) {
-        for (int i = threadIdx.x; i < words * cols; i += kWorkers) {
-            const int j = i / words, wd = i - j * words, u = wd / 16, q = wd % 16;
-            const int step = SMALL ? q / 4 : q % 4, lt = SMALL ? q % 4 : q / 4;
-            uint4 v[P];
-            state_pairs<T>(x + j * a.x_stride + wd * 8, wd * 8 < a.D, v);
-#pragma unroll
-            for (int p = 0; p < P; ++p) xs[(p * words + (u * 4 + step) * 4 + lt) * cols + j] = v[p];
-        }
-        workers_sync();
-    }
     float y[RT][NT][4];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -265,6 +328,14 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[i][n][e] = 0.0f;
 
+    // this lane's places in a stage
+    const unsigned char* code_rows = smem + (slice >> 1) * (tile_rows * 128) + (band * RT * 16 + g) * 128;
+    const int half = (slice & 1) * 4, row8 = 8 * a.head_bytes;
+    int piece[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) piece[k] = STEPS < 4 ? ((half + k) ^ g) * 16 + t * 4 : ((half + t) ^ g) * 16;
+    const unsigned char* head_rows = heads_at + (band * RT * 16 + g) * a.head_bytes;
+    const unsigned char* my_states = states_at + slice * kStates;
     int stage = 0;
     uint32_t round = 0;
     for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
@@ -272,81 +343,62 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
             if (!barrier_wait(full + 8 * stage, round & 1) && a.error_flag) atomicOr(a.error_flag, 16);
             const int u = (c << a.slices_log2) + slice;
             if (u < units) {
-                const unsigned char* code_rows = smem + stage * code_bytes + (slice >> 1) * (tile_rows * 128) + (band * RT * 16 + g) * 128;
-                const int half = (slice & 1) * 4;
+                const unsigned char* codes = code_rows + stage * kCodeBytes;
+                const unsigned char* states = my_states + stage * slices * kStates;
                 const int g0 = (c * slices * kUnit) >> a.group_log2;
-                const unsigned char* head_rows = heads_at + stage * head_bytes + (band * RT * 16 + g) * a.head_bytes + ((a.D / 2 + 4 * g0) & 15) - 4 * g0;
+                const unsigned char* heads = head_rows + stage * head_bytes + ((a.D / 2 + 4 * g0) & 15) - 4 * g0;
                 uint4 w[RT][2];
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const unsigned char* row = code_rows + (i * 16 + j * 8) * 128;
-                        if constexpr (SMALL) {
-                            auto word = [&](int s) { return *reinterpret_cast<const uint32_t*>(row + (((half + s) ^ g) * 16 + t * 4)); };
+                        const unsigned char* row = codes + (i * 16 + j * 8) * 128;
+                        if constexpr (STEPS < 4) {
+                            auto word = [&](int s) { return *reinterpret_cast<const uint32_t*>(row + piece[s]); };
                             w[i][j] = make_uint4(word(0), word(1), word(2), word(3));
                         } else {
-                            w[i][j] = *reinterpret_cast<const uint4*>(row + ((half + t) ^ g) * 16);
+                            w[i][j] = *reinterpret_cast<const uint4*>(row + piece[0]);
                         }
                     }
-                float acc[RT][NT][4], sum[NT][4];
-                const int steps = SMALL ? 1 << (a.group_log2 - 5) : 4;      // per group
+                float acc[RT][NT][4];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    if (s == 0 || (SMALL && (s & (steps - 1)) == 0)) {
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                sum[n][e] = 0.0f;
-#pragma unroll
-                                for (int i = 0; i < RT; ++i) acc[i][n][e] = 0.0f;
-                            }
-                    }
+                    const bool first = s % STEPS == 0, last = s % STEPS == STEPS - 1;
                     uint32_t p[RT][2][4];
 #pragma unroll
                     for (int i = 0; i < RT; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) decode<HALF>(s == 0 ? w[i][j].x : s == 1 ? w[i][j].y : s == 2 ? w[i][j].z : w[i][j].w, p[i][j]);
+                        for (int j = 0; j < 2; ++j) decode(s == 0 ? w[i][j].x : s == 1 ? w[i][j].y : s == 2 ? w[i][j].z : w[i][j].w, p[i][j]);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        // a column that no state stands in takes another's: what comes of it is not stored
-                        const int j = n * 8 + (lane >> 2) < cols ? n * 8 + (lane >> 2) : cols - 1;
-                        uint4 b[P];
-                        if constexpr (SHARED) {
-#pragma unroll
-                            for (int q = 0; q < P; ++q) b[q] = xs[(q * words + (u * 4 + s) * 4 + t) * cols + j];
-                        } else {
-                            const int k = u * kUnit + (SMALL ? 32 * s + 8 * t : 32 * t + 8 * s);
-                            state_pairs<T>(x + j * a.x_stride + k, k < a.D, b);
-                        }
-                        constexpr uint32_t one = HALF ? 0x3c003c00u : 0x3f803f80u;
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int q = 0; q < P; ++q) {
+                            const uint4 b = *reinterpret_cast<const uint4*>(states + ((s * NT + n) * P + q) * 512 + lane * 16);
 #pragma unroll
                             for (int i = 0; i < RT; ++i) {
-                                mma<HALF>(acc[i][n], p[i][0][0], p[i][1][0], p[i][0][1], p[i][1][1], b[q].x, b[q].y);
-                                mma<HALF>(acc[i][n], p[i][0][2], p[i][1][2], p[i][0][3], p[i][1][3], b[q].z, b[q].w);
+                                if (first && q == 0) mma<true>(acc[i][n], p[i][0][0], p[i][1][0], p[i][0][1], p[i][1][1], b.x, b.y);
+                                else mma<false>(acc[i][n], p[i][0][0], p[i][1][0], p[i][0][1], p[i][1][1], b.x, b.y);
+                                mma<false>(acc[i][n], p[i][0][2], p[i][1][2], p[i][0][3], p[i][1][3], b.z, b.w);
                             }
-                            // the states' own sums, in every row of the result: rows of ones
-                            mma<HALF>(sum[n], one, one, one, one, b[q].x, b[q].y);
-                            mma<HALF>(sum[n], one, one, one, one, b[q].z, b[q].w);
                         }
-                    }
-                    if (s == 3 || (SMALL && ((s + 1) & (steps - 1)) == 0)) {
+                    if (last) {
+                        // groups behind the last have states of zero: any scale and bias will do
                         int gi = (u * kUnit + 32 * s) >> a.group_log2;
                         gi = gi < groups ? gi : groups - 1;
+                        float2 sum[NT];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) sum[n] = *reinterpret_cast<const float2*>(states + P * NT * 2048 + (s / STEPS * NT * 8 + n * 8 + 2 * t) * 4);
 #pragma unroll
                         for (int i = 0; i < RT; ++i)
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const uint32_t head = *reinterpret_cast<const uint32_t*>(head_rows + (i * 16 + j * 8) * a.head_bytes + 4 * gi);
-                                const float sc = half_bits_to_float(head & 0xffffu), bi = fmaf(8.0f, sc, half_bits_to_float(head >> 16));
+                                const __half2 head = *reinterpret_cast<const __half2*>(heads + (i * 2 + j) * row8 + 4 * gi);
+                                const float sc = __low2float(head), bi = fmaf(8.0f, sc, __high2float(head));
 #pragma unroll
-                                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e)
-                                        y[i][n][2 * j + e] = fmaf(sc, acc[i][n][2 * j + e], fmaf(bi, sum[n][e], y[i][n][2 * j + e]));
+                                for (int n = 0; n < NT; ++n) {
+                                    y[i][n][2 * j] = fmaf(sc, acc[i][n][2 * j], fmaf(bi, sum[n].x, y[i][n][2 * j]));
+                                    y[i][n][2 * j + 1] = fmaf(sc, acc[i][n][2 * j + 1], fmaf(bi, sum[n].y, y[i][n][2 * j + 1]));
+                                }
                             }
                     }
                 }
@@ -391,6 +443,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                     const float* from = red + b * depth * kPart + col * kPitch + row % (RT * 16);
                     float v = 0.0f;
                     for (int k = 0; k < depth; ++k) v += from[k * kPart];
+                    v *= __ldcg(a.back + m0 + col);
                     if (a.bias) v += load_any(a.bias, a.bias_dtype, r);
                     store_any(a.out, a.out_dtype, (m0 + col) * a.out_stride + r, v);
                 }
@@ -433,49 +486,70 @@ bool encode_rows(CUtensorMap* map, const LinearArgs& a, int box_words, int box_r
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int RT, int NT, bool SMALL, bool SHARED>
-int launch_linear(const LinearArgs& a, int64_t shared, cudaStream_t s)
+int states_per_block(int64_t m) { return m <= 8 ? 1 : 2; }      // in eights
+int pieces_of(int dtype) { return dtype == TBE_B200_FP32 ? 2 : 1; }
+int steps_of(int group_log2) { return group_log2 == 5 ? 1 : group_log2 == 6 ? 2 : 4; }
+int64_t arranged_bytes(int64_t m, int64_t D, int dtype, int group_log2)
 {
-    auto* kernel = group_row_linear_kernel<T, RT, NT, SMALL, SHARED>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
-    if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "group_row_linear: %s", cudaGetErrorString(e));
-    const int tile_rows = RT * 16 * (kWarps >> a.slices_log2);
-    CUtensorMap codes, heads;
-    if (!encode_rows(&codes, a, 32, tile_rows, true) || !encode_rows(&heads, a, a.head_bytes / 4, tile_rows, false))
-        return fail(TBE_B200_ERR_CUDA, "group_row_linear: the rows could not be described to the copy engine");
-    const int64_t blocks = a.tiles < sm_count() ? a.tiles : sm_count();
-    kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>((a.m + NT * 8 - 1) / (NT * 8))), kThreads, shared, s>>>(a, codes, heads);
-    return check_launch("group_row_linear_kernel");
+    const int NT = states_per_block(m);
+    return (m + NT * 8 - 1) / (NT * 8) * ((D + kUnit - 1) / kUnit) * unit_bytes(NT, pieces_of(dtype), steps_of(group_log2));
 }
 
-template <typename T, int RT, int NT>
+template <int RT, int NT, int P, int STEPS>
 int launch_linear(LinearArgs a, cudaStream_t s)
 {
-    const int units = (a.D + kUnit - 1) / kUnit;
+    const int units = (a.D + kUnit - 1) / kUnit, sms = sm_count();
+    const int64_t fixed = static_cast<int64_t>(kParts) * NT * 8 * (RT * 16 + 4) * 4 + 16 * kMostStages;
+    auto stage_bytes = [&](int l) {
+        return static_cast<int64_t>(kWarps) * RT * 16 * (kUnit / 2) + static_cast<int64_t>(RT * 16 * (kWarps >> l)) * head_window(a.D, 1 << l, a.group_log2) +
+               (1 << l) * unit_bytes(NT, P, STEPS);
+    };
     // Shares of the elements: as few as keep every multiprocessor at work to the end, counted in units that a warp goes
     // through (tiles per block times chunks of a tile); a tile's end is worth about one more.
     int64_t best = 0;
-    for (int l = 1; l <= 4 && (l == 1 || (1 << l) <= units); ++l) {
+    for (int l = 1; l <= 4 && (l == 1 || (1 << l) <= units) && fixed + 2 * stage_bytes(l) <= kMostShared; ++l) {
         const int64_t tiles = (a.num_rows + RT * 16 * (kWarps >> l) - 1) / (RT * 16 * (kWarps >> l));
-        const int64_t cost = ((tiles + sm_count() - 1) / sm_count()) * ((units + (1 << l) - 1) / (1 << l) + 1);
+        const int64_t cost = ((tiles + sms - 1) / sms) * ((units + (1 << l) - 1) / (1 << l) + 1);
         if (l == 1 || cost < best) {
             best = cost;
             a.slices_log2 = l;
             a.tiles = tiles;
         }
     }
-    const bool small = a.group_log2 < 7;
-    const int slices = 1 << a.slices_log2, tile_rows = RT * 16 * (kWarps >> a.slices_log2);
-    a.head_bytes = head_window(slices, a.group_log2);
-    const int64_t stage = static_cast<int64_t>(tile_rows) * (slices * (kUnit / 2) + a.head_bytes);
-    const int64_t fixed = static_cast<int64_t>(kParts) * NT * 8 * (RT * 16 + 4) * 4 + 16 * kMostStages;
-    const int64_t states = static_cast<int64_t>(a.m < NT * 8 ? a.m : NT * 8) * units * kUnit * 2 * Operand<T>::kPieces;
-    const bool shared = fixed + states + 2 * stage <= kMostShared;
-    const int64_t stages = (kMostShared - fixed - (shared ? states : 0)) / stage;
+    const int tile_rows = RT * 16 * (kWarps >> a.slices_log2);
+    a.head_bytes = head_window(a.D, 1 << a.slices_log2, a.group_log2);
+    const int64_t stages = (kMostShared - fixed) / stage_bytes(a.slices_log2);
     a.stages = static_cast<int>(stages < kMostStages ? stages : kMostStages);
-    const int64_t bytes = fixed + a.stages * stage + (shared ? states : 0);
-    if (shared) return small ? launch_linear<T, RT, NT, true, true>(a, bytes, s) : launch_linear<T, RT, NT, false, true>(a, bytes, s);
-    return small ? launch_linear<T, RT, NT, true, false>(a, bytes, s) : launch_linear<T, RT, NT, false, false>(a, bytes, s);
+    const int64_t shared = fixed + a.stages * stage_bytes(a.slices_log2);
+    CUtensorMap codes, heads;
+    if (!encode_rows(&codes, a, 32, tile_rows, true) || !encode_rows(&heads, a, a.head_bytes / 4, tile_rows, false))
+        return fail(TBE_B200_ERR_CUDA, "group_row_linear: the rows could not be described to the copy engine");
+    auto* kernel = group_row_linear_kernel<RT, NT, P, STEPS>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
+    if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "group_row_linear: %s", cudaGetErrorString(e));
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(a.tiles < sms ? a.tiles : sms), static_cast<unsigned>((a.m + NT * 8 - 1) / (NT * 8)));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = shared;
+    config.stream = s;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    e = cudaLaunchKernelEx(&config, kernel, a, codes, heads);
+    if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "group_row_linear_kernel: %s", cudaGetErrorString(e));
+    return check_launch("group_row_linear_kernel");
+}
+
+template <int RT, int NT, int P>
+int launch_linear(const LinearArgs& a, cudaStream_t s)
+{
+    switch (a.group_log2) {
+        case 5: return launch_linear<RT, NT, P, 1>(a, s);
+        case 6: return launch_linear<RT, NT, P, 2>(a, s);
+        default: return launch_linear<RT, NT, P, 4>(a, s);
+    }
 }
 
 }  // namespace
@@ -483,9 +557,17 @@ int launch_linear(LinearArgs a, cudaStream_t s)
 
 using namespace tbe;
 
+extern "C" int64_t tbe_b200_group_row_linear_scratch_bytes(int64_t m, int64_t D, int32_t group_size, int32_t input_dtype)
+{
+    const int group_log2 = group_log2_of(group_size);
+    if (m < 0 || m > (1 << 19) || D < 1 || D > (1 << 20) || group_log2 < 0 || !element_bytes(input_dtype)) return -1;
+    return arranged_bytes(m, D, input_dtype, group_log2) + (4 * m + 15) / 16 * 16;
+}
+
 extern "C" int tbe_b200_group_row_linear(const void* input, int32_t input_dtype, int64_t input_stride, int64_t m, const uint8_t* rows,
                                          int64_t num_rows, int64_t row_bytes, int64_t D, int32_t group_size, const void* bias, int32_t bias_dtype,
-                                         void* output, int32_t output_dtype, int64_t output_stride, int32_t* error_flag, tbe_b200_stream_t stream)
+                                         void* output, int32_t output_dtype, int64_t output_stride, int32_t* error_flag, void* scratch,
+                                         int64_t scratch_bytes, tbe_b200_stream_t stream)
 {
     const int ib = element_bytes(input_dtype), ob = element_bytes(output_dtype);
     if (!ib || !ob || (bias && !element_bytes(bias_dtype))) return fail(TBE_B200_ERR_UNSUPPORTED, "group_row_linear: element types FP32, FP16 and BF16");
@@ -498,13 +580,26 @@ extern "C" int tbe_b200_group_row_linear(const void* input, int32_t input_dtype,
     if (!input || !rows || !output) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "group_row_linear: NULL pointer");
     if (!rows_aligned(input, input_stride, ib, 8)) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "group_row_linear: input rows must be 16-byte aligned");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    LinearArgs a{input, input_stride, m, rows, num_rows, row_bytes, static_cast<int>(D), group_log2_of(group_size), bias, bias_dtype, output_dtype,
-                 output, output_stride, error_flag, 0, 0, 0, 0};
-    return with_element(input_dtype, [&](auto* ti) {
+    const int group_log2 = group_log2_of(group_size), NT = states_per_block(m), steps = steps_of(group_log2);
+    const int64_t need = tbe_b200_group_row_linear_scratch_bytes(m, D, group_size, input_dtype), arranged = arranged_bytes(m, D, input_dtype, group_log2);
+    if (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15))
+        return fail(TBE_B200_ERR_INVALID_ARGUMENT, "group_row_linear: scratch must be %lld bytes, 16-byte aligned", (long long)need);
+    unsigned char* states = static_cast<unsigned char*>(scratch);
+    float* back = reinterpret_cast<float*>(states + arranged);
+    const int rc = with_element(input_dtype, [&](auto* ti) {
         using T = std::remove_pointer_t<decltype(ti)>;
-        // Rows 32 to a warp use every state twice; 16 where that leaves multiprocessors without any.
-        const bool many = num_rows >= static_cast<int64_t>(64) * sm_count();
-        if (m <= 8) return many ? launch_linear<T, 2, 1>(a, s) : launch_linear<T, 1, 1>(a, s);
-        return many ? launch_linear<T, 2, 2>(a, s) : launch_linear<T, 1, 2>(a, s);
+        arrange_states_kernel<T><<<static_cast<unsigned>(m), kStateThreads, 0, s>>>(static_cast<const T*>(input), input_stride, static_cast<int>(D), NT, steps, states, back);
+        return check_launch("arrange_states_kernel");
     });
+    if (rc) return rc;
+    const LinearArgs a{states, back, m, rows, num_rows, row_bytes, static_cast<int>(D), group_log2, bias, bias_dtype, output_dtype, output, output_stride,
+                       error_flag, 0, 0, 0, 0};
+    // Rows 32 to a warp use every state twice; 16 where that leaves multiprocessors without any.
+    const bool many = num_rows >= static_cast<int64_t>(64) * sm_count();
+    if (pieces_of(input_dtype) == 1) {
+        if (NT == 1) return many ? launch_linear<2, 1, 1>(a, s) : launch_linear<1, 1, 1>(a, s);
+        return many ? launch_linear<2, 2, 1>(a, s) : launch_linear<1, 2, 1>(a, s);
+    }
+    if (NT == 1) return many ? launch_linear<2, 1, 2>(a, s) : launch_linear<1, 1, 2>(a, s);
+    return many ? launch_linear<2, 2, 2>(a, s) : launch_linear<1, 2, 2>(a, s);
 }

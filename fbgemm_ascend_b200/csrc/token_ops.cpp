@@ -349,9 +349,13 @@ Tensor group_row_linear(const Tensor& input, const Tensor& rows, int64_t group_s
     std::vector<int64_t> shape = input.sizes().vec();
     shape.back() = N;
     Tensor out = at::empty(shape, x.options().dtype(type));
+    if (m == 0 || N == 0) return out;
+    const int64_t need = tbe_b200_group_row_linear_scratch_bytes(m, D, static_cast<int32_t>(group_size), it);
+    TORCH_CHECK(need >= 0, op, ": at most 2^19 vectors of at most 2^20 elements");
+    Tensor scratch = at::empty({need}, x.options().dtype(at::kByte));
     check_status(tbe_b200_group_row_linear(x.data_ptr(), it, row_stride(x), m, r.data_ptr<uint8_t>(), N, r.size(1), D, static_cast<int32_t>(group_size),
                                            b.defined() ? b.data_ptr() : nullptr, b.defined() ? element_type(b, op, "bias") : 0, out.data_ptr(),
-                                           static_cast<int32_t>(out_type), N, nullptr, current_stream()), op);
+                                           static_cast<int32_t>(out_type), N, nullptr, scratch.data_ptr(), need, current_stream()), op);
     return out;
 }
 

@@ -54,11 +54,15 @@ def _refusals():
     assert look(n=0) == 0
 
     lin = lambda **k: lib.tbe_b200_group_row_linear(k.get("x", one), k.get("it", FP32), k.get("xs", 8), k.get("m", 1), k.get("rows", one), 4, 16,
-                                                    k.get("D", 8), 32, k.get("bias"), k.get("bt", FP32), k.get("out", one), FP32, k.get("os", 4), None, None)
+                                                    k.get("D", 8), 32, k.get("bias"), k.get("bt", FP32), k.get("out", one), FP32, k.get("os", 4), None,
+                                                    k.get("scratch", one), k.get("bytes", 1 << 30), None)
     assert lin(it=INT8) == -2 and lin(bias=one, bt=INT8) == -2 and lin(os=3) == -1 and lin(xs=4) == -1 and lin(D=0) == -1 and lin(m=-1) == -1
     assert lin(x=None) == -1 and lin(out=None) == -1
     assert lin(x=8) == -1 and "aligned" in cabi.last_error()
     assert lin(m=2, xs=9) == -1 and lin(m=0) == 0
+    need = lib.tbe_b200_group_row_linear_scratch_bytes
+    assert need(1, 8, 32, FP32) > 0 and need(-1, 8, 32, FP32) == -1 and need(1, 0, 32, FP32) == -1 and need(1, 8, 48, FP32) == -1 and need(1, 8, 32, INT8) == -1
+    assert lin(scratch=None) == -1 and lin(scratch=8) == -1 and lin(bytes=need(1, 8, 32, FP32) - 1) == -1 and "scratch" in cabi.last_error()
 
 
 def test_no_cpu_path():
