@@ -8,6 +8,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <cstdlib>
 
 #include "tbe_elements.cuh"
 
@@ -18,9 +19,11 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 16;
 constexpr int kWorkers = 32 * kWarps;
 constexpr int kThreads = kWorkers + 32;
-constexpr int kParts = kWarps / 2;              // warps whose sums lie in shared memory at a time
 constexpr int kMostStages = 4;
 constexpr int kUnit = 128;                      // elements of a row that a warp takes at once: 16 bytes to each of four lanes
+constexpr int kBoxUnits = 2;                    // the 128 bytes of a row of a box
+// Units that a warp takes between two barriers: its share of a stage is 4096 codes either way.
+__host__ __device__ constexpr int units_at_once(int RT) { return 2 / RT; }
 constexpr int kMostShared = 227 * 1024;
 
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i)
@@ -208,12 +211,12 @@ __device__ __forceinline__ void bulk_copy(uint32_t to, const void* from, uint32_
 }
 __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
-// Bytes of a row's scales and biases that a chunk of `slices` (at least 2) units needs, as they are fetched: from the 16-byte
+// Bytes of a row's scales and biases that a chunk of `units` (an even number) needs, as they are fetched: from the 16-byte
 // border in front of them on, in whole 16-byte pieces, an odd number of them (so that eight rows' words lie in different
 // banks).  A chunk begins with a group, and where in 16 bytes repeats after four chunks at most.
-int head_window(int D, int slices, int group_log2)
+int head_window(int D, int units, int group_log2)
 {
-    const int bytes = 4 * (slices * kUnit >> group_log2);
+    const int step = 4 * (units * kUnit >> group_log2), bytes = step > 4 ? step : 4;
     int most = 0;
     for (int c = 0; c < 4; ++c) {
         const int pieces = ((D / 2 + c * bytes) % 16 + bytes + 15) / 16;
@@ -227,9 +230,9 @@ int head_window(int D, int slices, int group_log2)
 __device__ __forceinline__ int row_of(int g) { return (g >> 1) | ((g & 1) << 2); }
 
 // A block is kWarps warps that work and one that fetches.  A warp holds RT * 16 rows by NT * 8 states; the warps are `slices`
-// shares of the elements times `bands` groups of rows.  A stage holds a unit of 128 elements of its rows for every warp: the
-// codes of slices * 128 neighbouring elements of bands * RT * 16 rows, in boxes of 128 bytes by all rows, and one box of the
-// scales and biases of their groups.
+// shares of the elements times `bands` groups of rows.  A stage holds U units of 128 elements of its rows for every warp:
+// the codes of slices * U neighbouring units of bands * RT * 16 rows, in boxes of 128 bytes by all rows, one box of the scales
+// and biases of their groups, and the states' elements.
 //
 // In a unit lane (g, t) = (lane / 4, lane % 4) takes two rows of every 16.  One matrix instruction takes 4 elements of each lane,
 // and one group: where a group is at least a unit, lane t takes elements 32 t .. 32 t + 31 with one 16-byte load; small
@@ -242,20 +245,20 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
 {
     constexpr int kPitch = RT * 16 + 4;         // of a state's sums in shared memory: a warp's stores meet no bank twice
     constexpr int kPart = NT * 8 * kPitch;      // one warp's sums
-    constexpr int kStates = unit_bytes(NT, P, STEPS);
+    constexpr int U = units_at_once(RT), kStates = unit_bytes(NT, P, STEPS), kCodeBytes = kWarps * RT * 16 * U * (kUnit / 2);
+    constexpr int kBuffers = NT == 1 ? 2 : 1;   // of the warps' sums
     extern __shared__ __align__(1024) unsigned char smem[];
     const int bands = kWarps >> a.slices_log2, slices = 1 << a.slices_log2, tile_rows = bands * RT * 16;
-    constexpr int kCodeBytes = kWarps * RT * 16 * (kUnit / 2);
-    const int head_bytes = tile_rows * a.head_bytes;
+    const int head_bytes = tile_rows * a.head_bytes, state_bytes = slices * U * kStates;
     // boxes of codes first (1024-byte aligned), then those of heads, the states, sums, barriers
     unsigned char* heads_at = smem + a.stages * kCodeBytes;
     unsigned char* states_at = heads_at + a.stages * head_bytes;
-    float* red = reinterpret_cast<float*>(states_at + a.stages * slices * kStates);
-    const uint32_t full = shared_address(red + kParts * kPart), empty = full + 8 * kMostStages;
+    float* red = reinterpret_cast<float*>(states_at + a.stages * state_bytes);
+    const uint32_t full = shared_address(red + kBuffers * kWarps * kPart), empty = full + 8 * kMostStages;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int units = (a.D + kUnit - 1) / kUnit, groups = (a.D + (1 << a.group_log2) - 1) >> a.group_log2;
-    const int chunks = (units + slices - 1) >> a.slices_log2;
+    const int chunks = (units + U * slices - 1) / (U * slices);
     const int64_t m0 = static_cast<int64_t>(blockIdx.y) * (NT * 8);
     const int cols = static_cast<int>(a.m - m0 < NT * 8 ? a.m - m0 : NT * 8);
 
@@ -280,20 +283,20 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                 tile += gridDim.x;
             }
         };
-        auto states_of = [&](int c) { return (units - (c << a.slices_log2) < slices ? units - (c << a.slices_log2) : slices) * kStates; };
+        auto states_of = [&](int c) { return (units - c * U * slices < U * slices ? units - c * U * slices : U * slices) * kStates; };
         auto fetch_rows = [&](int stage) {
             const uint32_t bar = full + 8 * stage;
             const int first = static_cast<int>(tile * tile_rows);
             barrier_expect(bar, kCodeBytes + head_bytes + states_of(chunk));
             // what lies outside the matrix arrives as zeros
-            for (int k = 0; k < slices / 2; ++k)
-                box_copy(shared_address(smem + stage * kCodeBytes + k * (tile_rows * 128)), &code_map, (chunk * (slices / 2) + k) * 32, first, bar);
-            const int g0 = (chunk * slices * kUnit) >> a.group_log2;
+            const int boxes = slices * U / kBoxUnits;
+            for (int k = 0; k < boxes; ++k)
+                box_copy(shared_address(smem + stage * kCodeBytes + k * (tile_rows * 128)), &code_map, (chunk * boxes + k) * 32, first, bar);
+            const int g0 = (chunk * slices * U * kUnit) >> a.group_log2;
             box_copy(shared_address(heads_at + stage * head_bytes), &head_map, ((a.D / 2 + 4 * g0) & ~15) / 4, first, bar);
         };
         auto fetch_states = [&](int stage) {
-            bulk_copy(shared_address(states_at + stage * slices * kStates), arranged + static_cast<int64_t>(chunk << a.slices_log2) * kStates, states_of(chunk),
-                      full + 8 * stage);
+            bulk_copy(shared_address(states_at + stage * state_bytes), arranged + static_cast<int64_t>(chunk) * state_bytes, states_of(chunk), full + 8 * stage);
         };
         // The first stages' rows are on their way before the states are ready.
         int filled = 0;
@@ -338,24 +341,25 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
             for (int e = 0; e < 4; ++e) y[i][n][e] = 0.0f;
 
     // this lane's places in a stage
-    const unsigned char* code_rows = smem + (slice >> 1) * (tile_rows * 128) + (band * RT * 16 + g) * 128;
-    const int half = (slice & 1) * 4, row8 = 8 * a.head_bytes;
-    int piece[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) piece[k] = STEPS < 4 ? ((half + k) ^ g) * 16 + t * 4 : ((half + t) ^ g) * 16;
+    const unsigned char* code_rows = smem + slice * U / kBoxUnits * (tile_rows * 128) + (band * RT * 16 + g) * 128;
+    const int half = U == 1 ? slice & 1 : 0;
+    const int row8 = 8 * a.head_bytes;
     const unsigned char* head_rows = heads_at + (band * RT * 16 + g) * a.head_bytes;
-    const unsigned char* my_states = states_at + slice * kStates;
+    const unsigned char* my_states = states_at + slice * U * kStates;
+    int buffer = 0;
     int stage = 0;
     uint32_t round = 0;
     for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
         for (int c = 0; c < chunks; ++c) {
             if (!barrier_wait(full + 8 * stage, round & 1) && a.error_flag) atomicOr(a.error_flag, 16);
-            const int u = (c << a.slices_log2) + slice;
-            if (u < units) {
-                const unsigned char* codes = code_rows + stage * kCodeBytes;
-                const unsigned char* states = my_states + stage * slices * kStates;
-                const int g0 = (c * slices * kUnit) >> a.group_log2;
-                const unsigned char* heads = head_rows + stage * head_bytes + ((a.D / 2 + 4 * g0) & 15) - 4 * g0;
+            const int g0 = (c * slices * U * kUnit) >> a.group_log2;
+            const unsigned char* heads = head_rows + stage * head_bytes + ((a.D / 2 + 4 * g0) & 15) - 4 * g0;
+            const unsigned char* codes = code_rows + stage * kCodeBytes;
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int u = U * (c * slices + slice) + k;
+                if (u >= units) break;
+                const unsigned char* states = my_states + stage * state_bytes + k * kStates;
                 uint4 w[RT][2];
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
@@ -363,10 +367,10 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                     for (int j = 0; j < 2; ++j) {
                         const unsigned char* row = codes + (i * 16 + j * 8) * 128;
                         if constexpr (STEPS < 4) {
-                            auto word = [&](int s) { return *reinterpret_cast<const uint32_t*>(row + piece[s]); };
+                            auto word = [&](int s) { return *reinterpret_cast<const uint32_t*>(row + ((((k + half) * 4 + s) ^ g) * 16 + t * 4)); };
                             w[i][j] = make_uint4(word(0), word(1), word(2), word(3));
                         } else {
-                            w[i][j] = *reinterpret_cast<const uint4*>(row + piece[0]);
+                            w[i][j] = *reinterpret_cast<const uint4*>(row + (((k + half) * 4 + t) ^ g) * 16);
                         }
                     }
                 float acc[RT][NT][4];
@@ -419,52 +423,34 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                 ++round;
             }
         }
-        // The tile's end: the slices' sums are added in their order, half the warps' at a time.
-        const int fold = a.slices_log2 == 4 ? 1 : 0;      // all warps share one band: the upper half is added to the lower first
-        for (int half = 0; half < 2; ++half) {
-            const bool give = fold ? (half == 0) == (warp >= kParts) : (warp / kParts) == half;
-            if (give) {
-                float* part = red + (warp % kParts) * kPart;
-#pragma unroll
-                for (int i = 0; i < RT; ++i)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) part[(n * 8 + 2 * t + (e & 1)) * kPitch + i * 16 + (e >> 1) * 8 + g] = y[i][n][e];
-            }
-            workers_sync();
-            if (fold && half == 0) {
-                if (warp < kParts) {
-                    const float* part = red + warp * kPart;
-#pragma unroll
-                    for (int i = 0; i < RT; ++i)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) y[i][n][e] += part[(n * 8 + 2 * t + (e & 1)) * kPitch + i * 16 + (e >> 1) * 8 + g];
-                }
-            } else {
-                const int depth = fold ? kParts : slices, here = fold ? tile_rows : tile_rows / 2, from_row = fold ? 0 : half * here;
-                for (int i = threadIdx.x; i < here * cols; i += kWorkers) {
-                    const int col = i / here, row = i - col * here, b = row / (RT * 16);
-                    const int64_t r = tile * tile_rows + from_row + row;
-                    if (r >= a.num_rows) continue;
-                    const float* from = red + b * depth * kPart + col * kPitch + row % (RT * 16);
-                    float v = 0.0f;
-                    for (int k = 0; k < depth; ++k) v += from[k * kPart];
-                    v *= __ldcg(a.back + m0 + col);
-                    if (a.bias) v += load_any(a.bias, a.bias_dtype, r);
-                    store_any(a.out, a.out_dtype, (m0 + col) * a.out_stride + r, v);
-                }
-            }
-            workers_sync();
-        }
+        // The tile's end: the slices' sums are added in their order.
+        float* sums = red + buffer * (kWarps * kPart);
+        float* part = sums + warp * kPart;
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[i][n][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) {
+                    part[(n * 8 + 2 * t + (e & 1)) * kPitch + i * 16 + (e >> 1) * 8 + g] = y[i][n][e];
+                    y[i][n][e] = 0.0f;
+                }
+        workers_sync();
+        const int rows_log2 = 31 - __clz(tile_rows);
+        for (int i = threadIdx.x; i < cols << rows_log2; i += kWorkers) {
+            const int col = i >> rows_log2, row = i & (tile_rows - 1);
+            const int64_t r = tile * tile_rows + row;
+            if (r >= a.num_rows) continue;
+            const float* from = sums + (row / (RT * 16) << a.slices_log2) * kPart + col * kPitch + row % (RT * 16);
+            float v = 0.0f;
+            for (int k = 0; k < slices; ++k) v += from[k * kPart];
+            v *= __ldcg(a.back + m0 + col);
+            if (a.bias) v += load_any(a.bias, a.bias_dtype, r);
+            store_any(a.out, a.out_dtype, (m0 + col) * a.out_stride + r, v);
+        }
+        // the next tile's sums go to the other buffer, where there is one: its own barrier parts the two after it
+        if (kBuffers == 1) workers_sync();
+        else buffer ^= 1;
     }
 }
 
@@ -507,26 +493,28 @@ int64_t arranged_bytes(int64_t m, int64_t D, int dtype, int group_log2)
 template <int RT, int NT, int P, int STEPS>
 int launch_linear(LinearArgs a, cudaStream_t s)
 {
-    const int units = (a.D + kUnit - 1) / kUnit, sms = sm_count();
-    const int64_t fixed = static_cast<int64_t>(kParts) * NT * 8 * (RT * 16 + 4) * 4 + 16 * kMostStages;
+    constexpr int U = units_at_once(RT);
+    const int sms = sm_count();
+    const int64_t fixed = static_cast<int64_t>(NT == 1 ? 2 : 1) * kWarps * NT * 8 * (RT * 16 + 4) * 4 + 16 * kMostStages;
     auto stage_bytes = [&](int l) {
-        return static_cast<int64_t>(kWarps) * RT * 16 * (kUnit / 2) + static_cast<int64_t>(RT * 16 * (kWarps >> l)) * head_window(a.D, 1 << l, a.group_log2) +
-               (1 << l) * unit_bytes(NT, P, STEPS);
+        return static_cast<int64_t>(kWarps) * RT * 16 * U * (kUnit / 2) + static_cast<int64_t>(RT * 16 * (kWarps >> l)) * head_window(a.D, U << l, a.group_log2) +
+               (U << l) * unit_bytes(NT, P, STEPS);
     };
-    // Shares of the elements: as few as keep every multiprocessor at work to the end, counted in units that a warp goes
-    // through (tiles per block times chunks of a tile); a tile's end is worth about one more.
+    // Shares of the elements: as few as keep every multiprocessor at work to the end, counted in units of time that
+    // a warp needs for its share of a stage; a tile's end is worth about half of one.  A box is at most 256 rows.
+    const int shares = (a.D + U * kUnit - 1) / (U * kUnit), fewest = RT - 1;
     int64_t best = 0;
-    for (int l = 1; l <= 4 && (l == 1 || (1 << l) <= units) && fixed + 2 * stage_bytes(l) <= kMostShared; ++l) {
+    for (int l = fewest; l <= 4 && (l == fewest || ((1 << l) <= shares && fixed + 2 * stage_bytes(l) <= kMostShared)); ++l) {
         const int64_t tiles = (a.num_rows + RT * 16 * (kWarps >> l) - 1) / (RT * 16 * (kWarps >> l));
-        const int64_t cost = ((tiles + sms - 1) / sms) * ((units + (1 << l) - 1) / (1 << l) + 1);
-        if (l == 1 || cost < best) {
+        const int64_t cost = ((tiles + sms - 1) / sms) * (2 * ((shares + (1 << l) - 1) / (1 << l)) + 1);
+        if (l == fewest || cost < best) {
             best = cost;
             a.slices_log2 = l;
             a.tiles = tiles;
         }
     }
     const int tile_rows = RT * 16 * (kWarps >> a.slices_log2);
-    a.head_bytes = head_window(a.D, 1 << a.slices_log2, a.group_log2);
+    a.head_bytes = head_window(a.D, U << a.slices_log2, a.group_log2);
     const int64_t stages = (kMostShared - fixed) / stage_bytes(a.slices_log2);
     a.stages = static_cast<int>(stages < kMostStages ? stages : kMostStages);
     const int64_t shared = fixed + a.stages * stage_bytes(a.slices_log2);
@@ -604,7 +592,7 @@ extern "C" int tbe_b200_group_row_linear(const void* input, int32_t input_dtype,
     const LinearArgs a{states, back, m, rows, num_rows, row_bytes, static_cast<int>(D), group_log2, bias, bias_dtype, output_dtype, output, output_stride,
                        error_flag, 0, 0, 0, 0};
     // Rows 32 to a warp use every state twice; 16 where that leaves multiprocessors without any.
-    const bool many = num_rows >= static_cast<int64_t>(64) * sm_count();
+    const bool many = getenv("RT1") ? false : num_rows >= static_cast<int64_t>(64) * sm_count();
     if (pieces_of(input_dtype) == 1) {
         if (NT == 1) return many ? launch_linear<2, 1, 1>(a, s) : launch_linear<1, 1, 1>(a, s);
         return many ? launch_linear<2, 2, 1>(a, s) : launch_linear<1, 2, 1>(a, s);
