@@ -84,29 +84,225 @@ int launch_token_embedding(const TI* weight, int64_t num_embeddings, int64_t D, 
 //
 // Keys are tokens (num_embeddings stands for one that takes no part and sorts last), values their positions.  A stable
 // radix sort from the lowest digit up keeps the positions of equal tokens in order, which fixes the order of every sum.
-// Per digit: tile histograms, one block that turns them into places (digit by digit, tile by tile), and the scatter.
-constexpr int kSortItems = 16;
-constexpr int kSortTile = kThreads * kSortItems;
+// A warp owns neighbouring keys and takes them 32 at a time: lanes with the same digit find one another, and a running
+// count per warp and digit gives each its rank.
 constexpr int kMaxBins = 512;
-constexpr int kWarps = kThreads / 32;
 
-__device__ __forceinline__ uint32_t token_key(const void* tokens, bool wide, int64_t i, int64_t num_embeddings, int64_t padding_idx)
+struct SortInput {
+    const void* tokens;
+    int wide;
+    int64_t n, num_embeddings, padding_idx;
+};
+
+__device__ __forceinline__ uint32_t token_key(const SortInput& in, int64_t i)
 {
-    const int64_t t = load_token(tokens, wide, i);
-    return static_cast<uint32_t>((t < 0 || t >= num_embeddings || t == padding_idx) ? num_embeddings : t);
+    const int64_t t = load_token(in.tokens, in.wide, i);
+    return static_cast<uint32_t>((t < 0 || t >= in.num_embeddings || t == in.padding_idx) ? in.num_embeddings : t);
 }
 
-template <bool FIRST>
-__device__ __forceinline__ uint32_t sort_key(const void* tokens, const uint32_t* keys, int wide, int64_t i, int64_t num_embeddings, int64_t padding_idx)
+// The rank of this lane's key among those of its warp with the same digit so far; `count` is the warp's.
+template <typename C>
+__device__ __forceinline__ uint32_t warp_rank(uint32_t digit, bool live, C* count)
 {
-    if constexpr (FIRST) return token_key(tokens, wide, i, num_embeddings, padding_idx);
-    else return __ldg(keys + i);
+    const int lane = threadIdx.x & 31;
+    const uint32_t peers = __match_any_sync(kFull, live ? digit : 0xffffffffu);
+    const uint32_t before = live ? count[digit] : 0u;
+    __syncwarp();
+    if (live && lane == 31 - __clz(peers)) count[digit] = static_cast<C>(before + __popc(peers));
+    __syncwarp();
+    return before + __popc(peers & ((1u << lane) - 1u));
+}
+
+// Exclusive running sum over a block of 1024 threads; `total` is everything.
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* warp_tot, uint32_t& total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t incl = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t up = __shfl_up_sync(kFull, incl, d);
+        if (lane >= d) incl += up;
+    }
+    __syncthreads();      // warp_tot may still be read from an earlier call
+    if (lane == 31) warp_tot[warp] = incl;
+    __syncthreads();
+    uint32_t w = warp_tot[lane], run = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t up = __shfl_up_sync(kFull, run, d);
+        if (lane >= d) run += up;
+    }
+    total = __shfl_sync(kFull, run, 31);
+    return __shfl_sync(kFull, run - w, warp) + incl - v;
+}
+
+// ---- up to kClusterKeys tokens: one cluster sorts in shared memory, the other blocks clear the gradient meanwhile ------
+//
+// A block of the cluster holds ITEMS * 1024 neighbouring places.  Per digit: ranks in registers, digit counts exchanged
+// between the blocks, then every key straight to its place in whichever block's shared memory that is.  Launch and
+// synchronisation are all that it costs beside the clearing: with nothing to clear, 16384 tokens of 131072 take LATER us.
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortBlocks = 8;                       // the largest cluster that every device schedules
+constexpr int kOneBlockKeys = 4 * kSortThreads;      // so many are sorted by a block alone: barriers between blocks cost more
+constexpr int kMostItems = 16;
+constexpr int64_t kClusterKeys = int64_t(kSortBlocks) * kMostItems * kSortThreads;
+
+struct FillArgs {
+    char* out;
+    int64_t rows, row_bytes, stride_bytes;      // rows == 0: nothing to clear
+};
+
+__device__ __forceinline__ void clear_run(char* p, int64_t bytes, int64_t thread, int64_t threads, int unit)
+{
+    // up to the first 16-byte border and behind the last one element by element
+    const int64_t head = min((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15, bytes), body = (bytes - head) / 16;
+    for (int64_t i = thread; i < body; i += threads) st_stream16(p + head + 16 * i, make_uint4(0u, 0u, 0u, 0u));
+    const int64_t edge = (head + (bytes - head - 16 * body)) / unit;
+    for (int64_t i = thread; i < edge; i += threads) {
+        char* q = i * unit < head ? p + i * unit : p + 16 * body + i * unit;
+        if (unit == 4) *reinterpret_cast<uint32_t*>(q) = 0u;
+        else *reinterpret_cast<unsigned short*>(q) = 0;
+    }
+}
+
+__device__ __forceinline__ void clear_rows(const FillArgs& f, int unit, int64_t block, int64_t blocks)
+{
+    if (f.stride_bytes == f.row_bytes) {
+        clear_run(f.out, f.rows * f.row_bytes, block * blockDim.x + threadIdx.x, blocks * blockDim.x, unit);
+    } else {
+        const int64_t warps = blocks * (blockDim.x / 32);
+        for (int64_t r = block * (blockDim.x / 32) + threadIdx.x / 32; r < f.rows; r += warps)
+            clear_run(f.out + r * f.stride_bytes, f.row_bytes, threadIdx.x & 31, 32, unit);
+    }
+}
+
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The address of `p` of this block's shared memory in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t shared_of(const void* p, uint32_t rank)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+    return a;
+}
+
+constexpr int64_t sort_shared_bytes(int items) { return int64_t(items) * kSortThreads * 8 + kSortWarps * kMaxBins * 2 + kSortBlocks * kMaxBins * 4 + kMaxBins * 4 + 128; }
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kSortThreads, 1)
+sort_tokens_kernel(const SortInput in, int cluster, int passes, int width, uint2* __restrict__ sorted, const FillArgs fill, int unit)
+{
+    if (blockIdx.x >= cluster) {
+        clear_rows(fill, unit, blockIdx.x - cluster, gridDim.x - cluster);
+        return;
+    }
+    constexpr int kPer = ITEMS * kSortThreads;
+    extern __shared__ __align__(16) unsigned char sort_smem[];
+    unsigned long long* buf = reinterpret_cast<unsigned long long*>(sort_smem);
+    unsigned short(*count)[kMaxBins] = reinterpret_cast<unsigned short(*)[kMaxBins]>(buf + kPer);
+    uint32_t(*table)[kMaxBins] = reinterpret_cast<uint32_t(*)[kMaxBins]>(count + kSortWarps);
+    uint32_t* base = reinterpret_cast<uint32_t*>(table + kSortBlocks);
+    uint32_t* warp_tot = base + kMaxBins;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << width;
+    const uint32_t mine = cluster > 1 ? cluster_rank() : 0u;
+    const int64_t first = static_cast<int64_t>(mine) * kPer;
+    const int at = warp * (32 * ITEMS) + lane;
+    auto sync_all = [&] {
+        if (cluster > 1) cluster_sync();
+        else __syncthreads();
+    };
+    if (cluster > 1) cluster_sync();      // every block has begun: its shared memory may be written
+    for (int p = 0; p < passes; ++p) {
+        uint32_t key[ITEMS], pos[ITEMS], rank[ITEMS];
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            const int64_t i = first + at + j * 32;
+            key[j] = pos[j] = 0u;
+            if (i < in.n) {
+                if (p == 0) {
+                    key[j] = token_key(in, i);
+                    pos[j] = static_cast<uint32_t>(i);
+                } else {
+                    const unsigned long long both = buf[at + j * 32];
+                    key[j] = static_cast<uint32_t>(both >> 32);
+                    pos[j] = static_cast<uint32_t>(both);
+                }
+            }
+        }
+        for (int b = threadIdx.x; b < kSortWarps * kMaxBins / 2; b += kSortThreads) reinterpret_cast<uint32_t*>(count)[b] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) rank[j] = warp_rank((key[j] >> (p * width)) & (bins - 1), first + at + j * 32 < in.n, count[warp]);
+        __syncthreads();
+        if (threadIdx.x < bins) {
+            uint32_t run = 0;
+#pragma unroll 8
+            for (int w = 0; w < kSortWarps; ++w) {
+                const uint32_t c = count[w][threadIdx.x];
+                count[w][threadIdx.x] = static_cast<unsigned short>(run);
+                run += c;
+            }
+            if (cluster > 1) {
+                for (int r = 0; r < cluster; ++r)
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(shared_of(&table[mine][threadIdx.x], r)), "r"(run) : "memory");
+            } else {
+                table[0][threadIdx.x] = run;
+            }
+        }
+        sync_all();      // every block's counts are here, and every block holds its keys in registers
+        uint32_t all = 0, below = 0, total;
+        if (threadIdx.x < bins)
+            for (int r = 0; r < cluster; ++r) {
+                const uint32_t c = table[r][threadIdx.x];
+                all += c;
+                if (r < mine) below += c;
+            }
+        const uint32_t before = block_exclusive(all, warp_tot, total);
+        if (threadIdx.x < bins) base[threadIdx.x] = before + below;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            if (first + at + j * 32 >= in.n) continue;
+            const uint32_t d = (key[j] >> (p * width)) & (bins - 1), to = base[d] + count[warp][d] + rank[j];
+            const unsigned long long both = (static_cast<unsigned long long>(key[j]) << 32) | pos[j];
+            if (cluster > 1)
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(shared_of(buf + to % kPer, to / kPer)), "l"(both) : "memory");
+            else
+                buf[to] = both;
+        }
+        sync_all();
+    }
+    for (int i = threadIdx.x; i < kPer && first + i < in.n; i += kSortThreads) {
+        const unsigned long long both = buf[i];
+        sorted[first + i] = make_uint2(static_cast<uint32_t>(both >> 32), static_cast<uint32_t>(both));
+    }
+}
+
+// ---- more tokens than a cluster holds: per digit tile histograms, one block that turns them into places (digit by digit,
+// tile by tile), and the scatter ----------------------------------------------------------------------------------
+constexpr int kWarps = kThreads / 32;
+constexpr int kSortItems = 16;
+constexpr int kSortTile = kThreads * kSortItems;
+
+template <bool FIRST>
+__device__ __forceinline__ uint2 sort_entry(const SortInput& in, const uint2* from, int64_t i)
+{
+    if constexpr (FIRST) return make_uint2(token_key(in, i), static_cast<uint32_t>(i));
+    else return __ldg(from + i);
 }
 
 template <bool FIRST>
 __global__ void __launch_bounds__(kThreads)
-sort_histogram_kernel(const void* __restrict__ tokens, const uint32_t* __restrict__ keys, int wide, int64_t n, int64_t num_embeddings,
-                      int64_t padding_idx, int shift, int bins, uint32_t* __restrict__ hist)
+sort_histogram_kernel(const SortInput in, const uint2* __restrict__ from, int shift, int bins, uint32_t* __restrict__ hist)
 {
     __shared__ uint32_t count[kMaxBins];
     for (int b = threadIdx.x; b < bins; b += kThreads) count[b] = 0;
@@ -115,7 +311,7 @@ sort_histogram_kernel(const void* __restrict__ tokens, const uint32_t* __restric
 #pragma unroll 4
     for (int j = 0; j < kSortItems; ++j) {
         const int64_t i = base + j * kThreads + threadIdx.x;
-        if (i < n) atomicAdd(&count[(sort_key<FIRST>(tokens, keys, wide, i, num_embeddings, padding_idx) >> shift) & (bins - 1)], 1u);
+        if (i < in.n) atomicAdd(&count[(sort_entry<FIRST>(in, from, i).x >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += kThreads) hist[static_cast<int64_t>(b) * gridDim.x + blockIdx.x] = count[b];
@@ -125,69 +321,43 @@ sort_histogram_kernel(const void* __restrict__ tokens, const uint32_t* __restric
 __global__ void __launch_bounds__(1024) sort_places_kernel(uint32_t* __restrict__ hist, int64_t count)
 {
     __shared__ uint32_t warp_tot[32];
-    __shared__ uint32_t total;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t carry = 0;
     for (int64_t base = 0; base < count; base += 4096) {
         const int64_t first = base + threadIdx.x * 4;
-        uint32_t v[4], mine = 0;
+        uint32_t v[4], mine = 0, total;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             v[j] = first + j < count ? hist[first + j] : 0u;
             mine += v[j];
         }
-        uint32_t incl = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t up = __shfl_up_sync(kFull, incl, d);
-            if (lane >= d) incl += up;
-        }
-        __syncthreads();
-        if (lane == 31) warp_tot[warp] = incl;
-        __syncthreads();
-        uint32_t run = carry + incl - mine;
-        for (int w = 0; w < warp; ++w) run += warp_tot[w];
-        if (threadIdx.x == 1023) total = run + mine;
+        uint32_t run = carry + block_exclusive(mine, warp_tot, total);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (first + j < count) hist[first + j] = run;
             run += v[j];
         }
-        __syncthreads();
-        carry = total;
+        carry += total;
     }
 }
 
-// A warp owns 32 * kSortItems consecutive keys of the tile and takes them 32 at a time: lanes with the same digit find
-// one another, and a running count per warp and digit gives each its rank.
 template <bool FIRST>
 __global__ void __launch_bounds__(kThreads)
-sort_scatter_kernel(const void* __restrict__ tokens, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int wide, int64_t n,
-                    int64_t num_embeddings, int64_t padding_idx, int shift, int bins, const uint32_t* __restrict__ places,
-                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out)
+sort_scatter_kernel(const SortInput in, const uint2* __restrict__ from, int shift, int bins, const uint32_t* __restrict__ places, uint2* __restrict__ to)
 {
     __shared__ uint32_t count[kWarps][kMaxBins];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int b = threadIdx.x; b < kWarps * bins; b += kThreads) count[b / bins][b % bins] = 0;
+    for (int b = threadIdx.x; b < kWarps * kMaxBins; b += kThreads) (&count[0][0])[b] = 0;
     __syncthreads();
     const int64_t base = static_cast<int64_t>(blockIdx.x) * kSortTile + warp * (32 * kSortItems) + lane;
-    uint32_t key[kSortItems], rank[kSortItems];
+    uint2 entry[kSortItems];
+    uint32_t rank[kSortItems];
 #pragma unroll
     for (int j = 0; j < kSortItems; ++j) {
         const int64_t i = base + j * 32;
-        key[j] = i < n ? sort_key<FIRST>(tokens, keys, wide, i, num_embeddings, padding_idx) : 0u;
+        entry[j] = i < in.n ? sort_entry<FIRST>(in, from, i) : make_uint2(0u, 0u);
     }
 #pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
-        const bool live = base + j * 32 < n;
-        const uint32_t d = live ? (key[j] >> shift) & (bins - 1) : static_cast<uint32_t>(bins);
-        const uint32_t peers = __match_any_sync(kFull, d);
-        const uint32_t before = live ? count[warp][d] : 0u;
-        __syncwarp();
-        if (live && lane == 31 - __clz(peers)) count[warp][d] = before + __popc(peers);
-        __syncwarp();
-        rank[j] = before + __popc(peers & ((1u << lane) - 1u));
-    }
+    for (int j = 0; j < kSortItems; ++j) rank[j] = warp_rank((entry[j].x >> shift) & (bins - 1), base + j * 32 < in.n, count[warp]);
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += kThreads) {
         uint32_t run = places[static_cast<int64_t>(b) * gridDim.x + blockIdx.x];
@@ -199,133 +369,341 @@ sort_scatter_kernel(const void* __restrict__ tokens, const uint32_t* __restrict_
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
-        const int64_t i = base + j * 32;
-        if (i >= n) continue;
-        const uint32_t at = count[warp][(key[j] >> shift) & (bins - 1)] + rank[j];
-        keys_out[at] = key[j];
-        vals_out[at] = FIRST ? static_cast<uint32_t>(i) : __ldg(vals + i);
-    }
+    for (int j = 0; j < kSortItems; ++j)
+        if (base + j * 32 < in.n) to[count[warp][(entry[j].x >> shift) & (bins - 1)] + rank[j]] = entry[j];
 }
+
+__global__ void __launch_bounds__(kThreads) clear_rows_kernel(const FillArgs fill, int unit) { clear_rows(fill, unit, blockIdx.x, gridDim.x); }
 
 // ---- gradient: sums ---------------------------------------------------------------------------------------------
 //
-// The sorted positions are cut into tiles of kTileRows; a warp walks a tile over 32 * VEC columns and writes a row when its
-// token ends.  A token that goes on past the tile leaves its piece in `parts`: slot 0 of a tile holds the sum of the token
-// that came in from the tile before (the whole tile, if it goes on), slot 1 that of one that starts here and goes on.
-// join_parts_kernel adds the pieces in the order of the tiles.
-constexpr int kTileRows = 32;
+// The sorted positions are cut into tiles; a group of lanes (a warp where rows are wide) walks a tile over eight columns per
+// lane and writes a row when its token ends.  A token that goes on past the tile leaves its piece in `parts`: slot 0 of a
+// tile holds the sum of the token that came in from the tile before (the whole tile, if it goes on), slot 1 that of one that
+// starts here and goes on.  join_parts_kernel adds the pieces in the order of the tiles.
+constexpr int kColumns = 8;                 // per lane
+constexpr int kAhead = 4;                   // rows whose loads are in flight together
 
-template <typename TO, int VEC>
-__device__ __forceinline__ void write_sum(TO* out, float (&acc)[VEC], float scale, int accumulate)
-{
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] *= scale;
-    if (accumulate) {
-        Piece<TO, VEC> old;
-        load_piece<TO, VEC, false>(old, out);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += element(old, e);
-    }
-    store_piece<TO, VEC>(out, acc);
-}
+struct SumArgs {
+    const uint2* sorted;
+    int64_t n;
+    uint32_t none;
+    int64_t grad_stride, out_stride;
+    int D, padded_D;                        // padded_D: of a row of `parts`
+    int tile_rows, slices, lanes_log2;      // slices: of a row, lanes * 8 columns each
+    int64_t tiles;
+    float scale;
+    float* parts;
+};
 
-template <typename TI, typename TO, int VEC>
-__global__ void __launch_bounds__(kThreads)
-sum_tiles_kernel(const TI* __restrict__ grad, int64_t grad_stride, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int64_t n,
-                 uint32_t none, int64_t pieces, float scale, int accumulate, TO* out, int64_t out_stride, float* __restrict__ parts)
-{
-    const int lane = threadIdx.x & 31;
-    const int64_t tile = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    const int64_t c = static_cast<int64_t>(blockIdx.y) * 32 + lane;
-    const int64_t first = tile * kTileRows;
-    if (first >= n || c >= pieces) return;
-    const int rows = static_cast<int>(n - first < kTileRows ? n - first : kTileRows);
-    const int64_t D = pieces * VEC;
-    uint32_t cur = __ldg(keys + first);
-    const bool came_in = first > 0 && __ldg(keys + first - 1) == cur;
-    bool head = came_in;
-    float acc[VEC];
+// How a lane's eight columns lie: VEC neighbouring ones at a time, `lanes` pieces apart.  VEC 1 and 2 stand for rows that are not
+// aligned; two 16-bit elements then come out of the one or two words that hold them.
+template <typename T, int VEC>
+struct Columns {
+    static constexpr int kPieces = kColumns / VEC;
+    Piece<T, VEC> p[kPieces];
+
+    __device__ __forceinline__ void load(const T* row, int column, int step, int D)
+    {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
-    for (int r = 0; r < rows; ++r) {
-        const uint32_t key = __ldg(keys + first + r);
-        if (key != cur) {
-            if (head) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) parts[(tile * 2) * D + c * VEC + e] = acc[e];
+        for (int i = 0; i < kPieces; ++i) {
+            const int c = column + i * step;
+            if constexpr (VEC == 2 && sizeof(T) == 2) {
+                // Words are aligned, rows need not be: a word that holds one element of the row holds nothing foreign that is used.
+                const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
+                uint32_t v = 0;
+                if (c < D) {
+                    v = __ldg(w);
+                    if (a & 2) v = __funnelshift_r(v, c + 1 < D ? __ldg(w + 1) : 0u, 16);
+                    else if (c + 1 >= D) v &= 0xffffu;
+                }
+                p[i].w[0] = v;
+            } else if (c < D) {
+                load_piece<T, VEC>(p[i], row + c);
             } else {
-                write_sum<TO, VEC>(out + static_cast<int64_t>(cur) * out_stride + c * VEC, acc, scale, accumulate);
+                clear_piece(p[i]);
             }
-            head = false;
-            cur = key;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
         }
-        if (cur == none) return;      // they sort last
-        Piece<TI, VEC> p;
-        load_piece<TI, VEC>(p, grad + static_cast<int64_t>(__ldg(vals + first + r)) * grad_stride + c * VEC);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += element(p, e);
     }
-    const bool goes_on = first + rows < n && __ldg(keys + first + rows) == cur;
-    if (head || goes_on) {
-        const int64_t slot = tile * 2 + (head ? 0 : 1);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) parts[slot * D + c * VEC + e] = acc[e];
-    } else {
-        write_sum<TO, VEC>(out + static_cast<int64_t>(cur) * out_stride + c * VEC, acc, scale, accumulate);
-    }
-}
+    __device__ __forceinline__ float at(int e) const { return element(p[e / VEC], e % VEC); }
+};
 
-// A token that starts in tile t and goes on: its piece in slot 1 of t and slot 0 of the tiles that it reaches.
-template <typename TO>
-__global__ void __launch_bounds__(kThreads)
-join_parts_kernel(const uint32_t* __restrict__ keys, int64_t n, uint32_t none, int64_t D, float scale, int accumulate, TO* out, int64_t out_stride,
-                  const float* __restrict__ parts)
+template <typename TO, int VEC>
+__device__ __forceinline__ void load_row(float (&v)[kColumns], const TO* row, int column, int step, int D)
 {
-    const int64_t tile = blockIdx.x, first = tile * kTileRows, next = first + kTileRows;
-    if (next >= n) return;
-    const uint32_t cur = __ldg(keys + next - 1);
-    if (cur == none || __ldg(keys + next) != cur) return;
-    if (__ldg(keys + first) == cur && first > 0 && __ldg(keys + first - 1) == cur) return;      // came in: another tile's
-    const int64_t c = static_cast<int64_t>(blockIdx.y) * kThreads + threadIdx.x;
-    if (c >= D) return;
-    float sum[1] = {parts[(tile * 2 + 1) * D + c]};
-    for (int64_t t = tile + 1; t * kTileRows < n && __ldg(keys + t * kTileRows) == cur; ++t) sum[0] += parts[(t * 2) * D + c];
-    write_sum<TO, 1>(out + static_cast<int64_t>(cur) * out_stride + c, sum, scale, accumulate);
+    constexpr int kOne = VEC == 2 ? 1 : VEC;      // rows of VEC 2 are not aligned
+#pragma unroll
+    for (int i = 0; i < kColumns / kOne; ++i) {
+        const int c = column + (i * kOne / VEC) * step + (i * kOne) % VEC;
+        Piece<TO, kOne> p;
+        if (c < D) load_piece<TO, kOne, false>(p, row + c);
+        else clear_piece(p);
+#pragma unroll
+        for (int e = 0; e < kOne; ++e) v[i * kOne + e] = element(p, e);
+    }
 }
 
 template <typename TO, int VEC>
-__global__ void __launch_bounds__(kThreads) zero_rows_kernel(TO* __restrict__ out, int64_t rows, int64_t pieces, int64_t stride)
+__device__ __forceinline__ void store_row(TO* row, const float (&v)[kColumns], int column, int step, int D)
 {
-    const float zero[VEC] = {};
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < rows * pieces; i += step)
-        store_piece<TO, VEC>(out + (i / pieces) * stride + (i % pieces) * VEC, zero);
+    constexpr int kOne = VEC == 2 ? 1 : VEC;
+#pragma unroll
+    for (int i = 0; i < kColumns / kOne; ++i) {
+        const int c = column + (i * kOne / VEC) * step + (i * kOne) % VEC;
+        float one[kOne];
+#pragma unroll
+        for (int e = 0; e < kOne; ++e) one[e] = v[i * kOne + e];
+        if (c < D) store_piece<TO, kOne>(row + c, one);
+    }
+}
+
+template <typename TI, typename TO, int VEC, bool INTO>
+__global__ void __launch_bounds__(kThreads)
+sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
+{
+    const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
+    const int64_t group = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> a.lanes_log2;
+    const int64_t tile = group / a.slices;
+    const int slice = static_cast<int>(group - tile * a.slices);
+    if (tile >= a.tiles) return;
+    const int step = lanes * VEC, column = slice * (lanes * kColumns) + lane * VEC, D = a.D;
+    const int64_t first = tile * a.tile_rows;
+    const int rows = static_cast<int>(a.n - first < a.tile_rows ? a.n - first : a.tile_rows);
+    const uint2* entries = a.sorted + first;
+    uint32_t cur = __ldg(entries).x;
+    bool head = first > 0 && __ldg(entries - 1).x == cur;
+    float acc[kColumns] = {}, kept[kColumns] = {};
+    auto put_part = [&](int slot) {
+        float* part = a.parts + (tile * 2 + slot) * a.padded_D;
+        store_row<float, VEC>(part, acc, column, step, D);
+    };
+    auto put_row = [&] {
+        float v[kColumns];
+#pragma unroll
+        for (int e = 0; e < kColumns; ++e) v[e] = INTO ? fmaf(a.scale, acc[e], kept[e]) : a.scale * acc[e];
+        store_row<TO, VEC>(out + static_cast<int64_t>(cur) * a.out_stride, v, column, step, D);
+    };
+    bool fresh = !head;        // the row in the buffer has still to be fetched
+    uint2 next[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) next[k] = k < rows ? __ldg(entries + k) : make_uint2(a.none, 0u);
+    bool over = false;
+    for (int r = 0; r < rows && !over; r += kAhead) {
+        uint2 now[kAhead];
+        Columns<TI, VEC> row[kAhead];
+        float old[INTO ? kAhead : 1][kColumns];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            now[k] = next[k];
+            if (now[k].x != a.none) row[k].load(grad + static_cast<int64_t>(now[k].y) * a.grad_stride, column, step, D);
+            if constexpr (INTO) {
+                const uint32_t before = k == 0 ? cur : now[k == 0 ? 0 : k - 1].x;
+                if (now[k].x != a.none && (now[k].x != before || (r + k == 0 && fresh)))
+                    load_row<TO, VEC>(old[k], out + static_cast<int64_t>(now[k].x) * a.out_stride, column, step, D);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) next[k] = r + kAhead + k < rows ? __ldg(entries + r + kAhead + k) : make_uint2(a.none, 0u);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (over) continue;
+            const bool starts = now[k].x != cur;
+            if (starts) {
+                if (r + k >= rows) {       // behind the tile
+                    over = true;
+                    continue;
+                }
+                if (head) put_part(0);
+                else put_row();
+                head = false;
+                cur = now[k].x;
+#pragma unroll
+                for (int e = 0; e < kColumns; ++e) acc[e] = 0.0f;
+            }
+            if (cur == a.none) {           // they sort last
+                over = true;
+                continue;
+            }
+            if (r + k >= rows) {
+                over = true;
+                continue;
+            }
+            if constexpr (INTO)
+                if (starts || (r + k == 0 && fresh)) {
+#pragma unroll
+                    for (int e = 0; e < kColumns; ++e) kept[e] = old[k][e];
+                }
+#pragma unroll
+            for (int e = 0; e < kColumns; ++e) acc[e] += row[k].at(e);
+        }
+    }
+    if (cur == a.none) return;
+    const bool goes_on = first + rows < a.n && __ldg(entries + rows).x == cur;
+    if (head || goes_on) put_part(head ? 0 : 1);
+    else put_row();
+}
+
+// A token that starts in tile t and goes on: its piece in slot 1 of t and slot 0 of the tiles that it reaches.  The block's
+// warps take equal runs of the pieces; their sums are added in order.
+constexpr int kJoinColumns = 32;
+template <typename TO, bool INTO>
+__global__ void __launch_bounds__(kThreads) join_parts_kernel(const SumArgs a, TO* out)
+{
+    const int64_t tile = blockIdx.x, first = tile * a.tile_rows, next = first + a.tile_rows;
+    if (next >= a.n) return;
+    const uint32_t cur = __ldg(a.sorted + next - 1).x;
+    if (cur == a.none || __ldg(a.sorted + next).x != cur) return;
+    if (first > 0 && __ldg(a.sorted + first).x == cur && __ldg(a.sorted + first - 1).x == cur) return;      // came in: another tile's
+    // tiles behind this one that begin with the token
+    __shared__ float partial[kWarps][kJoinColumns];
+    int64_t reached = 0;
+    for (;;) {
+        const int64_t t = tile + 1 + reached + threadIdx.x;
+        const int more = __syncthreads_count(t < a.tiles && __ldg(a.sorted + t * a.tile_rows).x == cur);
+        reached += more;
+        if (more < kThreads) break;
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = blockIdx.y * kJoinColumns + lane;
+    const int64_t pieces = reached + 1, run = (pieces + kWarps - 1) / kWarps, from = warp * run, to = from + run < pieces ? from + run : pieces;
+    float sum = 0.0f;
+    if (c < a.D)
+#pragma unroll 8
+        for (int64_t k = from; k < to; ++k) sum += a.parts[((tile + k) * 2 + (k == 0 ? 1 : 0)) * a.padded_D + c];
+    partial[warp][lane] = sum;
+    __syncthreads();
+    if (warp != 0 || c >= a.D) return;
+    float v[1] = {0.0f};
+    for (int w = 0; w < kWarps; ++w) v[0] += partial[w][lane];
+    TO* p = out + static_cast<int64_t>(cur) * a.out_stride + c;
+    v[0] *= a.scale;
+    if constexpr (INTO) {
+        Piece<TO, 1> old;
+        load_piece<TO, 1, false>(old, p);
+        v[0] += element(old, 0);
+    }
+    store_piece<TO, 1>(p, v);
 }
 
 int64_t align16(int64_t b) { return (b + 15) / 16 * 16; }
 
-struct GradLayout {
-    int64_t keys[2], vals[2], hist, parts, total;
+// Where things lie in the scratch, and how the sums are cut: about as many groups of lanes as the GPU holds, each with a tile
+// and a slice of the columns.
+struct GradPlan {
+    int64_t sorted[2], hist, parts, total;
     int64_t tiles, sort_tiles;
+    int tile_rows, slices, lanes_log2, padded_D;
 };
 
-bool grad_layout(int64_t n, int64_t num_embeddings, int64_t D, GradLayout& l)
+constexpr int64_t kResidentWarps = 148 * 24;
+
+bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
 {
     if (n < 0 || n > 0x7fffffff || num_embeddings < 1 || num_embeddings > 0x7fffffff || D < 1 || D > (1 << 20)) return false;
-    l.tiles = (n + kTileRows - 1) / kTileRows;
-    l.sort_tiles = (n + kSortTile - 1) / kSortTile;
+    l.lanes_log2 = 2;
+    while (l.lanes_log2 < 5 && (kColumns << l.lanes_log2) < D) ++l.lanes_log2;
+    l.slices = static_cast<int>((D + (kColumns << l.lanes_log2) - 1) / (kColumns << l.lanes_log2));
+    const int64_t groups = kResidentWarps << (5 - l.lanes_log2), want = (n * l.slices + groups - 1) / groups;
+    l.tile_rows = static_cast<int>(want < 8 ? 8 : want > 256 ? 256 : (want + kAhead - 1) / kAhead * kAhead);
+    l.tiles = (n + l.tile_rows - 1) / l.tile_rows;
+    l.padded_D = static_cast<int>((D + 7) / 8 * 8);
+    l.sort_tiles = n > kClusterKeys ? (n + kSortTile - 1) / kSortTile : 0;
     int64_t at = 0;
-    for (int i = 0; i < 2; ++i) {
-        l.keys[i] = at; at += align16(4 * n);
-        l.vals[i] = at; at += align16(4 * n);
-    }
+    l.sorted[0] = at; at += align16(8 * n);
+    l.sorted[1] = at; at += l.sort_tiles ? align16(8 * n) : 0;
     l.hist = at; at += align16(4 * kMaxBins * l.sort_tiles);
-    l.parts = at; at += align16(l.tiles * 2 * D * 4);
+    l.parts = at; at += l.tiles * 2 * l.padded_D * 4;
     l.total = at;
     return true;
+}
+
+template <int ITEMS>
+int launch_sort(const SortInput& in, int cluster, int passes, int width, uint2* sorted, const FillArgs& fill, int unit, int64_t fillers, cudaStream_t s)
+{
+    auto* kernel = sort_tokens_kernel<ITEMS>;
+    const int shared = static_cast<int>(sort_shared_bytes(ITEMS));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "token_embedding_grad: %s", cudaGetErrorString(e));
+    cudaLaunchAttribute together{};
+    together.id = cudaLaunchAttributeClusterDimension;
+    together.val.clusterDim.x = cluster;
+    together.val.clusterDim.y = together.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(cluster + fillers));
+    config.blockDim = dim3(kSortThreads);
+    config.dynamicSmemBytes = shared;
+    config.stream = s;
+    config.attrs = &together;
+    config.numAttrs = 1;
+    e = cudaLaunchKernelEx(&config, kernel, in, cluster, passes, width, sorted, fill, unit);
+    if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "sort_tokens_kernel: %s", cudaGetErrorString(e));
+    return check_launch("sort_tokens_kernel");
+}
+
+// Sorted (token, position) pairs into one of the two halves of the scratch, whose number is returned in `half`; the
+// gradient cleared on the way.
+int sort_and_clear(const SortInput& in, const GradPlan& l, char* scratch, const FillArgs& fill, int unit, int& half, cudaStream_t s)
+{
+    half = 0;
+    // blocks that clear: 64 KB each at least, one per multiprocessor at most
+    int64_t fillers = (fill.rows * fill.row_bytes + 65535) / 65536;
+    const int sms = sm_count();
+    if (in.n == 0 || in.n > kClusterKeys) {
+        if (fillers) {
+            clear_rows_kernel<<<static_cast<unsigned>(fillers < 4 * sms ? fillers : 4 * sms), kThreads, 0, s>>>(fill, unit);
+            if (const int rc = check_launch("clear_rows_kernel")) return rc;
+        }
+        if (in.n == 0) return TBE_B200_OK;
+    }
+    // digits of equal width, at most nine bits, that cover the keys 0 .. num_embeddings
+    int bits = 1;
+    while ((in.num_embeddings >> bits) != 0) ++bits;
+    const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes, bins = 1 << width;
+    if (in.n <= kClusterKeys) {
+        const int cluster = in.n <= kOneBlockKeys ? 1 : kSortBlocks;
+        const int64_t items = (in.n + cluster * kSortThreads - 1) / (cluster * kSortThreads);
+        fillers = fillers < sms - cluster ? fillers : sms - cluster;
+        fillers = (fillers + cluster - 1) / cluster * cluster;
+        if (cluster + fillers > sms) fillers -= cluster;
+        uint2* sorted = reinterpret_cast<uint2*>(scratch + l.sorted[0]);
+        if (items <= 1) return launch_sort<1>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
+        if (items <= 2) return launch_sort<2>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
+        if (items <= 4) return launch_sort<4>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
+        if (items <= 8) return launch_sort<8>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
+        return launch_sort<kMostItems>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
+    }
+    uint32_t* hist = reinterpret_cast<uint32_t*>(scratch + l.hist);
+    const unsigned tiles = static_cast<unsigned>(l.sort_tiles);
+    for (int p = 0; p < passes; ++p) {
+        const uint2* from = reinterpret_cast<const uint2*>(scratch + l.sorted[half]);
+        uint2* to = reinterpret_cast<uint2*>(scratch + l.sorted[half ^ 1]);
+        if (p == 0) sort_histogram_kernel<true><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist);
+        else sort_histogram_kernel<false><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist);
+        sort_places_kernel<<<1, 1024, 0, s>>>(hist, static_cast<int64_t>(bins) * tiles);
+        if (p == 0) sort_scatter_kernel<true><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist, to);
+        else sort_scatter_kernel<false><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist, to);
+        if (const int rc = check_launch("sort kernels")) return rc;
+        half ^= 1;
+    }
+    return TBE_B200_OK;
+}
+
+template <typename TI, typename TO, bool INTO>
+int launch_sums(const SumArgs& a, const TI* grad, TO* out, cudaStream_t s)
+{
+    const int64_t blocks = ((a.tiles * a.slices << a.lanes_log2) + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffff) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding_grad: too many tokens");
+    const unsigned g = static_cast<unsigned>(blocks);
+    auto fits = [&](int vec) {
+        return a.D % vec == 0 && rows_aligned(grad, a.grad_stride, sizeof(TI), vec) && rows_aligned(out, a.out_stride, sizeof(TO), vec);
+    };
+    constexpr int kWhole = sizeof(TI) == 4 ? 4 : 8, kSplit = sizeof(TI) == 4 ? 1 : 2;      // 16 bytes of an aligned row; a word of others
+    if (fits(kWhole)) sum_tiles_kernel<TI, TO, kWhole, INTO><<<g, kThreads, 0, s>>>(a, grad, out);
+    else sum_tiles_kernel<TI, TO, kSplit, INTO><<<g, kThreads, 0, s>>>(a, grad, out);
+    if (const int rc = check_launch("sum_tiles_kernel")) return rc;
+    join_parts_kernel<TO, INTO><<<dim3(static_cast<unsigned>(a.tiles), static_cast<unsigned>((a.D + kJoinColumns - 1) / kJoinColumns)), kThreads, 0, s>>>(a, out);
+    return check_launch("join_parts_kernel");
 }
 
 }  // namespace
@@ -362,8 +740,8 @@ extern "C" int tbe_b200_token_embedding(const void* weight, int32_t weight_dtype
 
 extern "C" int64_t tbe_b200_token_embedding_grad_scratch_bytes(int64_t n, int64_t num_embeddings, int64_t D)
 {
-    GradLayout l;
-    return grad_layout(n, num_embeddings, D, l) ? l.total : -1;
+    GradPlan l;
+    return plan_grad(n, num_embeddings, D, l) ? l.total : -1;
 }
 
 extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtype, int64_t grad_stride, const void* tokens, int32_t token_bits,
@@ -374,8 +752,8 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
     const int ib = element_bytes(grad_dtype), ob = element_bytes(grad_weight_dtype);
     if (!ib || !ob) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding_grad: element types FP32, FP16 and BF16, got %d and %d", grad_dtype, grad_weight_dtype);
     if (token_bits != 32 && token_bits != 64) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: token_bits must be 32 or 64, got %d", token_bits);
-    GradLayout l;
-    if (!grad_layout(n, num_embeddings, D, l))
+    GradPlan l;
+    if (!plan_grad(n, num_embeddings, D, l))
         return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: n and num_embeddings must be below 2^31, D at most 2^20, the last two positive");
     if (padding_idx < -1 || padding_idx >= num_embeddings) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: padding_idx %lld is no row", (long long)padding_idx);
     if (grad_stride < 0 || grad_weight_stride < D) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: bad row stride");
@@ -384,56 +762,19 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
         return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: scratch must be %lld bytes, 16-byte aligned", (long long)l.total);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     char* base = static_cast<char*>(scratch);
+    const SortInput in{tokens, token_bits == 64, n, num_embeddings, padding_idx};
+    const FillArgs fill{static_cast<char*>(grad_weight), accumulate ? 0 : num_embeddings, D * ob, grad_weight_stride * ob};
+    int half;
+    if (const int rc = sort_and_clear(in, l, base, fill, ob, half, s)) return rc;
+    if (n == 0) return TBE_B200_OK;
+    const SumArgs a{reinterpret_cast<const uint2*>(base + l.sorted[half]), n, static_cast<uint32_t>(num_embeddings), grad_stride, grad_weight_stride,
+                    static_cast<int>(D), l.padded_D, l.tile_rows, l.slices, l.lanes_log2, l.tiles, scale, reinterpret_cast<float*>(base + l.parts)};
     return with_element(grad_weight_dtype, [&](auto* to) {
-        using TO = std::remove_pointer_t<decltype(to)>;
-        TO* o = static_cast<TO*>(grad_weight);
-        if (!accumulate) {
-            const bool v8 = D % 8 == 0 && rows_aligned(o, grad_weight_stride, ob, 8);
-            const int64_t pieces = v8 ? D / 8 : D, want = (num_embeddings * pieces + kThreads - 1) / kThreads, most = sm_count() * 32;
-            const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
-            if (v8) zero_rows_kernel<TO, 8><<<blocks, kThreads, 0, s>>>(o, num_embeddings, pieces, grad_weight_stride);
-            else zero_rows_kernel<TO, 1><<<blocks, kThreads, 0, s>>>(o, num_embeddings, pieces, grad_weight_stride);
-            if (const int rc = check_launch("zero_rows_kernel")) return rc;
-        }
-        if (n == 0) return static_cast<int>(TBE_B200_OK);
-        // digits of equal width, at most nine bits, that cover the keys 0 .. num_embeddings
-        int bits = 1;
-        while ((num_embeddings >> bits) != 0) ++bits;
-        const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes, bins = 1 << width, wide = token_bits == 64;
-        uint32_t* hist = reinterpret_cast<uint32_t*>(base + l.hist);
-        const unsigned tiles = static_cast<unsigned>(l.sort_tiles);
-        int cur = 0;
-        for (int p = 0; p < passes; ++p) {
-            const uint32_t* k_in = reinterpret_cast<const uint32_t*>(base + l.keys[cur]);
-            const uint32_t* v_in = reinterpret_cast<const uint32_t*>(base + l.vals[cur]);
-            uint32_t* k_out = reinterpret_cast<uint32_t*>(base + l.keys[cur ^ 1]);
-            uint32_t* v_out = reinterpret_cast<uint32_t*>(base + l.vals[cur ^ 1]);
-            if (p == 0) sort_histogram_kernel<true><<<tiles, kThreads, 0, s>>>(tokens, k_in, wide, n, num_embeddings, padding_idx, p * width, bins, hist);
-            else sort_histogram_kernel<false><<<tiles, kThreads, 0, s>>>(tokens, k_in, wide, n, num_embeddings, padding_idx, p * width, bins, hist);
-            sort_places_kernel<<<1, 1024, 0, s>>>(hist, static_cast<int64_t>(bins) * tiles);
-            if (p == 0) sort_scatter_kernel<true><<<tiles, kThreads, 0, s>>>(tokens, k_in, v_in, wide, n, num_embeddings, padding_idx, p * width, bins, hist, k_out, v_out);
-            else sort_scatter_kernel<false><<<tiles, kThreads, 0, s>>>(tokens, k_in, v_in, wide, n, num_embeddings, padding_idx, p * width, bins, hist, k_out, v_out);
-            if (const int rc = check_launch("sort kernels")) return rc;
-            cur ^= 1;
-        }
-        const uint32_t* keys = reinterpret_cast<const uint32_t*>(base + l.keys[cur]);
-        const uint32_t* vals = reinterpret_cast<const uint32_t*>(base + l.vals[cur]);
-        float* parts = reinterpret_cast<float*>(base + l.parts);
-        const uint32_t none = static_cast<uint32_t>(num_embeddings);
-        const int rc = with_element(grad_dtype, [&](auto* ti) {
+        return with_element(grad_dtype, [&](auto* ti) {
+            using TO = std::remove_pointer_t<decltype(to)>;
             using TI = std::remove_pointer_t<decltype(ti)>;
-            const TI* g = static_cast<const TI*>(grad);
-            const unsigned gx = static_cast<unsigned>((l.tiles + kWarps - 1) / kWarps);
-            auto fits = [&](int vec) { return D % vec == 0 && rows_aligned(g, grad_stride, ib, vec) && rows_aligned(o, grad_weight_stride, ob, vec); };
-            auto grid = [&](int vec) { return dim3(gx, static_cast<unsigned>((D / vec + 31) / 32)); };
-            if (fits(8)) sum_tiles_kernel<TI, TO, 8><<<grid(8), kThreads, 0, s>>>(g, grad_stride, keys, vals, n, none, D / 8, scale, accumulate, o, grad_weight_stride, parts);
-            else if (fits(4)) sum_tiles_kernel<TI, TO, 4><<<grid(4), kThreads, 0, s>>>(g, grad_stride, keys, vals, n, none, D / 4, scale, accumulate, o, grad_weight_stride, parts);
-            else sum_tiles_kernel<TI, TO, 1><<<grid(1), kThreads, 0, s>>>(g, grad_stride, keys, vals, n, none, D, scale, accumulate, o, grad_weight_stride, parts);
-            return check_launch("sum_tiles_kernel");
+            if (accumulate) return launch_sums<TI, TO, true>(a, static_cast<const TI*>(grad), static_cast<TO*>(grad_weight), s);
+            return launch_sums<TI, TO, false>(a, static_cast<const TI*>(grad), static_cast<TO*>(grad_weight), s);
         });
-        if (rc) return rc;
-        join_parts_kernel<TO><<<dim3(static_cast<unsigned>(l.tiles), static_cast<unsigned>((D + kThreads - 1) / kThreads)), kThreads, 0, s>>>(
-            keys, n, none, D, scale, accumulate, o, grad_weight_stride, parts);
-        return check_launch("join_parts_kernel");
     });
 }
