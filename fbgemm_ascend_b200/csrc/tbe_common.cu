@@ -42,6 +42,17 @@ int sm_count()
     return n;
 }
 
+int allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done)
+{
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) dev = 64;
+    if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return TBE_B200_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "shared memory of a kernel: %s", cudaGetErrorString(e));
+    if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    return TBE_B200_OK;
+}
+
 }  // namespace tbe
 
 extern "C" const char* tbe_b200_last_error(void) { return tbe::g_last_error; }

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "tbe_b200.h"
 
 namespace tbe {
@@ -19,6 +21,10 @@ int check_launch(const char* what);
 
 // Number of SMs of the current device (cached per device).
 int sm_count();
+
+// Lets `kernel` take `bytes` of dynamic shared memory on the current device; asked of the driver once per device, which
+// `done` (a bit per device, one word per kernel) keeps.  A status.
+int allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done);
 
 constexpr int kWarp = 32;
 

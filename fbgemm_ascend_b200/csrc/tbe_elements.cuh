@@ -50,6 +50,42 @@ __device__ __forceinline__ void clear_piece(Piece<T, VEC>& r)
     for (int i = 0; i < Piece<T, VEC>::kWords; ++i) r.w[i] = 0u;
 }
 
+// A piece that may start at any element and reach past `end` (the address behind its row): read in aligned 16-byte words, none of
+// which lies wholly outside the row, and shifted into place.  What is not the row's is left as it is there.
+template <typename T, int VEC>
+struct SplitPiece {
+    static constexpr int kBytes = Piece<T, VEC>::kBytes;
+    static constexpr int kQuads = (kBytes + 15) / 16 + 1;
+    uint4 q[kQuads];
+    uint32_t offset;      // of the first element in the first word, bytes
+
+    __device__ __forceinline__ void load(const T* p, const T* end)
+    {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p), e = reinterpret_cast<uintptr_t>(end);
+        offset = static_cast<uint32_t>(a & 15);
+        const uintptr_t first = a & ~uintptr_t(15), behind = a + kBytes < e ? a + kBytes : e;
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) q[i] = first + 16 * i < behind ? ldg16(reinterpret_cast<const void*>(first + 16 * i)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ Piece<T, VEC> piece() const
+    {
+        constexpr int W = Piece<T, VEC>::kWords;
+        uint32_t w[4 * kQuads];
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+            w[4 * i] = q[i].x; w[4 * i + 1] = q[i].y; w[4 * i + 2] = q[i].z; w[4 * i + 3] = q[i].w;
+        }
+#pragma unroll
+        for (int i = 0; i < W + 2; ++i) w[i] = (offset & 8) ? w[i + 2 < 4 * kQuads ? i + 2 : i] : w[i];
+#pragma unroll
+        for (int i = 0; i < W + 1; ++i) w[i] = (offset & 4) ? w[i + 1] : w[i];
+        Piece<T, VEC> r;
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.w[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], (offset & 2) * 8) : w[i];
+        return r;
+    }
+};
+
 // 16-bit types come two to a word; bf16 is the upper half of an fp32.
 template <typename T, int VEC>
 __device__ __forceinline__ float element(const Piece<T, VEC>& r, int i)

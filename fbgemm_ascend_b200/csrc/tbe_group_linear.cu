@@ -8,7 +8,6 @@
 #include <cuda.h>
 
 #include <atomic>
-#include <cstdlib>
 
 #include "tbe_elements.cuh"
 
@@ -522,8 +521,8 @@ int launch_linear(LinearArgs a, cudaStream_t s)
     if (!encode_rows(&codes, a, 32, tile_rows, true) || !encode_rows(&heads, a, a.head_bytes / 4, tile_rows, false))
         return fail(TBE_B200_ERR_CUDA, "group_row_linear: the rows could not be described to the copy engine");
     auto* kernel = group_row_linear_kernel<RT, NT, P, STEPS>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
-    if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "group_row_linear: %s", cudaGetErrorString(e));
+    static std::atomic<uint64_t> allowed{0};
+    if (const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kMostShared, allowed)) return rc;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
@@ -534,7 +533,7 @@ int launch_linear(LinearArgs a, cudaStream_t s)
     config.stream = s;
     config.attrs = &early;
     config.numAttrs = 1;
-    e = cudaLaunchKernelEx(&config, kernel, a, codes, heads);
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a, codes, heads);
     if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "group_row_linear_kernel: %s", cudaGetErrorString(e));
     return check_launch("group_row_linear_kernel");
 }
@@ -592,7 +591,7 @@ extern "C" int tbe_b200_group_row_linear(const void* input, int32_t input_dtype,
     const LinearArgs a{states, back, m, rows, num_rows, row_bytes, static_cast<int>(D), group_log2, bias, bias_dtype, output_dtype, output, output_stride,
                        error_flag, 0, 0, 0, 0};
     // Rows 32 to a warp use every state twice; 16 where that leaves multiprocessors without any.
-    const bool many = getenv("RT1") ? false : num_rows >= static_cast<int64_t>(64) * sm_count();
+    const bool many = num_rows >= static_cast<int64_t>(64) * sm_count();
     if (pieces_of(input_dtype) == 1) {
         if (NT == 1) return many ? launch_linear<2, 1, 1>(a, s) : launch_linear<1, 1, 1>(a, s);
         return many ? launch_linear<2, 2, 1>(a, s) : launch_linear<1, 2, 1>(a, s);

@@ -138,7 +138,7 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* warp_t
 
 // ---- up to kClusterKeys tokens: one cluster sorts in shared memory, the other blocks clear the gradient meanwhile ------
 //
-// A block of the cluster holds ITEMS * 1024 neighbouring places.  Per digit: ranks in registers, digit counts exchanged
+// A block of the cluster holds items (at most ITEMS) * 1024 neighbouring places.  Per digit: ranks in registers, digit counts exchanged
 // between the blocks, then every key straight to its place in whichever block's shared memory that is.  Launch and
 // synchronisation are all that it costs beside the clearing: with nothing to clear, 16384 tokens of 131072 take LATER us.
 constexpr int kSortThreads = 1024;
@@ -153,28 +153,39 @@ struct FillArgs {
     int64_t rows, row_bytes, stride_bytes;      // rows == 0: nothing to clear
 };
 
-__device__ __forceinline__ void clear_run(char* p, int64_t bytes, int64_t thread, int64_t threads, int unit)
+constexpr int kZeroBytes = 32 * 1024;      // of shared memory that a clearing block keeps at zero and copies out
+
+// Clears `bytes` at p: thread `thread` of `threads` takes every threads-th run of kZeroBytes, by bulk copies from `zeros`; what
+// lies in front of the first 16-byte border and behind the last goes element by element.
+__device__ __forceinline__ void clear_run(char* p, int64_t bytes, int64_t thread, int64_t threads, int unit, const void* zeros)
 {
-    // up to the first 16-byte border and behind the last one element by element
-    const int64_t head = min((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15, bytes), body = (bytes - head) / 16;
-    for (int64_t i = thread; i < body; i += threads) st_stream16(p + head + 16 * i, make_uint4(0u, 0u, 0u, 0u));
-    const int64_t edge = (head + (bytes - head - 16 * body)) / unit;
+    const int64_t head = min((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15, bytes), body = (bytes - head) & ~int64_t(15);
+    for (int64_t at = thread * kZeroBytes; at < body; at += threads * kZeroBytes) {
+        const uint32_t run = static_cast<uint32_t>(body - at < kZeroBytes ? body - at : kZeroBytes);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p + head + at), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(zeros))),
+                     "r"(run) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    const int64_t edge = (bytes - body) / unit;
     for (int64_t i = thread; i < edge; i += threads) {
-        char* q = i * unit < head ? p + i * unit : p + 16 * body + i * unit;
+        char* q = i * unit < head ? p + i * unit : p + body + i * unit;
         if (unit == 4) *reinterpret_cast<uint32_t*>(q) = 0u;
         else *reinterpret_cast<unsigned short*>(q) = 0;
     }
 }
 
-__device__ __forceinline__ void clear_rows(const FillArgs& f, int unit, int64_t block, int64_t blocks)
+// A block's share of the rows; `zeros`: kZeroBytes of shared memory, 16-byte aligned.
+__device__ __forceinline__ void clear_rows(const FillArgs& f, int unit, int64_t block, int64_t blocks, unsigned char* zeros)
 {
+    for (int i = threadIdx.x; i < kZeroBytes / 16; i += blockDim.x) reinterpret_cast<uint4*>(zeros)[i] = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
     if (f.stride_bytes == f.row_bytes) {
-        clear_run(f.out, f.rows * f.row_bytes, block * blockDim.x + threadIdx.x, blocks * blockDim.x, unit);
+        if (threadIdx.x == 0) clear_run(f.out, f.rows * f.row_bytes, block, blocks, unit, zeros);
     } else {
-        const int64_t warps = blocks * (blockDim.x / 32);
-        for (int64_t r = block * (blockDim.x / 32) + threadIdx.x / 32; r < f.rows; r += warps)
-            clear_run(f.out + r * f.stride_bytes, f.row_bytes, threadIdx.x & 31, 32, unit);
+        for (int64_t r = block * blockDim.x + threadIdx.x; r < f.rows; r += blocks * blockDim.x) clear_run(f.out + r * f.stride_bytes, f.row_bytes, 0, 1, unit, zeros);
     }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t cluster_rank()
@@ -199,23 +210,23 @@ constexpr int64_t sort_shared_bytes(int items) { return int64_t(items) * kSortTh
 
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads, 1)
-sort_tokens_kernel(const SortInput in, int cluster, int passes, int width, uint2* __restrict__ sorted, const FillArgs fill, int unit)
+sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int width, uint2* __restrict__ sorted, const FillArgs fill, int unit)
 {
+    extern __shared__ __align__(16) unsigned char sort_smem[];
     if (blockIdx.x >= cluster) {
-        clear_rows(fill, unit, blockIdx.x - cluster, gridDim.x - cluster);
+        clear_rows(fill, unit, blockIdx.x - cluster, gridDim.x - cluster, sort_smem);
         return;
     }
-    constexpr int kPer = ITEMS * kSortThreads;
-    extern __shared__ __align__(16) unsigned char sort_smem[];
     unsigned long long* buf = reinterpret_cast<unsigned long long*>(sort_smem);
-    unsigned short(*count)[kMaxBins] = reinterpret_cast<unsigned short(*)[kMaxBins]>(buf + kPer);
+    unsigned short(*count)[kMaxBins] = reinterpret_cast<unsigned short(*)[kMaxBins]>(buf + ITEMS * kSortThreads);
     uint32_t(*table)[kMaxBins] = reinterpret_cast<uint32_t(*)[kMaxBins]>(count + kSortWarps);
     uint32_t* base = reinterpret_cast<uint32_t*>(table + kSortBlocks);
     uint32_t* warp_tot = base + kMaxBins;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << width;
     const uint32_t mine = cluster > 1 ? cluster_rank() : 0u;
-    const int64_t first = static_cast<int64_t>(mine) * kPer;
-    const int at = warp * (32 * ITEMS) + lane;
+    const int per = items * kSortThreads;
+    const int64_t first = static_cast<int64_t>(mine) * per;
+    const int at = warp * (32 * items) + lane;
     auto sync_all = [&] {
         if (cluster > 1) cluster_sync();
         else __syncthreads();
@@ -227,7 +238,7 @@ sort_tokens_kernel(const SortInput in, int cluster, int passes, int width, uint2
         for (int j = 0; j < ITEMS; ++j) {
             const int64_t i = first + at + j * 32;
             key[j] = pos[j] = 0u;
-            if (i < in.n) {
+            if (j < items && i < in.n) {
                 if (p == 0) {
                     key[j] = token_key(in, i);
                     pos[j] = static_cast<uint32_t>(i);
@@ -241,7 +252,8 @@ sort_tokens_kernel(const SortInput in, int cluster, int passes, int width, uint2
         for (int b = threadIdx.x; b < kSortWarps * kMaxBins / 2; b += kSortThreads) reinterpret_cast<uint32_t*>(count)[b] = 0u;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < ITEMS; ++j) rank[j] = warp_rank((key[j] >> (p * width)) & (bins - 1), first + at + j * 32 < in.n, count[warp]);
+        for (int j = 0; j < ITEMS; ++j)
+            if (j < items) rank[j] = warp_rank((key[j] >> (p * width)) & (bins - 1), first + at + j * 32 < in.n, count[warp]);
         __syncthreads();
         if (threadIdx.x < bins) {
             uint32_t run = 0;
@@ -271,17 +283,17 @@ sort_tokens_kernel(const SortInput in, int cluster, int passes, int width, uint2
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
-            if (first + at + j * 32 >= in.n) continue;
+            if (j >= items || first + at + j * 32 >= in.n) continue;
             const uint32_t d = (key[j] >> (p * width)) & (bins - 1), to = base[d] + count[warp][d] + rank[j];
             const unsigned long long both = (static_cast<unsigned long long>(key[j]) << 32) | pos[j];
             if (cluster > 1)
-                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(shared_of(buf + to % kPer, to / kPer)), "l"(both) : "memory");
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(shared_of(buf + to % per, to / per)), "l"(both) : "memory");
             else
                 buf[to] = both;
         }
         sync_all();
     }
-    for (int i = threadIdx.x; i < kPer && first + i < in.n; i += kSortThreads) {
+    for (int i = threadIdx.x; i < per && first + i < in.n; i += kSortThreads) {
         const unsigned long long both = buf[i];
         sorted[first + i] = make_uint2(static_cast<uint32_t>(both >> 32), static_cast<uint32_t>(both));
     }
@@ -373,7 +385,11 @@ sort_scatter_kernel(const SortInput in, const uint2* __restrict__ from, int shif
         if (base + j * 32 < in.n) to[count[warp][(entry[j].x >> shift) & (bins - 1)] + rank[j]] = entry[j];
 }
 
-__global__ void __launch_bounds__(kThreads) clear_rows_kernel(const FillArgs fill, int unit) { clear_rows(fill, unit, blockIdx.x, gridDim.x); }
+__global__ void __launch_bounds__(kThreads) clear_rows_kernel(const FillArgs fill, int unit)
+{
+    __shared__ __align__(16) unsigned char zeros[kZeroBytes];
+    clear_rows(fill, unit, blockIdx.x, gridDim.x, zeros);
+}
 
 // ---- gradient: sums ---------------------------------------------------------------------------------------------
 //
@@ -396,43 +412,45 @@ struct SumArgs {
     float* parts;
 };
 
-// How a lane's eight columns lie: VEC neighbouring ones at a time, `lanes` pieces apart.  VEC 1 and 2 stand for rows that are not
-// aligned; two 16-bit elements then come out of the one or two words that hold them.
-template <typename T, int VEC>
+// A lane's eight columns lie in pieces of 16 bytes, `lanes` pieces apart.
+template <typename T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+template <typename T, bool ALIGNED>
 struct Columns {
-    static constexpr int kPieces = kColumns / VEC;
-    Piece<T, VEC> p[kPieces];
+    static constexpr int VEC = kVec<T>, kPieces = kColumns / VEC;
+    typename std::conditional<ALIGNED, Piece<T, VEC>, SplitPiece<T, VEC>>::type p[kPieces];
 
     __device__ __forceinline__ void load(const T* row, int column, int step, int D)
     {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int c = column + i * step;
-            if constexpr (VEC == 2 && sizeof(T) == 2) {
-                // Words are aligned, rows need not be: a word that holds one element of the row holds nothing foreign that is used.
-                const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
-                uint32_t v = 0;
-                if (c < D) {
-                    v = __ldg(w);
-                    if (a & 2) v = __funnelshift_r(v, c + 1 < D ? __ldg(w + 1) : 0u, 16);
-                    else if (c + 1 >= D) v &= 0xffffu;
-                }
-                p[i].w[0] = v;
-            } else if (c < D) {
-                load_piece<T, VEC>(p[i], row + c);
+            if constexpr (ALIGNED) {
+                if (c < D) load_piece<T, VEC>(p[i], row + c);
+                else clear_piece(p[i]);
             } else {
-                clear_piece(p[i]);
+                p[i].load(row + (c < D ? c : D), row + D);
             }
         }
     }
-    __device__ __forceinline__ float at(int e) const { return element(p[e / VEC], e % VEC); }
+    __device__ __forceinline__ void add_to(float (&acc)[kColumns]) const
+    {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            Piece<T, VEC> r;
+            if constexpr (ALIGNED) r = p[i];
+            else r = p[i].piece();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[i * VEC + e] += element(r, e);
+        }
+    }
 };
 
-template <typename TO, int VEC>
+// The same columns (those of rows of TI) of a row of another type.
+template <typename TI, typename TO, bool ALIGNED>
 __device__ __forceinline__ void load_row(float (&v)[kColumns], const TO* row, int column, int step, int D)
 {
-    constexpr int kOne = VEC == 2 ? 1 : VEC;      // rows of VEC 2 are not aligned
+    constexpr int VEC = kVec<TI>, kOne = ALIGNED ? VEC : 1;
 #pragma unroll
     for (int i = 0; i < kColumns / kOne; ++i) {
         const int c = column + (i * kOne / VEC) * step + (i * kOne) % VEC;
@@ -444,10 +462,10 @@ __device__ __forceinline__ void load_row(float (&v)[kColumns], const TO* row, in
     }
 }
 
-template <typename TO, int VEC>
+template <typename TI, typename TO, bool ALIGNED>
 __device__ __forceinline__ void store_row(TO* row, const float (&v)[kColumns], int column, int step, int D)
 {
-    constexpr int kOne = VEC == 2 ? 1 : VEC;
+    constexpr int VEC = kVec<TI>, kOne = ALIGNED ? VEC : 1;
 #pragma unroll
     for (int i = 0; i < kColumns / kOne; ++i) {
         const int c = column + (i * kOne / VEC) * step + (i * kOne) % VEC;
@@ -458,7 +476,7 @@ __device__ __forceinline__ void store_row(TO* row, const float (&v)[kColumns], i
     }
 }
 
-template <typename TI, typename TO, int VEC, bool INTO>
+template <typename TI, typename TO, bool ALIGNED, bool INTO>
 __global__ void __launch_bounds__(kThreads)
 sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
 {
@@ -467,6 +485,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
     const int64_t tile = group / a.slices;
     const int slice = static_cast<int>(group - tile * a.slices);
     if (tile >= a.tiles) return;
+    constexpr int VEC = kVec<TI>;
     const int step = lanes * VEC, column = slice * (lanes * kColumns) + lane * VEC, D = a.D;
     const int64_t first = tile * a.tile_rows;
     const int rows = static_cast<int>(a.n - first < a.tile_rows ? a.n - first : a.tile_rows);
@@ -476,13 +495,13 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
     float acc[kColumns] = {}, kept[kColumns] = {};
     auto put_part = [&](int slot) {
         float* part = a.parts + (tile * 2 + slot) * a.padded_D;
-        store_row<float, VEC>(part, acc, column, step, D);
+        store_row<TI, float, true>(part, acc, column, step, a.padded_D);
     };
     auto put_row = [&] {
         float v[kColumns];
 #pragma unroll
         for (int e = 0; e < kColumns; ++e) v[e] = INTO ? fmaf(a.scale, acc[e], kept[e]) : a.scale * acc[e];
-        store_row<TO, VEC>(out + static_cast<int64_t>(cur) * a.out_stride, v, column, step, D);
+        store_row<TI, TO, ALIGNED>(out + static_cast<int64_t>(cur) * a.out_stride, v, column, step, D);
     };
     bool fresh = !head;        // the row in the buffer has still to be fetched
     uint2 next[kAhead];
@@ -491,7 +510,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
     bool over = false;
     for (int r = 0; r < rows && !over; r += kAhead) {
         uint2 now[kAhead];
-        Columns<TI, VEC> row[kAhead];
+        Columns<TI, ALIGNED> row[kAhead];
         float old[INTO ? kAhead : 1][kColumns];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
@@ -500,7 +519,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
             if constexpr (INTO) {
                 const uint32_t before = k == 0 ? cur : now[k == 0 ? 0 : k - 1].x;
                 if (now[k].x != a.none && (now[k].x != before || (r + k == 0 && fresh)))
-                    load_row<TO, VEC>(old[k], out + static_cast<int64_t>(now[k].x) * a.out_stride, column, step, D);
+                    load_row<TI, TO, ALIGNED>(old[k], out + static_cast<int64_t>(now[k].x) * a.out_stride, column, step, D);
             }
         }
 #pragma unroll
@@ -534,8 +553,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
 #pragma unroll
                     for (int e = 0; e < kColumns; ++e) kept[e] = old[k][e];
                 }
-#pragma unroll
-            for (int e = 0; e < kColumns; ++e) acc[e] += row[k].at(e);
+            row[k].add_to(acc);
         }
     }
     if (cur == a.none) return;
@@ -544,46 +562,90 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
     else put_row();
 }
 
-// A token that starts in tile t and goes on: its piece in slot 1 of t and slot 0 of the tiles that it reaches.  The block's
-// warps take equal runs of the pieces; their sums are added in order.
-constexpr int kJoinColumns = 32;
+// A token that starts in tile t and goes on: its piece in slot 1 of t and slot 0 of the tiles that it reaches, added in order.
+// A block looks at a tile and 128 columns for each of its warps, which add up a token of up to kFewPieces pieces alone.  A longer
+// one occupies as many tiles, whose blocks have nothing else to do: each takes 128 columns in turn, with its warps' sums of
+// equal runs of the pieces added in order.
+constexpr int kJoinColumns = 128;
+constexpr int kFewPieces = 64;
+
+// How many of the tiles t0, t0 + direction, ... begin with `key`, one after the other.
+__device__ __forceinline__ int64_t tiles_that_begin_with(const SumArgs& a, uint32_t key, int64_t t0, int direction)
+{
+    int64_t found = 0;
+    for (;;) {
+        const int64_t t = t0 + direction * (found + threadIdx.x);
+        const int more = __syncthreads_count(t >= 0 && t < a.tiles && __ldg(a.sorted + t * a.tile_rows).x == key);
+        found += more;
+        if (more < kThreads) return found;
+    }
+}
+
+__device__ __forceinline__ float4 add_pieces(const SumArgs& a, int64_t tile, int64_t from, int64_t to, int c)
+{
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int64_t k = from; k < to; ++k) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(a.parts + ((tile + k) * 2 + (k == 0 ? 1 : 0)) * a.padded_D + c));
+        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    return sum;
+}
+
+template <typename TO, bool INTO>
+__device__ __forceinline__ void put_sum(const SumArgs& a, TO* row, float4 sum, int c)
+{
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (c + e >= a.D) continue;
+        Piece<TO, 1> old;
+        clear_piece(old);
+        if constexpr (INTO) load_piece<TO, 1, false>(old, row + c + e);
+        const float one[1] = {INTO ? fmaf(a.scale, v[e], element(old, 0)) : a.scale * v[e]};
+        store_piece<TO, 1>(row + c + e, one);
+    }
+}
+
 template <typename TO, bool INTO>
 __global__ void __launch_bounds__(kThreads) join_parts_kernel(const SumArgs a, TO* out)
 {
+    __shared__ float4 partial[kWarps][32];
     const int64_t tile = blockIdx.x, first = tile * a.tile_rows, next = first + a.tile_rows;
-    if (next >= a.n) return;
-    const uint32_t cur = __ldg(a.sorted + next - 1).x;
-    if (cur == a.none || __ldg(a.sorted + next).x != cur) return;
-    if (first > 0 && __ldg(a.sorted + first).x == cur && __ldg(a.sorted + first - 1).x == cur) return;      // came in: another tile's
-    // tiles behind this one that begin with the token
-    __shared__ float partial[kWarps][kJoinColumns];
-    int64_t reached = 0;
-    for (;;) {
-        const int64_t t = tile + 1 + reached + threadIdx.x;
-        const int more = __syncthreads_count(t < a.tiles && __ldg(a.sorted + t * a.tile_rows).x == cur);
-        reached += more;
-        if (more < kThreads) break;
-    }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = blockIdx.y * kJoinColumns + lane;
-    const int64_t pieces = reached + 1, run = (pieces + kWarps - 1) / kWarps, from = warp * run, to = from + run < pieces ? from + run : pieces;
-    float sum = 0.0f;
-    if (c < a.D)
-#pragma unroll 8
-        for (int64_t k = from; k < to; ++k) sum += a.parts[((tile + k) * 2 + (k == 0 ? 1 : 0)) * a.padded_D + c];
-    partial[warp][lane] = sum;
-    __syncthreads();
-    if (warp != 0 || c >= a.D) return;
-    float v[1] = {0.0f};
-    for (int w = 0; w < kWarps; ++w) v[0] += partial[w][lane];
-    TO* p = out + static_cast<int64_t>(cur) * a.out_stride + c;
-    v[0] *= a.scale;
-    if constexpr (INTO) {
-        Piece<TO, 1> old;
-        load_piece<TO, 1, false>(old, p);
-        v[0] += element(old, 0);
+    const uint32_t begins = __ldg(a.sorted + first).x, before = first > 0 ? __ldg(a.sorted + first - 1).x : a.none;
+    const uint32_t ends = next < a.n ? __ldg(a.sorted + next - 1).x : a.none, after = next < a.n ? __ldg(a.sorted + next).x : a.none;
+    const bool came_in = begins != a.none && before == begins;
+    if (came_in) {
+        const int64_t back = tiles_that_begin_with(a, begins, tile - 1, -1), reach = tiles_that_begin_with(a, begins, tile + 1, 1);
+        // the first of the `back` tiles may be where the token starts
+        const int64_t far = tile - back, lead = far > 0 && __ldg(a.sorted + far * a.tile_rows - 1).x == begins ? far - 1 : far;
+        const int64_t pieces = tile + reach - lead + 1;
+        if (pieces > kFewPieces) {
+            const int64_t run = (pieces + kWarps - 1) / kWarps, from = warp * run < pieces ? warp * run : pieces, to = from + run < pieces ? from + run : pieces;
+            // the tile where it starts has blocks of its own only if it begins with it; the others share the columns
+            const int64_t helpers = (pieces - 1) * gridDim.y, me = (tile - lead - 1) * gridDim.y + blockIdx.y;
+            for (int64_t chunk = me; chunk * kJoinColumns < a.D; chunk += helpers) {
+                const int c = static_cast<int>(chunk) * kJoinColumns + lane * 4;
+                partial[warp][lane] = c < a.D ? add_pieces(a, lead, from, to, c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                __syncthreads();
+                if (warp == 0 && c < a.D) {
+                    float4 sum = partial[0][lane];
+                    for (int w = 1; w < kWarps; ++w) {
+                        const float4 v = partial[w][lane];
+                        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+                    }
+                    put_sum<TO, INTO>(a, out + static_cast<int64_t>(begins) * a.out_stride, sum, c);
+                }
+                __syncthreads();
+            }
+        }
     }
-    store_piece<TO, 1>(p, v);
+    if (ends == a.none || after != ends || (came_in && begins == ends)) return;
+    const int64_t pieces = 1 + tiles_that_begin_with(a, ends, tile + 1, 1);
+    const int c = (blockIdx.y * kWarps + warp) * kJoinColumns + lane * 4;
+    if (pieces > kFewPieces || c >= a.D) return;
+    put_sum<TO, INTO>(a, out + static_cast<int64_t>(ends) * a.out_stride, add_pieces(a, tile, 0, pieces, c), c);
 }
 
 int64_t align16(int64_t b) { return (b + 15) / 16 * 16; }
@@ -605,7 +667,9 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
     while (l.lanes_log2 < 5 && (kColumns << l.lanes_log2) < D) ++l.lanes_log2;
     l.slices = static_cast<int>((D + (kColumns << l.lanes_log2) - 1) / (kColumns << l.lanes_log2));
     const int64_t groups = kResidentWarps << (5 - l.lanes_log2), want = (n * l.slices + groups - 1) / groups;
-    l.tile_rows = static_cast<int>(want < 8 ? 8 : want > 256 ? 256 : (want + kAhead - 1) / kAhead * kAhead);
+    // long tokens leave a piece per tile: not too many of them where rows are narrow
+    const int64_t least = n <= 8192 ? 8 : 32;
+    l.tile_rows = static_cast<int>(want < least ? least : want > 256 ? 256 : (want + kAhead - 1) / kAhead * kAhead);
     l.tiles = (n + l.tile_rows - 1) / l.tile_rows;
     l.padded_D = static_cast<int>((D + 7) / 8 * 8);
     l.sort_tiles = n > kClusterKeys ? (n + kSortTile - 1) / kSortTile : 0;
@@ -619,12 +683,12 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
 }
 
 template <int ITEMS>
-int launch_sort(const SortInput& in, int cluster, int passes, int width, uint2* sorted, const FillArgs& fill, int unit, int64_t fillers, cudaStream_t s)
+int launch_sort(const SortInput& in, int cluster, int items, int passes, int width, uint2* sorted, const FillArgs& fill, int unit, int64_t fillers, cudaStream_t s)
 {
     auto* kernel = sort_tokens_kernel<ITEMS>;
     const int shared = static_cast<int>(sort_shared_bytes(ITEMS));
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-    if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "token_embedding_grad: %s", cudaGetErrorString(e));
+    static std::atomic<uint64_t> allowed{0};
+    if (const int rc = allow_shared(reinterpret_cast<const void*>(kernel), shared, allowed)) return rc;
     cudaLaunchAttribute together{};
     together.id = cudaLaunchAttributeClusterDimension;
     together.val.clusterDim.x = cluster;
@@ -636,7 +700,7 @@ int launch_sort(const SortInput& in, int cluster, int passes, int width, uint2* 
     config.stream = s;
     config.attrs = &together;
     config.numAttrs = 1;
-    e = cudaLaunchKernelEx(&config, kernel, in, cluster, passes, width, sorted, fill, unit);
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, in, cluster, items, passes, width, sorted, fill, unit);
     if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "sort_tokens_kernel: %s", cudaGetErrorString(e));
     return check_launch("sort_tokens_kernel");
 }
@@ -662,16 +726,14 @@ int sort_and_clear(const SortInput& in, const GradPlan& l, char* scratch, const 
     const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes, bins = 1 << width;
     if (in.n <= kClusterKeys) {
         const int cluster = in.n <= kOneBlockKeys ? 1 : kSortBlocks;
-        const int64_t items = (in.n + cluster * kSortThreads - 1) / (cluster * kSortThreads);
+        const int items = static_cast<int>((in.n + cluster * kSortThreads - 1) / (cluster * kSortThreads));
         fillers = fillers < sms - cluster ? fillers : sms - cluster;
         fillers = (fillers + cluster - 1) / cluster * cluster;
         if (cluster + fillers > sms) fillers -= cluster;
         uint2* sorted = reinterpret_cast<uint2*>(scratch + l.sorted[0]);
-        if (items <= 1) return launch_sort<1>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
-        if (items <= 2) return launch_sort<2>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
-        if (items <= 4) return launch_sort<4>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
-        if (items <= 8) return launch_sort<8>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
-        return launch_sort<kMostItems>(in, cluster, passes, width, sorted, fill, unit, fillers, s);
+        if (items <= 2) return launch_sort<2>(in, cluster, items, passes, width, sorted, fill, unit, fillers, s);
+        if (items <= 6) return launch_sort<6>(in, cluster, items, passes, width, sorted, fill, unit, fillers, s);
+        return launch_sort<kMostItems>(in, cluster, items, passes, width, sorted, fill, unit, fillers, s);
     }
     uint32_t* hist = reinterpret_cast<uint32_t*>(scratch + l.hist);
     const unsigned tiles = static_cast<unsigned>(l.sort_tiles);
@@ -695,14 +757,12 @@ int launch_sums(const SumArgs& a, const TI* grad, TO* out, cudaStream_t s)
     const int64_t blocks = ((a.tiles * a.slices << a.lanes_log2) + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffff) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding_grad: too many tokens");
     const unsigned g = static_cast<unsigned>(blocks);
-    auto fits = [&](int vec) {
-        return a.D % vec == 0 && rows_aligned(grad, a.grad_stride, sizeof(TI), vec) && rows_aligned(out, a.out_stride, sizeof(TO), vec);
-    };
-    constexpr int kWhole = sizeof(TI) == 4 ? 4 : 8, kSplit = sizeof(TI) == 4 ? 1 : 2;      // 16 bytes of an aligned row; a word of others
-    if (fits(kWhole)) sum_tiles_kernel<TI, TO, kWhole, INTO><<<g, kThreads, 0, s>>>(a, grad, out);
-    else sum_tiles_kernel<TI, TO, kSplit, INTO><<<g, kThreads, 0, s>>>(a, grad, out);
+    constexpr int kWhole = kVec<TI>;
+    const bool aligned = a.D % kWhole == 0 && rows_aligned(grad, a.grad_stride, sizeof(TI), kWhole) && rows_aligned(out, a.out_stride, sizeof(TO), kWhole);
+    if (aligned) sum_tiles_kernel<TI, TO, true, INTO><<<g, kThreads, 0, s>>>(a, grad, out);
+    else sum_tiles_kernel<TI, TO, false, INTO><<<g, kThreads, 0, s>>>(a, grad, out);
     if (const int rc = check_launch("sum_tiles_kernel")) return rc;
-    join_parts_kernel<TO, INTO><<<dim3(static_cast<unsigned>(a.tiles), static_cast<unsigned>((a.D + kJoinColumns - 1) / kJoinColumns)), kThreads, 0, s>>>(a, out);
+    join_parts_kernel<TO, INTO><<<dim3(static_cast<unsigned>(a.tiles), static_cast<unsigned>((a.D + kWarps * kJoinColumns - 1) / (kWarps * kJoinColumns))), kThreads, 0, s>>>(a, out);
     return check_launch("join_parts_kernel");
 }
 

@@ -227,7 +227,7 @@ public:
 // join) wait for the capture, and the process would not survive it: refused here, before anything is recorded.
 void check_capture(const Tensor& t, const char* op)
 {
-    if (!at::GradMode::is_enabled() || !t.requires_grad() || !t.is_leaf() || !t.is_cuda()) return;
+    if (!t.is_leaf() || !t.is_cuda()) return;
     const c10::cuda::CUDAGuard guard(t.device());
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
@@ -241,6 +241,10 @@ void check_capture(const Tensor& t, const char* op)
 Tensor token_embedding_autograd(const Tensor& weight, const Tensor& tokens, double scale, std::optional<int64_t> padding_idx,
                                 std::optional<int64_t> output_dtype)
 {
+    if (!(at::GradMode::is_enabled() && weight.requires_grad())) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return token_embedding_cuda(weight, tokens, scale, padding_idx, output_dtype);
+    }
     check_capture(weight, "token_embedding");
     return TokenEmbeddingFunction::apply(weight, tokens, scale, padding_idx, output_dtype);
 }
@@ -248,6 +252,10 @@ Tensor token_embedding_autograd(const Tensor& weight, const Tensor& tokens, doub
 Tensor token_embedding_grad_autograd(const Tensor& grad, const Tensor& tokens, int64_t num_embeddings, double scale,
                                      std::optional<int64_t> padding_idx, std::optional<int64_t> output_dtype)
 {
+    if (!(at::GradMode::is_enabled() && grad.requires_grad())) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return token_embedding_grad_cuda(grad, tokens, num_embeddings, scale, padding_idx, output_dtype);
+    }
     check_capture(grad, "token_embedding_grad");
     return TokenEmbeddingGradFunction::apply(grad, tokens, num_embeddings, scale, padding_idx, output_dtype);
 }
