@@ -151,17 +151,21 @@ constexpr int64_t kClusterKeys = int64_t(kSortBlocks) * kMostItems * kSortThread
 struct FillArgs {
     char* out;
     int64_t rows, row_bytes, stride_bytes;      // rows == 0: nothing to clear
+    int64_t early;                              // so many are cleared beside the sort, the others beside the sums
+    uint32_t* met;                              // a bit per row: tokens name it (null: early == rows)
 };
 
-constexpr int kZeroBytes = 32 * 1024;      // of shared memory that a clearing block keeps at zero and copies out
+// Shared memory that a clearing block keeps at zero and copies out, beside the sort and beside the sums.
+constexpr int kZeroBytes = 32 * 1024, kFewZeroBytes = 8 * 1024;
 
-// Clears `bytes` at p: thread `thread` of `threads` takes every threads-th run of kZeroBytes, by bulk copies from `zeros`; what
+// Clears `bytes` at p: thread `thread` of `threads` takes every threads-th run of ZEROS bytes, by bulk copies from `zeros`; what
 // lies in front of the first 16-byte border and behind the last goes element by element.
+template <int ZEROS>
 __device__ __forceinline__ void clear_run(char* p, int64_t bytes, int64_t thread, int64_t threads, int unit, const void* zeros)
 {
     const int64_t head = min((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15, bytes), body = (bytes - head) & ~int64_t(15);
-    for (int64_t at = thread * kZeroBytes; at < body; at += threads * kZeroBytes) {
-        const uint32_t run = static_cast<uint32_t>(body - at < kZeroBytes ? body - at : kZeroBytes);
+    for (int64_t at = thread * ZEROS; at < body; at += threads * ZEROS) {
+        const uint32_t run = static_cast<uint32_t>(body - at < ZEROS ? body - at : ZEROS);
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p + head + at), "r"(static_cast<uint32_t>(__cvta_generic_to_shared(zeros))),
                      "r"(run) : "memory");
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -174,16 +178,43 @@ __device__ __forceinline__ void clear_run(char* p, int64_t bytes, int64_t thread
     }
 }
 
-// A block's share of the rows; `zeros`: kZeroBytes of shared memory, 16-byte aligned.
-__device__ __forceinline__ void clear_rows(const FillArgs& f, int unit, int64_t block, int64_t blocks, unsigned char* zeros)
+template <int ZEROS>
+__device__ __forceinline__ void make_zeros(unsigned char* zeros)
 {
-    for (int i = threadIdx.x; i < kZeroBytes / 16; i += blockDim.x) reinterpret_cast<uint4*>(zeros)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = threadIdx.x; i < ZEROS / 16; i += blockDim.x) reinterpret_cast<uint4*>(zeros)[i] = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
+}
+
+// A block's share of the first `early` rows; `zeros`: kZeroBytes of shared memory, 16-byte aligned.
+__device__ __forceinline__ void clear_rows(const FillArgs& f, int unit, int64_t block, int64_t blocks, unsigned char* zeros)
+{
+    make_zeros<kZeroBytes>(zeros);
     if (f.stride_bytes == f.row_bytes) {
-        if (threadIdx.x == 0) clear_run(f.out, f.rows * f.row_bytes, block, blocks, unit, zeros);
+        if (threadIdx.x == 0) clear_run<kZeroBytes>(f.out, f.early * f.row_bytes, block, blocks, unit, zeros);
     } else {
-        for (int64_t r = block * blockDim.x + threadIdx.x; r < f.rows; r += blocks * blockDim.x) clear_run(f.out + r * f.stride_bytes, f.row_bytes, 0, 1, unit, zeros);
+        for (int64_t r = block * blockDim.x + threadIdx.x; r < f.early; r += blocks * blockDim.x)
+            clear_run<kZeroBytes>(f.out + r * f.stride_bytes, f.row_bytes, 0, 1, unit, zeros);
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// A block's share of the rows behind the first `early` (a multiple of 32) that no token names: a thread takes 32 rows.
+__device__ __forceinline__ void clear_unmet_rows(const FillArgs& f, int unit, int64_t block, int64_t blocks, unsigned char* zeros)
+{
+    make_zeros<kFewZeroBytes>(zeros);
+    const int64_t words = (f.rows + 31) / 32;
+    for (int64_t w = f.early / 32 + block + threadIdx.x * blocks; w < words; w += blocks * blockDim.x) {
+        const int64_t left = f.rows - w * 32;
+        uint32_t clear = ~__ldg(f.met + w) & (left < 32 ? (1u << left) - 1u : kFull);
+        while (clear) {
+            const int first = __ffs(clear) - 1;
+            const uint32_t behind = ~(clear >> first);
+            int run = behind ? __ffs(behind) - 1 : 32 - first;
+            if (f.stride_bytes != f.row_bytes) run = 1;
+            clear_run<kFewZeroBytes>(f.out + (w * 32 + first) * f.stride_bytes, run * f.row_bytes, 0, 1, unit, zeros);
+            clear &= run == 32 ? 0u : ~(((1u << run) - 1u) << first);
+        }
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
@@ -231,6 +262,8 @@ sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int w
         if (cluster > 1) cluster_sync();
         else __syncthreads();
     };
+    if (fill.met)
+        for (int64_t w = mine * kSortThreads + threadIdx.x; w < (fill.rows + 31) / 32; w += cluster * kSortThreads) fill.met[w] = 0u;
     if (cluster > 1) cluster_sync();      // every block has begun: its shared memory may be written
     for (int p = 0; p < passes; ++p) {
         uint32_t key[ITEMS], pos[ITEMS], rank[ITEMS];
@@ -295,7 +328,10 @@ sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int w
     }
     for (int i = threadIdx.x; i < per && first + i < in.n; i += kSortThreads) {
         const unsigned long long both = buf[i];
-        sorted[first + i] = make_uint2(static_cast<uint32_t>(both >> 32), static_cast<uint32_t>(both));
+        const uint32_t key = static_cast<uint32_t>(both >> 32);
+        sorted[first + i] = make_uint2(key, static_cast<uint32_t>(both));
+        // once per token and block at least; the words were cleared two barriers ago or more
+        if (fill.met && key < in.num_embeddings && (i == 0 || static_cast<uint32_t>(buf[i - 1] >> 32) != key)) atomicOr(fill.met + key / 32, 1u << (key & 31));
     }
 }
 
@@ -478,10 +514,15 @@ __device__ __forceinline__ void store_row(TO* row, const float (&v)[kColumns], i
 
 template <typename TI, typename TO, bool ALIGNED, bool INTO>
 __global__ void __launch_bounds__(kThreads)
-sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out)
+sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const FillArgs fill, int fillers)
 {
+    if (blockIdx.x < fillers) {
+        __shared__ __align__(16) unsigned char zeros[INTO ? 16 : kFewZeroBytes];
+        if constexpr (!INTO) clear_unmet_rows(fill, sizeof(TO), blockIdx.x, fillers, zeros);
+        return;
+    }
     const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const int64_t group = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> a.lanes_log2;
+    const int64_t group = (static_cast<int64_t>(blockIdx.x - fillers) * kThreads + threadIdx.x) >> a.lanes_log2;
     const int64_t tile = group / a.slices;
     const int slice = static_cast<int>(group - tile * a.slices);
     if (tile >= a.tiles) return;
@@ -653,12 +694,12 @@ int64_t align16(int64_t b) { return (b + 15) / 16 * 16; }
 // Where things lie in the scratch, and how the sums are cut: about as many groups of lanes as the GPU holds, each with a tile
 // and a slice of the columns.
 struct GradPlan {
-    int64_t sorted[2], hist, parts, total;
+    int64_t sorted[2], hist, met, parts, total;
     int64_t tiles, sort_tiles;
     int tile_rows, slices, lanes_log2, padded_D;
 };
 
-constexpr int64_t kResidentWarps = 148 * 24;
+constexpr int64_t kResidentWarps = 148 * 32;
 
 bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
 {
@@ -677,6 +718,7 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
     l.sorted[0] = at; at += align16(8 * n);
     l.sorted[1] = at; at += l.sort_tiles ? align16(8 * n) : 0;
     l.hist = at; at += align16(4 * kMaxBins * l.sort_tiles);
+    l.met = at; at += align16((num_embeddings + 31) / 32 * 4);
     l.parts = at; at += l.tiles * 2 * l.padded_D * 4;
     l.total = at;
     return true;
@@ -711,7 +753,7 @@ int sort_and_clear(const SortInput& in, const GradPlan& l, char* scratch, const 
 {
     half = 0;
     // blocks that clear: 64 KB each at least, one per multiprocessor at most
-    int64_t fillers = (fill.rows * fill.row_bytes + 65535) / 65536;
+    int64_t fillers = (fill.early * fill.row_bytes + 65535) / 65536;
     const int sms = sm_count();
     if (in.n == 0 || in.n > kClusterKeys) {
         if (fillers) {
@@ -752,15 +794,16 @@ int sort_and_clear(const SortInput& in, const GradPlan& l, char* scratch, const 
 }
 
 template <typename TI, typename TO, bool INTO>
-int launch_sums(const SumArgs& a, const TI* grad, TO* out, cudaStream_t s)
+int launch_sums(const SumArgs& a, const TI* grad, TO* out, const FillArgs& fill, cudaStream_t s)
 {
+    const int fillers = fill.early < fill.rows ? sm_count() : 0;
     const int64_t blocks = ((a.tiles * a.slices << a.lanes_log2) + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffff) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding_grad: too many tokens");
-    const unsigned g = static_cast<unsigned>(blocks);
+    if (blocks > 0x7fffffff - fillers) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding_grad: too many tokens");
+    const unsigned g = static_cast<unsigned>(blocks + fillers);
     constexpr int kWhole = kVec<TI>;
     const bool aligned = a.D % kWhole == 0 && rows_aligned(grad, a.grad_stride, sizeof(TI), kWhole) && rows_aligned(out, a.out_stride, sizeof(TO), kWhole);
-    if (aligned) sum_tiles_kernel<TI, TO, true, INTO><<<g, kThreads, 0, s>>>(a, grad, out);
-    else sum_tiles_kernel<TI, TO, false, INTO><<<g, kThreads, 0, s>>>(a, grad, out);
+    if (aligned) sum_tiles_kernel<TI, TO, true, INTO><<<g, kThreads, 0, s>>>(a, grad, out, fill, fillers);
+    else sum_tiles_kernel<TI, TO, false, INTO><<<g, kThreads, 0, s>>>(a, grad, out, fill, fillers);
     if (const int rc = check_launch("sum_tiles_kernel")) return rc;
     join_parts_kernel<TO, INTO><<<dim3(static_cast<unsigned>(a.tiles), static_cast<unsigned>((a.D + kWarps * kJoinColumns - 1) / (kWarps * kJoinColumns))), kThreads, 0, s>>>(a, out);
     return check_launch("join_parts_kernel");
@@ -823,7 +866,17 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     char* base = static_cast<char*>(scratch);
     const SortInput in{tokens, token_bits == 64, n, num_embeddings, padding_idx};
-    const FillArgs fill{static_cast<char*>(grad_weight), accumulate ? 0 : num_embeddings, D * ob, grad_weight_stride * ob};
+    FillArgs fill{static_cast<char*>(grad_weight), accumulate ? 0 : num_embeddings, D * ob, grad_weight_stride * ob, 0, nullptr};
+    fill.early = fill.rows;
+    if (n > 0 && n <= kClusterKeys) {
+        // Writing alone runs at 4 TB/s, beside reads at most of what a copy writes: the sums' reads cost little then.  As many rows
+        // are cleared beside the sort as that takes; where little is left, all.
+        const int64_t beside_sort = ((int64_t(36) << 20) + n * 1400) / fill.row_bytes / 32 * 32;
+        if (beside_sort + beside_sort / 4 < fill.rows) {
+            fill.early = beside_sort;
+            fill.met = reinterpret_cast<uint32_t*>(base + l.met);
+        }
+    }
     int half;
     if (const int rc = sort_and_clear(in, l, base, fill, ob, half, s)) return rc;
     if (n == 0) return TBE_B200_OK;
@@ -833,8 +886,8 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
         return with_element(grad_dtype, [&](auto* ti) {
             using TO = std::remove_pointer_t<decltype(to)>;
             using TI = std::remove_pointer_t<decltype(ti)>;
-            if (accumulate) return launch_sums<TI, TO, true>(a, static_cast<const TI*>(grad), static_cast<TO*>(grad_weight), s);
-            return launch_sums<TI, TO, false>(a, static_cast<const TI*>(grad), static_cast<TO*>(grad_weight), s);
+            if (accumulate) return launch_sums<TI, TO, true>(a, static_cast<const TI*>(grad), static_cast<TO*>(grad_weight), fill, s);
+            return launch_sums<TI, TO, false>(a, static_cast<const TI*>(grad), static_cast<TO*>(grad_weight), fill, s);
         });
     });
 }

@@ -185,6 +185,36 @@ def test_grad(n, V, D, kind):
         assert torch.equal(got, again)                            # the order of the sums is fixed
 
 
+@pytest.mark.parametrize("n,V,D,ti,to", [(700, 300_007, 64, F32, F32), (5000, 300_007, 101, BF16, F16), (70_000, 150_000, 128, BF16, F32),
+                                         (1, 1_000_033, 32, F16, F32), (200_000, 400_000, 64, F32, BF16)])
+@pytest.mark.parametrize("kind", ["uniform", "hot", "wild", "none"])
+def test_grad_of_a_large_table(n, V, D, ti, to, kind):
+    """Tables whose rows are cleared partly beside the sums, where no token names them."""
+    g = gen(n)
+    dy, t = randn(g, n, D, dtype=ti, std=0.01), tokens_of(g, n, V, kind, torch.int64)
+    junk = torch.full((V, D), float("nan"), device="cuda", dtype=to)          # what the allocator hands out next
+    del junk
+    got = ops().token_embedding_grad(dy, t, V, padding_idx=7, output_dtype=CODE[to])
+    want, mass, count = grad64(dy, t, V, 1.0, 7)
+    within(got, want, grad_bound(want, mass, count, to))
+    assert bool((got[(count == 0)[:, 0]] == 0).all())
+
+
+@pytest.mark.parametrize("n,V,D,stride", [(900, 60_000, 200, 264), (900, 60_000, 199, 201), (40, 77, 8, 9)])
+def test_grad_into_rows_that_lie_apart(n, V, D, stride):
+    """The C entry point over a wider buffer: every row is written, nothing between the rows."""
+    from fbgemm_ascend_b200 import cabi
+    g = gen(n)
+    lib = cabi.lib()
+    dy, t = randn(g, n, D), tokens_of(g, n, V, "hot", torch.int64)
+    out = torch.full((V, stride), 7.0, device="cuda")
+    need = lib.tbe_b200_token_embedding_grad_scratch_bytes(n, V, D)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    cabi.check(lib.tbe_b200_token_embedding_grad(dy.data_ptr(), 0, D, t.data_ptr(), 64, n, V, D, 2.0, -1, 0, out.data_ptr(), 0, stride, scratch.data_ptr(),
+                                                 need, torch.cuda.current_stream().cuda_stream), "grad")
+    assert torch.equal(out[:, :D], ops().token_embedding_grad(dy, t, V, scale=2.0)) and bool((out[:, D:] == 7.0).all())
+
+
 @pytest.mark.parametrize("n,V,D,kind", [(1, 9, 8, "same"), (500, 60, 40, "hot"), (4097, 300, 1001, "wild"), (5000, 100_000, 64, "uniform"),
                                         (300, 40, 33, "same"), (40, 9, 16, "none")])
 @pytest.mark.parametrize("ti,to", [(BF16, F32), (F32, F32), (BF16, BF16), (F16, F16)])
