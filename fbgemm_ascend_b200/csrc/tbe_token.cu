@@ -19,64 +19,97 @@ __device__ __forceinline__ int64_t load_token(const void* tokens, bool wide, int
 
 // ---- lookup ---------------------------------------------------------------------------------------------------
 //
-// `lanes` threads (a power of two, at most the block) share a row and walk its pieces; a thread holds ROWS rows' pieces
-// at a time, so that a block has ROWS * 16 bytes per thread in flight.
-template <typename TI, typename TO, int VEC, int ROWS>
+// `lanes` threads (a power of two, at most the block) share a row and walk its pieces of VEC elements; a thread holds ROWS
+// rows' pieces at a time, so that a block has ROWS * 16 bytes per thread in flight.
+//
+// ALIGNED: rows of both sides can be moved in pieces of so many elements.  0: they cannot; pieces are cut by the result's 16-byte borders, so that
+// it is still written in whole ones but for a row's two ends, and what goes into them is read in aligned words and shifted.
+template <typename TI, typename TO, int ALIGNED, int ROWS>
 __global__ void __launch_bounds__(kThreads)
-token_embedding_kernel(const TI* __restrict__ weight, int64_t num_embeddings, int pieces, int64_t weight_stride, const void* __restrict__ tokens,
-                       int wide, int64_t n, float scale, TO* __restrict__ out, int64_t out_stride, int lanes_log2, int32_t* error_flag)
+token_embedding_kernel(const TI* __restrict__ weight, int64_t num_embeddings, int D, int64_t weight_stride, const void* __restrict__ tokens, int wide,
+                       int64_t n, float scale, TO* __restrict__ out, int64_t out_stride, int lanes_log2, int32_t* error_flag)
 {
+    constexpr int VEC = ALIGNED ? ALIGNED : 16 / static_cast<int>(sizeof(TO));
     const int lanes = 1 << lanes_log2, k = threadIdx.x & (lanes - 1);
     const int rows_at_once = kThreads >> lanes_log2;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * (rows_at_once * ROWS) + (threadIdx.x >> lanes_log2);
     const TI* src[ROWS];
+    TO* to[ROWS];
+    int lead[ROWS];      // elements in front of the result's first border, with those of a piece that starts in front of the row
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
         const int64_t i = first + static_cast<int64_t>(j) * rows_at_once;
         src[j] = nullptr;
+        to[j] = nullptr;
+        lead[j] = 0;
         if (i < n) {
             const int64_t t = load_token(tokens, wide, i);
             if (t >= 0 && t < num_embeddings) src[j] = weight + t * weight_stride;
             else if (t != -1 && error_flag && k == 0) atomicOr(error_flag, 4);
+            to[j] = out + i * out_stride;
+            if constexpr (!ALIGNED) lead[j] = static_cast<int>((reinterpret_cast<uintptr_t>(to[j]) & 15) / sizeof(TO));
         }
     }
-    for (int c = k; c < pieces; c += lanes) {
-        Piece<TI, VEC> p[ROWS];
+    const int pieces = (D + (ALIGNED ? 0 : VEC - 1) + VEC - 1) / VEC;
+    for (int p = k; p < pieces; p += lanes) {
+        typename std::conditional<ALIGNED, Piece<TI, VEC>, SplitPiece<TI, VEC>>::type in[ROWS];
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            if (src[j]) load_piece<TI, VEC>(p[j], src[j] + static_cast<int64_t>(c) * VEC);
-            else clear_piece(p[j]);
+            if constexpr (ALIGNED) {
+                if (src[j]) load_piece<TI, VEC>(in[j], src[j] + static_cast<int64_t>(p) * VEC);
+                else clear_piece(in[j]);
+            } else {
+                // a piece that begins in front of the row is read from the row's first element on
+                const int c = p * VEC - lead[j], from = c < 0 ? 0 : c;
+                if (src[j] && from < D) in[j].load(src[j] + from, src[j] + D);
+            }
         }
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            const int64_t i = first + static_cast<int64_t>(j) * rows_at_once;
-            if (i >= n) continue;
+            if (!to[j]) continue;
             float v[VEC];
+            if constexpr (ALIGNED) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = src[j] ? scale * element(p[j], e) : 0.0f;
-            store_piece<TO, VEC>(out + i * out_stride + static_cast<int64_t>(c) * VEC, v);
+                for (int e = 0; e < VEC; ++e) v[e] = src[j] ? scale * element(in[j], e) : 0.0f;
+                store_piece<TO, VEC>(to[j] + static_cast<int64_t>(p) * VEC, v);
+            } else {
+                const int c = p * VEC - lead[j];
+                if (c >= D) continue;
+                Piece<TI, VEC> r;
+                if (src[j]) r = in[j].piece();
+                else clear_piece(r);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] = src[j] ? scale * element(r, e) : 0.0f;
+                if (c >= 0 && c + VEC <= D) {
+                    store_piece<TO, VEC>(to[j] + c, v);
+                } else {
+                    const int from = c < 0 ? 0 : c, most = c + VEC < D ? c + VEC : D;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float one[1] = {v[e]};
+                        if (from + e < most) store_piece<TO, 1>(to[j] + from + e, one);
+                    }
+                }
+            }
         }
     }
 }
 
-template <typename TI, typename TO, int VEC>
+template <typename TI, typename TO, int ALIGNED>
 int launch_token_embedding(const TI* weight, int64_t num_embeddings, int64_t D, int64_t weight_stride, const void* tokens, int wide, int64_t n,
                            float scale, TO* out, int64_t out_stride, int32_t* error_flag, cudaStream_t s)
 {
-    const int pieces = static_cast<int>(D / VEC);
+    constexpr int VEC = ALIGNED ? ALIGNED : 16 / static_cast<int>(sizeof(TO)), kRows = ALIGNED ? 4 : 2;
+    const int64_t pieces = (D + VEC - 1) / VEC;
     int lanes_log2 = 0;
     while ((1 << lanes_log2) < pieces && (1 << lanes_log2) < kThreads) ++lanes_log2;
     const int at_once = kThreads >> lanes_log2;
-    const bool many = n >= static_cast<int64_t>(sm_count()) * 8 * at_once * 4;
-    const int64_t per = static_cast<int64_t>(at_once) * (many ? 4 : 1);
-    const int64_t blocks = (n + per - 1) / per;
+    const bool many = n >= static_cast<int64_t>(sm_count()) * 8 * at_once * kRows;
+    const int64_t per = static_cast<int64_t>(at_once) * (many ? kRows : 1), blocks = (n + per - 1) / per;
     if (blocks > 0x7fffffff) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding: too many tokens");
-    if (many)
-        token_embedding_kernel<TI, TO, VEC, 4><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(
-            weight, num_embeddings, pieces, weight_stride, tokens, wide, n, scale, out, out_stride, lanes_log2, error_flag);
-    else
-        token_embedding_kernel<TI, TO, VEC, 1><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(
-            weight, num_embeddings, pieces, weight_stride, tokens, wide, n, scale, out, out_stride, lanes_log2, error_flag);
+    auto* kernel = many ? token_embedding_kernel<TI, TO, ALIGNED, kRows> : token_embedding_kernel<TI, TO, ALIGNED, 1>;
+    kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(weight, num_embeddings, static_cast<int>(D), weight_stride, tokens, wide, n, scale, out,
+                                                              out_stride, lanes_log2, error_flag);
     return check_launch("token_embedding_kernel");
 }
 
@@ -821,7 +854,7 @@ extern "C" int tbe_b200_token_embedding(const void* weight, int32_t weight_dtype
     const int ib = element_bytes(weight_dtype), ob = element_bytes(output_dtype);
     if (!ib || !ob) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding: element types FP32, FP16 and BF16, got %d and %d", weight_dtype, output_dtype);
     if (token_bits != 32 && token_bits != 64) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: token_bits must be 32 or 64, got %d", token_bits);
-    if (n < 0 || D < 0 || num_embeddings < 0 || D > 0x7fffffff) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: size out of range");
+    if (n < 0 || D < 0 || num_embeddings < 0 || D > 0x40000000) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: size out of range");
     if (weight_stride < D || output_stride < D) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: row strides must be at least D");
     if (n == 0 || D == 0) return TBE_B200_OK;
     if (!tokens || !output || (num_embeddings > 0 && !weight)) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: NULL pointer");
@@ -836,7 +869,7 @@ extern "C" int tbe_b200_token_embedding(const void* weight, int32_t weight_dtype
             auto fits = [&](int vec) { return D % vec == 0 && rows_aligned(w, weight_stride, ib, vec) && rows_aligned(o, output_stride, ob, vec); };
             if (fits(8)) return launch_token_embedding<TI, TO, 8>(w, num_embeddings, D, weight_stride, tokens, wide, n, scale, o, output_stride, error_flag, s);
             if (fits(4)) return launch_token_embedding<TI, TO, 4>(w, num_embeddings, D, weight_stride, tokens, wide, n, scale, o, output_stride, error_flag, s);
-            return launch_token_embedding<TI, TO, 1>(w, num_embeddings, D, weight_stride, tokens, wide, n, scale, o, output_stride, error_flag, s);
+            return launch_token_embedding<TI, TO, 0>(w, num_embeddings, D, weight_stride, tokens, wide, n, scale, o, output_stride, error_flag, s);
         });
     });
 }
