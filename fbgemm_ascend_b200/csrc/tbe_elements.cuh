@@ -50,22 +50,38 @@ __device__ __forceinline__ void clear_piece(Piece<T, VEC>& r)
     for (int i = 0; i < Piece<T, VEC>::kWords; ++i) r.w[i] = 0u;
 }
 
-// A piece that may start at any element and reach past `end` (the address behind its row): read in aligned 16-byte words, none of
-// which lies wholly outside the row, and shifted into place.  What is not the row's is left as it is there.
+// A row that starts at any element: the 16-byte border in front of it, and where it begins and ends behind that, bytes.
+struct SplitRow {
+    const char* base;
+    int begin, end;
+
+    template <typename T>
+    __device__ __forceinline__ void of(const T* row, int D)
+    {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(row);
+        base = reinterpret_cast<const char*>(a & ~uintptr_t(15));
+        begin = static_cast<int>(a & 15);
+        end = begin + D * static_cast<int>(sizeof(T));
+    }
+};
+
+// A piece of such a row, which may reach past its end: read in aligned 16-byte words, none of which lies wholly outside the
+// row, and shifted into place.  What is not the row's is left as it is there.
 template <typename T, int VEC>
 struct SplitPiece {
     static constexpr int kBytes = Piece<T, VEC>::kBytes;
     static constexpr int kQuads = (kBytes + 15) / 16 + 1;
     uint4 q[kQuads];
-    uint32_t offset;      // of the first element in the first word, bytes
+    int offset;      // of the first element in the first word, bytes
 
-    __device__ __forceinline__ void load(const T* p, const T* end)
+    // from element c on; c at most the row's number of elements
+    __device__ __forceinline__ void load(const SplitRow& row, int c)
     {
-        const uintptr_t a = reinterpret_cast<uintptr_t>(p), e = reinterpret_cast<uintptr_t>(end);
-        offset = static_cast<uint32_t>(a & 15);
-        const uintptr_t first = a & ~uintptr_t(15), behind = a + kBytes < e ? a + kBytes : e;
+        const int at = row.begin + c * static_cast<int>(sizeof(T)), first = at & ~15, behind = at + kBytes < row.end ? at + kBytes : row.end;
+        offset = at & 15;
+        const char* p = row.base + first;
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) q[i] = first + 16 * i < behind ? ldg16(reinterpret_cast<const void*>(first + 16 * i)) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < kQuads; ++i) q[i] = first + 16 * i < behind ? ldg16(p + 16 * i) : make_uint4(0u, 0u, 0u, 0u);
     }
     __device__ __forceinline__ Piece<T, VEC> piece() const
     {

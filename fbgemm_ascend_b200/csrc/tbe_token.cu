@@ -34,6 +34,7 @@ token_embedding_kernel(const TI* __restrict__ weight, int64_t num_embeddings, in
     const int rows_at_once = kThreads >> lanes_log2;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * (rows_at_once * ROWS) + (threadIdx.x >> lanes_log2);
     const TI* src[ROWS];
+    SplitRow split[ROWS];
     TO* to[ROWS];
     int lead[ROWS];      // elements in front of the result's first border, with those of a piece that starts in front of the row
 #pragma unroll
@@ -47,7 +48,10 @@ token_embedding_kernel(const TI* __restrict__ weight, int64_t num_embeddings, in
             if (t >= 0 && t < num_embeddings) src[j] = weight + t * weight_stride;
             else if (t != -1 && error_flag && k == 0) atomicOr(error_flag, 4);
             to[j] = out + i * out_stride;
-            if constexpr (!ALIGNED) lead[j] = static_cast<int>((reinterpret_cast<uintptr_t>(to[j]) & 15) / sizeof(TO));
+            if constexpr (!ALIGNED) {
+                lead[j] = static_cast<int>((reinterpret_cast<uintptr_t>(to[j]) & 15) / sizeof(TO));
+                split[j].of(src[j], D);
+            }
         }
     }
     const int pieces = (D + (ALIGNED ? 0 : VEC - 1) + VEC - 1) / VEC;
@@ -61,7 +65,7 @@ token_embedding_kernel(const TI* __restrict__ weight, int64_t num_embeddings, in
             } else {
                 // a piece that begins in front of the row is read from the row's first element on
                 const int c = p * VEC - lead[j], from = c < 0 ? 0 : c;
-                if (src[j] && from < D) in[j].load(src[j] + from, src[j] + D);
+                if (src[j] && from < D) in[j].load(split[j], from);
             }
         }
 #pragma unroll
@@ -491,6 +495,8 @@ struct Columns {
 
     __device__ __forceinline__ void load(const T* row, int column, int step, int D)
     {
+        SplitRow split;
+        if constexpr (!ALIGNED) split.of(row, D);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int c = column + i * step;
@@ -498,7 +504,7 @@ struct Columns {
                 if (c < D) load_piece<T, VEC>(p[i], row + c);
                 else clear_piece(p[i]);
             } else {
-                p[i].load(row + (c < D ? c : D), row + D);
+                p[i].load(split, c < D ? c : D);
             }
         }
     }
@@ -854,7 +860,7 @@ extern "C" int tbe_b200_token_embedding(const void* weight, int32_t weight_dtype
     const int ib = element_bytes(weight_dtype), ob = element_bytes(output_dtype);
     if (!ib || !ob) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding: element types FP32, FP16 and BF16, got %d and %d", weight_dtype, output_dtype);
     if (token_bits != 32 && token_bits != 64) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: token_bits must be 32 or 64, got %d", token_bits);
-    if (n < 0 || D < 0 || num_embeddings < 0 || D > 0x40000000) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: size out of range");
+    if (n < 0 || D < 0 || num_embeddings < 0 || D > 0x10000000) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: size out of range");
     if (weight_stride < D || output_stride < D) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: row strides must be at least D");
     if (n == 0 || D == 0) return TBE_B200_OK;
     if (!tokens || !output || (num_embeddings > 0 && !weight)) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding: NULL pointer");
