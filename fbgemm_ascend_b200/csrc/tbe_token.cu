@@ -21,100 +21,117 @@ __device__ __forceinline__ int64_t load_token(const void* tokens, bool wide, int
 //
 // `lanes` threads (a power of two, at most the block) share a row and walk its pieces of VEC elements; a thread holds ROWS
 // rows' pieces at a time, so that a block has ROWS * 16 bytes per thread in flight.
-//
-// ALIGNED: rows of both sides can be moved in pieces of so many elements.  0: they cannot; pieces are cut by the result's 16-byte borders, so that
-// it is still written in whole ones but for a row's two ends, and what goes into them is read in aligned words and shifted.
-template <typename TI, typename TO, int ALIGNED, int ROWS>
+__device__ __forceinline__ const char* row_of_token(const void* weight, int64_t row_bytes, int64_t num_embeddings, const void* tokens, int wide, int64_t i,
+                                                    bool report, int32_t* error_flag)
+{
+    const int64_t t = load_token(tokens, wide, i);
+    if (t >= 0 && t < num_embeddings) return static_cast<const char*>(weight) + t * row_bytes;
+    if (t != -1 && error_flag && report) atomicOr(error_flag, 4);
+    return nullptr;
+}
+
+template <typename TI, typename TO, int VEC, int ROWS>
 __global__ void __launch_bounds__(kThreads)
 token_embedding_kernel(const TI* __restrict__ weight, int64_t num_embeddings, int D, int64_t weight_stride, const void* __restrict__ tokens, int wide,
                        int64_t n, float scale, TO* __restrict__ out, int64_t out_stride, int lanes_log2, int32_t* error_flag)
 {
-    constexpr int VEC = ALIGNED ? ALIGNED : 16 / static_cast<int>(sizeof(TO));
-    const int lanes = 1 << lanes_log2, k = threadIdx.x & (lanes - 1);
+    const int lanes = 1 << lanes_log2, k = threadIdx.x & (lanes - 1), pieces = D / VEC;
     const int rows_at_once = kThreads >> lanes_log2;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * (rows_at_once * ROWS) + (threadIdx.x >> lanes_log2);
     const TI* src[ROWS];
-    SplitRow split[ROWS];
-    TO* to[ROWS];
-    int lead[ROWS];      // elements in front of the result's first border, with those of a piece that starts in front of the row
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
         const int64_t i = first + static_cast<int64_t>(j) * rows_at_once;
-        src[j] = nullptr;
-        to[j] = nullptr;
-        lead[j] = 0;
-        if (i < n) {
-            const int64_t t = load_token(tokens, wide, i);
-            if (t >= 0 && t < num_embeddings) src[j] = weight + t * weight_stride;
-            else if (t != -1 && error_flag && k == 0) atomicOr(error_flag, 4);
-            to[j] = out + i * out_stride;
-            if constexpr (!ALIGNED) {
-                lead[j] = static_cast<int>((reinterpret_cast<uintptr_t>(to[j]) & 15) / sizeof(TO));
-                split[j].of(src[j], D);
-            }
-        }
+        src[j] = i < n ? reinterpret_cast<const TI*>(row_of_token(weight, weight_stride * sizeof(TI), num_embeddings, tokens, wide, i, k == 0, error_flag)) : nullptr;
     }
-    const int pieces = (D + (ALIGNED ? 0 : VEC - 1) + VEC - 1) / VEC;
     for (int p = k; p < pieces; p += lanes) {
-        typename std::conditional<ALIGNED, Piece<TI, VEC>, SplitPiece<TI, VEC>>::type in[ROWS];
+        Piece<TI, VEC> in[ROWS];
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            if constexpr (ALIGNED) {
-                if (src[j]) load_piece<TI, VEC>(in[j], src[j] + static_cast<int64_t>(p) * VEC);
-                else clear_piece(in[j]);
-            } else {
-                // a piece that begins in front of the row is read from the row's first element on
-                const int c = p * VEC - lead[j], from = c < 0 ? 0 : c;
-                if (src[j] && from < D) in[j].load(split[j], from);
-            }
+            if (src[j]) load_piece<TI, VEC>(in[j], src[j] + static_cast<int64_t>(p) * VEC);
+            else clear_piece(in[j]);
         }
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            if (!to[j]) continue;
+            const int64_t i = first + static_cast<int64_t>(j) * rows_at_once;
+            if (i >= n) continue;
             float v[VEC];
-            if constexpr (ALIGNED) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = src[j] ? scale * element(in[j], e) : 0.0f;
-                store_piece<TO, VEC>(to[j] + static_cast<int64_t>(p) * VEC, v);
-            } else {
-                const int c = p * VEC - lead[j];
-                if (c >= D) continue;
-                Piece<TI, VEC> r;
-                if (src[j]) r = in[j].piece();
-                else clear_piece(r);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = src[j] ? scale * element(r, e) : 0.0f;
-                if (c >= 0 && c + VEC <= D) {
-                    store_piece<TO, VEC>(to[j] + c, v);
-                } else {
-                    const int from = c < 0 ? 0 : c, most = c + VEC < D ? c + VEC : D;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float one[1] = {v[e]};
-                        if (from + e < most) store_piece<TO, 1>(to[j] + from + e, one);
-                    }
-                }
-            }
+            for (int e = 0; e < VEC; ++e) v[e] = src[j] ? scale * element(in[j], e) : 0.0f;
+            store_piece<TO, VEC>(out + i * out_stride + static_cast<int64_t>(p) * VEC, v);
         }
     }
 }
 
-template <typename TI, typename TO, int ALIGNED>
+// Rows that cannot be moved in pieces.  Cut by the result's 16-byte borders, all but the ends of a row is still written in whole
+// pieces, and what goes into them is read in aligned words and shifted; a lane has kSplitAtOnce of them in flight.  The ends go
+// element by element.  At most a warp shares a row: what a row costs beside its pieces is a good part of the instructions, which
+// bound this form.
+constexpr int kSplitAtOnce = 4;
+
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(kThreads)
+token_embedding_split_kernel(const TI* __restrict__ weight, int64_t num_embeddings, int D, int64_t weight_stride, const void* __restrict__ tokens, int wide,
+                             int64_t n, float scale, TO* __restrict__ out, int64_t out_stride, int lanes_log2, int32_t* error_flag)
+{
+    constexpr int VEC = 16 / static_cast<int>(sizeof(TO));
+    const int lanes = 1 << lanes_log2, k = threadIdx.x & (lanes - 1);
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> lanes_log2;
+    if (i >= n) return;
+    const TI* src = reinterpret_cast<const TI*>(row_of_token(weight, weight_stride * sizeof(TI), num_embeddings, tokens, wide, i, k == 0, error_flag));
+    TO* to = out + i * out_stride;
+    int head = static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(to) & 15)) & 15) / sizeof(TO));
+    head = head < D ? head : D;
+    const int whole = (D - head) / VEC, ends = D - whole * VEC;
+    SplitRow split;
+    split.of(src, D);
+    for (int p = k; p < whole; p += kSplitAtOnce * lanes) {
+        SplitPiece<TI, VEC> in[kSplitAtOnce];
+#pragma unroll
+        for (int j = 0; j < kSplitAtOnce; ++j)
+            if (src && p + j * lanes < whole) in[j].load(split, head + (p + j * lanes) * VEC);
+#pragma unroll
+        for (int j = 0; j < kSplitAtOnce; ++j) {
+            if (p + j * lanes >= whole) break;
+            float v[VEC] = {};
+            if (src) {
+                const Piece<TI, VEC> r = in[j].piece();
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] = scale * element(r, e);
+            }
+            store_piece<TO, VEC>(to + head + (p + j * lanes) * VEC, v);
+        }
+    }
+    for (int e = k; e < ends; e += lanes) {
+        const int c = e < head ? e : whole * VEC + e;
+        Piece<TI, 1> r;
+        clear_piece(r);
+        if (src) load_piece<TI, 1>(r, src + c);
+        const float v[1] = {src ? scale * element(r, 0) : 0.0f};
+        store_piece<TO, 1>(to + c, v);
+    }
+}
+
+template <typename TI, typename TO, int VEC>
 int launch_token_embedding(const TI* weight, int64_t num_embeddings, int64_t D, int64_t weight_stride, const void* tokens, int wide, int64_t n,
                            float scale, TO* out, int64_t out_stride, int32_t* error_flag, cudaStream_t s)
 {
-    constexpr int VEC = ALIGNED ? ALIGNED : 16 / static_cast<int>(sizeof(TO)), kRows = ALIGNED ? 4 : 2;
-    const int64_t pieces = (D + VEC - 1) / VEC;
+    const int64_t pieces = VEC ? D / (VEC ? VEC : 1) : D / (16 / static_cast<int64_t>(sizeof(TO)));
+    const bool few = n <= static_cast<int64_t>(sm_count()) * 8;      // rows: as many threads to each as there are
+    const int most = VEC || few ? kThreads : 32, share = VEC || few ? 1 : kSplitAtOnce;
     int lanes_log2 = 0;
-    while ((1 << lanes_log2) < pieces && (1 << lanes_log2) < kThreads) ++lanes_log2;
+    while ((share << lanes_log2) < pieces && (1 << lanes_log2) < most) ++lanes_log2;
     const int at_once = kThreads >> lanes_log2;
-    const bool many = n >= static_cast<int64_t>(sm_count()) * 8 * at_once * kRows;
-    const int64_t per = static_cast<int64_t>(at_once) * (many ? kRows : 1), blocks = (n + per - 1) / per;
+    const bool many = VEC && n >= static_cast<int64_t>(sm_count()) * 8 * at_once * 4;
+    const int64_t per = static_cast<int64_t>(at_once) * (many ? 4 : 1), blocks = (n + per - 1) / per;
     if (blocks > 0x7fffffff) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding: too many tokens");
-    auto* kernel = many ? token_embedding_kernel<TI, TO, ALIGNED, kRows> : token_embedding_kernel<TI, TO, ALIGNED, 1>;
-    kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(weight, num_embeddings, static_cast<int>(D), weight_stride, tokens, wide, n, scale, out,
-                                                              out_stride, lanes_log2, error_flag);
-    return check_launch("token_embedding_kernel");
+    auto launch = [&](auto* kernel) {
+        kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(weight, num_embeddings, static_cast<int>(D), weight_stride, tokens, wide, n, scale, out,
+                                                                  out_stride, lanes_log2, error_flag);
+        return check_launch("token_embedding_kernel");
+    };
+    if constexpr (VEC == 0) return launch(token_embedding_split_kernel<TI, TO>);
+    else return many ? launch(token_embedding_kernel<TI, TO, VEC, 4>) : launch(token_embedding_kernel<TI, TO, VEC, 1>);
 }
 
 // ---- gradient: sort by token ----------------------------------------------------------------------------------
