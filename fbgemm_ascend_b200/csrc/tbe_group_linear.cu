@@ -81,54 +81,48 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 // A state's elements become fp16: as they are, or times the power of two that brings the state's largest into 2^14 .. 2^15
 // (bf16 keeps its 8 bits then, but for elements below 2^-28 of the largest, which are off by 2^-40 of it at most); fp32 in
 // two pieces, 22 bits and a sign, off by 2^-23 at most.  The sums are scaled back.
-// For NT * 8 states and a unit of 128 elements: four steps of NT sets of P pieces of 512 bytes, 16 to each lane, then the
-// sums of the states over every group of the unit.
+//
+// For a unit of 128 elements: four steps, in each 64 bytes per state and piece, 16 to each of four lanes; then the sums of the
+// states over every group of the unit.  A block that arranges the states itself (LOCAL) keeps only those that there are; else
+// there is room for NT * 8.
 template <typename T> constexpr int kPieces = sizeof(T) == 4 ? 2 : 1;
 
 __host__ __device__ constexpr int sums_bytes(int NT, int steps) { return 4 / steps * NT * 32; }
 __host__ __device__ constexpr int unit_bytes(int NT, int P, int steps) { return P * NT * 2048 + sums_bytes(NT, steps); }
+__host__ __device__ constexpr int local_unit_bytes(int cols, int NT, int P, int steps) { return P * cols * 256 + sums_bytes(NT, steps); }
 
-constexpr int kStateThreads = 512;
+__device__ __forceinline__ int largest_bits(float v) { return static_cast<int>(__float_as_uint(v) & 0x7fffffffu); }      // magnitudes order like their bits
 
-// One block per state.
+// 2^e with 14 - e the exponent of the largest, both ways within fp32's normal numbers.
+__device__ __forceinline__ int scale_exponent(int largest) { return min(126, 14 - ((largest >> 23) - 127)); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
+// The largest magnitude among elements `first` on, 8 at a time and `stride` words of 8 apart, of a row of D.
 template <typename T>
-__global__ void __launch_bounds__(kStateThreads)
-arrange_states_kernel(const T* __restrict__ x, int64_t x_stride, int D, int NT, int steps, unsigned char* __restrict__ arranged, float* __restrict__ back)
+__device__ __forceinline__ int largest_of(const T* row, int D, int first, int stride)
+{
+    int most = 0;
+    for (int i = first; i < D / 8; i += stride) {
+        Piece<T, 8> r;
+        load_piece<T, 8>(r, row + i * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max(most, largest_bits(element(r, e)));
+    }
+    return __reduce_max_sync(kFull, most);
+}
+
+// Words of 8 elements `first`, `first` + stride ... of a state (whole warps, neighbouring lanes neighbouring words).  Where word
+// (step, t) of unit u goes: at(u, step, piece, t); where the sum of the unit's group k goes: sum_at(u, k).
+template <typename T, int STEPS, typename At, typename SumAt>
+__device__ __forceinline__ void arrange_words(const T* row, int D, float scale, int first, int stride, At at, SumAt sum_at)
 {
     constexpr int P = kPieces<T>;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int m = blockIdx.x, units = (D + kUnit - 1) / kUnit, words = units * (kUnit / 8);
-    const T* row = x + m * x_stride;
-    float scale = 1.0f;
-    if constexpr (!std::is_same<T, __half>::value) {
-        __shared__ int largest;
-        if (threadIdx.x == 0) largest = 0;
-        __syncthreads();
-        int most = 0;      // magnitudes order like their bits
-        for (int i = threadIdx.x; i < D / 8; i += kStateThreads) {
-            Piece<T, 8> r;
-            load_piece<T, 8>(r, row + i * 8);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) most = max(most, static_cast<int>(__float_as_uint(element(r, e)) & 0x7fffffffu));
-        }
-        most = __reduce_max_sync(kFull, most);
-        if ((threadIdx.x & 31) == 0) atomicMax(&largest, most);
-        __syncthreads();
-        // 2^e, 14 - e the largest's exponent; both ways within fp32's normal numbers
-        const int e = min(126, 14 - ((largest >> 23) - 127));
-        scale = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        if (threadIdx.x == 0) back[m] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    } else if (threadIdx.x == 0) {
-        back[m] = 1.0f;
-    }
-    const int n = (m % (NT * 8)) / 8, col = m % 8, unit_size = unit_bytes(NT, P, steps);
-    unsigned char* to = arranged + static_cast<int64_t>(m / (NT * 8)) * units * unit_size;
-    for (int i = threadIdx.x; i < (words + 31) / 32 * 32; i += kStateThreads) {      // whole warps go round
+    const int words = (D + kUnit - 1) / kUnit * (kUnit / 8);
+    for (int i = first; i < (words + 31) / 32 * 32; i += stride) {
         Piece<T, 8> r;
         if (i * 8 < D) load_piece<T, 8>(r, row + i * 8);
         else clear_piece(r);
-        const int u = i / 16, q = i % 16, step = steps < 4 ? q / 4 : q % 4, t = steps < 4 ? q % 4 : q / 4;
-        unsigned char* unit = to + static_cast<int64_t>(u) * unit_size;
+        const int u = i / 16, q = i % 16, step = STEPS < 4 ? q / 4 : q % 4, t = STEPS < 4 ? q % 4 : q / 4;
         __half h[P][8];
         float sum = 0.0f;
 #pragma unroll
@@ -142,21 +136,57 @@ arrange_states_kernel(const T* __restrict__ x, int64_t x_stride, int D, int NT, 
             }
             sum += __half2float(h[0][e]);
         }
-        for (int d = 1; d < 4 * steps; d <<= 1) sum += __shfl_xor_sync(kFull, sum, d);
+        for (int d = 1; d < 4 * STEPS; d <<= 1) sum += __shfl_xor_sync(kFull, sum, d);
         if (i >= words) continue;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const __half2 pair[4] = {__halves2half2(h[p][0], h[p][4]), __halves2half2(h[p][1], h[p][5]), __halves2half2(h[p][2], h[p][6]), __halves2half2(h[p][3], h[p][7])};
-            *reinterpret_cast<uint4*>(unit + ((step * NT + n) * P + p) * 512 + (col * 4 + t) * 16) = *reinterpret_cast<const uint4*>(pair);
+            *at(u, step, p, t) = *reinterpret_cast<const uint4*>(pair);
         }
-        if (q % (4 * steps) == 0) *reinterpret_cast<float*>(unit + P * NT * 2048 + (q / (4 * steps) * NT * 8 + n * 8 + col) * 4) = sum;
+        if (q % (4 * STEPS) == 0) *sum_at(u, q / (4 * STEPS)) = sum;
     }
+}
+
+constexpr int kStateThreads = 512;
+
+// One block per state.
+template <typename T, int STEPS>
+__global__ void __launch_bounds__(kStateThreads)
+arrange_states_kernel(const T* __restrict__ x, int64_t x_stride, int D, int NT, unsigned char* __restrict__ arranged, float* __restrict__ back)
+{
+    constexpr int P = kPieces<T>;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int m = blockIdx.x, units = (D + kUnit - 1) / kUnit;
+    const T* row = x + m * x_stride;
+    float scale = 1.0f;
+    if constexpr (!std::is_same<T, __half>::value) {
+        __shared__ int largest;
+        if (threadIdx.x == 0) largest = 0;
+        __syncthreads();
+        const int most = largest_of(row, D, threadIdx.x, kStateThreads);
+        if ((threadIdx.x & 31) == 0) atomicMax(&largest, most);
+        __syncthreads();
+        const int e = scale_exponent(largest);
+        scale = power_of_two(e);
+        if (threadIdx.x == 0) back[m] = power_of_two(-e);
+    } else if (threadIdx.x == 0) {
+        back[m] = 1.0f;
+    }
+    const int n = (m % (NT * 8)) / 8, col = m % 8, unit_size = unit_bytes(NT, P, STEPS);
+    unsigned char* to = arranged + static_cast<int64_t>(m / (NT * 8)) * units * unit_size;
+    arrange_words<T, STEPS>(
+        row, D, scale, threadIdx.x, kStateThreads,
+        [&](int u, int step, int p, int t) {
+            return reinterpret_cast<uint4*>(to + static_cast<int64_t>(u) * unit_size + ((step * NT + n) * P + p) * 512 + (col * 4 + t) * 16);
+        },
+        [&](int u, int k) { return reinterpret_cast<float*>(to + static_cast<int64_t>(u) * unit_size + P * NT * 2048 + (k * NT * 8 + n * 8 + col) * 4); });
 }
 
 struct LinearArgs {
     const unsigned char* arranged;              // states as arrange_states_kernel leaves them, and what undoes their scales
     const float* back;
-    int64_t m;
+    const void* x;                              // LOCAL: as they are
+    int64_t x_stride, m;
     const uint8_t* rows;
     int64_t num_rows, row_bytes;
     int D, group_log2;
@@ -237,8 +267,9 @@ __device__ __forceinline__ int row_of(int g) { return (g >> 1) | ((g & 1) << 2);
 // and one group: where a group is at least a unit, lane t takes elements 32 t .. 32 t + 31 with one 16-byte load; small
 // groups (32 and 64) need an instruction's elements side by side, so that lane t takes elements 32 s + 8 t .. + 7 in step
 // s, a word at a time.
-// STEPS: how many steps of a unit a group spans.  P: pieces of a state's element.
-template <int RT, int NT, int P, int STEPS>
+// STEPS: how many steps of a unit a group spans.  P: pieces of a state's element.  T: the states' type, where the workers arrange
+// them themselves before they begin and keep them in shared memory (LOCAL); void: they come with every stage.
+template <typename T, int RT, int NT, int P, int STEPS>
 __global__ void __launch_bounds__(kThreads, 1)
 group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap head_map)
 {
@@ -246,14 +277,19 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     constexpr int kPart = NT * 8 * kPitch;      // one warp's sums
     constexpr int U = units_at_once(RT), kStates = unit_bytes(NT, P, STEPS), kCodeBytes = kWarps * RT * 16 * U * (kUnit / 2);
     constexpr int kBuffers = NT == 1 ? 2 : 1;   // of the warps' sums
+    constexpr bool LOCAL = !std::is_void<T>::value;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int bands = kWarps >> a.slices_log2, slices = 1 << a.slices_log2, tile_rows = bands * RT * 16;
-    const int head_bytes = tile_rows * a.head_bytes, state_bytes = slices * U * kStates;
+    const int head_bytes = tile_rows * a.head_bytes, state_bytes = LOCAL ? 0 : slices * U * kStates;
     // boxes of codes first (1024-byte aligned), then those of heads, the states, sums, barriers
     unsigned char* heads_at = smem + a.stages * kCodeBytes;
     unsigned char* states_at = heads_at + a.stages * head_bytes;
     float* red = reinterpret_cast<float*>(states_at + a.stages * state_bytes);
     const uint32_t full = shared_address(red + kBuffers * kWarps * kPart), empty = full + 8 * kMostStages;
+    // LOCAL: what undoes the states' scales, the largest of each, the states
+    float* backs = red + kBuffers * kWarps * kPart + 4 * kMostStages;
+    int* largest = reinterpret_cast<int*>(backs + 16);
+    unsigned char* local = reinterpret_cast<unsigned char*>(largest + 16);
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int units = (a.D + kUnit - 1) / kUnit, groups = (a.D + (1 << a.group_log2) - 1) >> a.group_log2;
@@ -282,7 +318,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                 tile += gridDim.x;
             }
         };
-        auto states_of = [&](int c) { return (units - c * U * slices < U * slices ? units - c * U * slices : U * slices) * kStates; };
+        auto states_of = [&](int c) { return LOCAL ? 0 : (units - c * U * slices < U * slices ? units - c * U * slices : U * slices) * kStates; };
         auto fetch_rows = [&](int stage) {
             const uint32_t bar = full + 8 * stage;
             const int first = static_cast<int>(tile * tile_rows);
@@ -303,12 +339,14 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
             fetch_rows(filled);
             next();
         }
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        tile = blockIdx.x;
-        chunk = 0;
-        for (int i = 0; i < filled; ++i) {
-            fetch_states(i);
-            next();
+        if constexpr (!LOCAL) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            tile = blockIdx.x;
+            chunk = 0;
+            for (int i = 0; i < filled; ++i) {
+                fetch_states(i);
+                next();
+            }
         }
         int stage = 0;
         uint32_t round = 0;
@@ -318,7 +356,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                 return;
             }
             fetch_rows(stage);
-            fetch_states(stage);
+            if constexpr (!LOCAL) fetch_states(stage);
             next();
             if (++stage == a.stages) {
                 stage = 0;
@@ -329,7 +367,37 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     }
 
     // ---- the warps that work ---------------------------------------------------------------------------------------
-    asm volatile("griddepcontrol.wait;" ::: "memory");      // `back` is read at a tile's end
+    const int local_unit = local_unit_bytes(cols, NT, P, STEPS);
+    if constexpr (LOCAL) {
+        // as many warps to each state
+        int share_log2 = 4;
+        while ((kWarps >> share_log2) < cols) --share_log2;
+        const int j = warp >> share_log2, first = (warp & ((1 << share_log2) - 1)) * 32 + lane, stride = 32 << share_log2;
+        const T* row = static_cast<const T*>(a.x) + (m0 + j) * a.x_stride;
+        float scale = 1.0f;
+        if constexpr (!std::is_same<T, __half>::value) {
+            if (threadIdx.x < 16) largest[threadIdx.x] = 0;
+            workers_sync();
+            if (j < cols) {
+                const int most = largest_of(row, a.D, first, stride);
+                if (lane == 0) atomicMax(&largest[j], most);
+            }
+            workers_sync();
+            const int e = scale_exponent(largest[j]);
+            scale = power_of_two(e);
+            if (j < cols && first == 0) backs[j] = power_of_two(-e);
+        } else if (threadIdx.x < 16) {
+            backs[threadIdx.x] = 1.0f;
+        }
+        if (j < cols)
+            arrange_words<T, STEPS>(
+                row, a.D, scale, first, stride,
+                [&](int u, int step, int p, int t) { return reinterpret_cast<uint4*>(local + u * local_unit + ((step * P + p) * cols + j) * 64 + t * 16); },
+                [&](int u, int k) { return reinterpret_cast<float*>(local + u * local_unit + P * cols * 256 + (k * NT * 8 + j) * 4); });
+        workers_sync();
+    } else {
+        asm volatile("griddepcontrol.wait;" ::: "memory");      // `back` is read at a tile's end
+    }
     const int g = row_of(lane >> 2), t = lane & 3, slice = warp & (slices - 1), band = warp >> a.slices_log2;
     float y[RT][NT][4];
 #pragma unroll
@@ -344,7 +412,10 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     const int half = U == 1 ? slice & 1 : 0;
     const int row8 = 8 * a.head_bytes;
     const unsigned char* head_rows = heads_at + (band * RT * 16 + g) * a.head_bytes;
-    const unsigned char* my_states = states_at + slice * U * kStates;
+    // a column that no state stands in takes another's: what comes of it is not stored
+    int column[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) column[n] = (n * 8 + (lane >> 2) < cols ? n * 8 + (lane >> 2) : cols - 1) * 64 + t * 16;
     int buffer = 0;
     int stage = 0;
     uint32_t round = 0;
@@ -358,7 +429,8 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
             for (int k = 0; k < U; ++k) {
                 const int u = U * (c * slices + slice) + k;
                 if (u >= units) break;
-                const unsigned char* states = my_states + stage * state_bytes + k * kStates;
+                const unsigned char* states = LOCAL ? local + u * local_unit : states_at + stage * state_bytes + (slice * U + k) * kStates;
+                const unsigned char* sums_of_states = states + (LOCAL ? P * cols * 256 : P * NT * 2048);
                 uint4 w[RT][2];
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
@@ -385,7 +457,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int q = 0; q < P; ++q) {
-                            const uint4 b = *reinterpret_cast<const uint4*>(states + ((s * NT + n) * P + q) * 512 + lane * 16);
+                            const uint4 b = *reinterpret_cast<const uint4*>(states + (LOCAL ? (s * P + q) * (cols * 64) + column[n] : ((s * NT + n) * P + q) * 512 + lane * 16));
 #pragma unroll
                             for (int i = 0; i < RT; ++i) {
                                 if (first && q == 0) mma<true>(acc[i][n], p[i][0][0], p[i][1][0], p[i][0][1], p[i][1][1], b.x, b.y);
@@ -399,7 +471,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                         gi = gi < groups ? gi : groups - 1;
                         float2 sum[NT];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) sum[n] = *reinterpret_cast<const float2*>(states + P * NT * 2048 + (s / STEPS * NT * 8 + n * 8 + 2 * t) * 4);
+                        for (int n = 0; n < NT; ++n) sum[n] = *reinterpret_cast<const float2*>(sums_of_states + (s / STEPS * NT * 8 + n * 8 + 2 * t) * 4);
 #pragma unroll
                         for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -443,7 +515,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
             const float* from = sums + (row / (RT * 16) << a.slices_log2) * kPart + col * kPitch + row % (RT * 16);
             float v = 0.0f;
             for (int k = 0; k < slices; ++k) v += from[k * kPart];
-            v *= __ldcg(a.back + m0 + col);
+            v *= LOCAL ? backs[col] : __ldcg(a.back + m0 + col);
             if (a.bias) v += load_any(a.bias, a.bias_dtype, r);
             store_any(a.out, a.out_dtype, (m0 + col) * a.out_stride + r, v);
         }
@@ -483,21 +555,34 @@ bool encode_rows(CUtensorMap* map, const LinearArgs& a, int box_words, int box_r
 int states_per_block(int64_t m) { return m <= 8 ? 1 : 2; }      // in eights
 int pieces_of(int dtype) { return dtype == TBE_B200_FP32 ? 2 : 1; }
 int steps_of(int group_log2) { return group_log2 == 5 ? 1 : group_log2 == 6 ? 2 : 4; }
+int64_t units_of(int64_t D) { return (D + kUnit - 1) / kUnit; }
+
+// Whether a block keeps all states in shared memory: it then arranges them itself, which saves a launch and the scratch.  What
+// is left holds two stages of any shape.
+constexpr int64_t kMostLocal = 96 * 1024;
+int64_t local_bytes(int64_t m, int64_t D, int dtype, int group_log2)
+{
+    return units_of(D) * local_unit_bytes(static_cast<int>(m), states_per_block(m), pieces_of(dtype), steps_of(group_log2));
+}
+bool is_local(int64_t m, int64_t D, int dtype, int group_log2) { return m <= 16 && local_bytes(m, D, dtype, group_log2) <= kMostLocal; }
+
 int64_t arranged_bytes(int64_t m, int64_t D, int dtype, int group_log2)
 {
     const int NT = states_per_block(m);
-    return (m + NT * 8 - 1) / (NT * 8) * ((D + kUnit - 1) / kUnit) * unit_bytes(NT, pieces_of(dtype), steps_of(group_log2));
+    return (m + NT * 8 - 1) / (NT * 8) * units_of(D) * unit_bytes(NT, pieces_of(dtype), steps_of(group_log2));
 }
 
-template <int RT, int NT, int P, int STEPS>
+template <typename T, int RT, int NT, int P, int STEPS>
 int launch_linear(LinearArgs a, cudaStream_t s)
 {
     constexpr int U = units_at_once(RT);
+    constexpr bool LOCAL = !std::is_void<T>::value;
     const int sms = sm_count();
-    const int64_t fixed = static_cast<int64_t>(NT == 1 ? 2 : 1) * kWarps * NT * 8 * (RT * 16 + 4) * 4 + 16 * kMostStages;
+    const int64_t fixed = static_cast<int64_t>(NT == 1 ? 2 : 1) * kWarps * NT * 8 * (RT * 16 + 4) * 4 + 16 * kMostStages +
+                          (LOCAL ? 128 + units_of(a.D) * local_unit_bytes(static_cast<int>(a.m), NT, P, STEPS) : 0);
     auto stage_bytes = [&](int l) {
         return static_cast<int64_t>(kWarps) * RT * 16 * U * (kUnit / 2) + static_cast<int64_t>(RT * 16 * (kWarps >> l)) * head_window(a.D, U << l, a.group_log2) +
-               (U << l) * unit_bytes(NT, P, STEPS);
+               (LOCAL ? 0 : (U << l) * unit_bytes(NT, P, STEPS));
     };
     // Shares of the elements: as few as keep every multiprocessor at work to the end, counted in units of time that
     // a warp needs for its share of a stage; a tile's end is worth about half of one.  A box is at most 256 rows.
@@ -520,7 +605,7 @@ int launch_linear(LinearArgs a, cudaStream_t s)
     CUtensorMap codes, heads;
     if (!encode_rows(&codes, a, 32, tile_rows, true) || !encode_rows(&heads, a, a.head_bytes / 4, tile_rows, false))
         return fail(TBE_B200_ERR_CUDA, "group_row_linear: the rows could not be described to the copy engine");
-    auto* kernel = group_row_linear_kernel<RT, NT, P, STEPS>;
+    auto* kernel = group_row_linear_kernel<T, RT, NT, P, STEPS>;
     static std::atomic<uint64_t> allowed{0};
     if (const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kMostShared, allowed)) return rc;
     cudaLaunchAttribute early{};
@@ -532,20 +617,38 @@ int launch_linear(LinearArgs a, cudaStream_t s)
     config.dynamicSmemBytes = shared;
     config.stream = s;
     config.attrs = &early;
-    config.numAttrs = 1;
+    config.numAttrs = LOCAL ? 0 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a, codes, heads);
     if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "group_row_linear_kernel: %s", cudaGetErrorString(e));
     return check_launch("group_row_linear_kernel");
 }
 
-template <int RT, int NT, int P>
+// T: the states' type where blocks arrange them themselves, else void.
+template <typename T, int P>
 int launch_linear(const LinearArgs& a, cudaStream_t s)
 {
-    switch (a.group_log2) {
-        case 5: return launch_linear<RT, NT, P, 1>(a, s);
-        case 6: return launch_linear<RT, NT, P, 2>(a, s);
-        default: return launch_linear<RT, NT, P, 4>(a, s);
-    }
+    // Rows 32 to a warp use every state twice; 16 where that leaves multiprocessors without any.
+    const bool many = a.num_rows >= static_cast<int64_t>(64) * sm_count(), two = states_per_block(a.m) == 2;
+    auto by_group = [&](auto rt, auto nt) {
+        constexpr int RT = decltype(rt)::value, NT = decltype(nt)::value;
+        switch (a.group_log2) {
+            case 5: return launch_linear<T, RT, NT, P, 1>(a, s);
+            case 6: return launch_linear<T, RT, NT, P, 2>(a, s);
+            default: return launch_linear<T, RT, NT, P, 4>(a, s);
+        }
+    };
+    const std::integral_constant<int, 1> one{};
+    const std::integral_constant<int, 2> both{};
+    if (many) return two ? by_group(both, both) : by_group(both, one);
+    return two ? by_group(one, both) : by_group(one, one);
+}
+
+template <typename T>
+int launch_arrange(const T* x, int64_t x_stride, int64_t m, int D, int group_log2, unsigned char* arranged, float* back, cudaStream_t s)
+{
+    auto* kernel = group_log2 == 5 ? arrange_states_kernel<T, 1> : group_log2 == 6 ? arrange_states_kernel<T, 2> : arrange_states_kernel<T, 4>;
+    kernel<<<static_cast<unsigned>(m), kStateThreads, 0, s>>>(x, x_stride, D, states_per_block(m), arranged, back);
+    return check_launch("arrange_states_kernel");
 }
 
 }  // namespace
@@ -557,7 +660,7 @@ extern "C" int64_t tbe_b200_group_row_linear_scratch_bytes(int64_t m, int64_t D,
 {
     const int group_log2 = group_log2_of(group_size);
     if (m < 0 || m > (1 << 19) || D < 1 || D > (1 << 20) || group_log2 < 0 || !element_bytes(input_dtype)) return -1;
-    return arranged_bytes(m, D, input_dtype, group_log2) + (4 * m + 15) / 16 * 16;
+    return is_local(m, D, input_dtype, group_log2) ? 0 : arranged_bytes(m, D, input_dtype, group_log2) + (4 * m + 15) / 16 * 16;
 }
 
 extern "C" int tbe_b200_group_row_linear(const void* input, int32_t input_dtype, int64_t input_stride, int64_t m, const uint8_t* rows,
@@ -576,26 +679,25 @@ extern "C" int tbe_b200_group_row_linear(const void* input, int32_t input_dtype,
     if (!input || !rows || !output) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "group_row_linear: NULL pointer");
     if (!rows_aligned(input, input_stride, ib, 8)) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "group_row_linear: input rows must be 16-byte aligned");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const int group_log2 = group_log2_of(group_size), NT = states_per_block(m), steps = steps_of(group_log2);
-    const int64_t need = tbe_b200_group_row_linear_scratch_bytes(m, D, group_size, input_dtype), arranged = arranged_bytes(m, D, input_dtype, group_log2);
+    const int group_log2 = group_log2_of(group_size);
+    LinearArgs a{nullptr, nullptr, input, input_stride, m, rows, num_rows, row_bytes, static_cast<int>(D), group_log2, bias, bias_dtype, output_dtype, output,
+                 output_stride, error_flag, 0, 0, 0, 0};
+    if (is_local(m, D, input_dtype, group_log2))
+        return with_element(input_dtype, [&](auto* ti) {
+            using T = std::remove_pointer_t<decltype(ti)>;
+            return launch_linear<T, kPieces<T>>(a, s);
+        });
+    const int64_t need = tbe_b200_group_row_linear_scratch_bytes(m, D, group_size, input_dtype);
     if (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15))
         return fail(TBE_B200_ERR_INVALID_ARGUMENT, "group_row_linear: scratch must be %lld bytes, 16-byte aligned", (long long)need);
     unsigned char* states = static_cast<unsigned char*>(scratch);
-    float* back = reinterpret_cast<float*>(states + arranged);
+    float* back = reinterpret_cast<float*>(states + arranged_bytes(m, D, input_dtype, group_log2));
+    a.arranged = states;
+    a.back = back;
     const int rc = with_element(input_dtype, [&](auto* ti) {
         using T = std::remove_pointer_t<decltype(ti)>;
-        arrange_states_kernel<T><<<static_cast<unsigned>(m), kStateThreads, 0, s>>>(static_cast<const T*>(input), input_stride, static_cast<int>(D), NT, steps, states, back);
-        return check_launch("arrange_states_kernel");
+        return launch_arrange<T>(static_cast<const T*>(input), input_stride, m, static_cast<int>(D), group_log2, states, back, s);
     });
     if (rc) return rc;
-    const LinearArgs a{states, back, m, rows, num_rows, row_bytes, static_cast<int>(D), group_log2, bias, bias_dtype, output_dtype, output, output_stride,
-                       error_flag, 0, 0, 0, 0};
-    // Rows 32 to a warp use every state twice; 16 where that leaves multiprocessors without any.
-    const bool many = num_rows >= static_cast<int64_t>(64) * sm_count();
-    if (pieces_of(input_dtype) == 1) {
-        if (NT == 1) return many ? launch_linear<2, 1, 1>(a, s) : launch_linear<1, 1, 1>(a, s);
-        return many ? launch_linear<2, 2, 1>(a, s) : launch_linear<1, 2, 1>(a, s);
-    }
-    if (NT == 1) return many ? launch_linear<2, 1, 2>(a, s) : launch_linear<1, 1, 2>(a, s);
-    return many ? launch_linear<2, 2, 2>(a, s) : launch_linear<1, 2, 2>(a, s);
+    return pieces_of(input_dtype) == 1 ? launch_linear<void, 1>(a, s) : launch_linear<void, 2>(a, s);
 }

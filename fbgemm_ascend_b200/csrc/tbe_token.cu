@@ -253,14 +253,14 @@ __device__ __forceinline__ void clear_rows(const FillArgs& f, int unit, int64_t 
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-// A block's share of the rows behind the first `early` (a multiple of 32) that no token names: a thread takes 32 rows.
-__device__ __forceinline__ void clear_unmet_rows(const FillArgs& f, int unit, int64_t block, int64_t blocks, unsigned char* zeros)
+// Of the rows 32 w0 .. 32 w1 those that no token names (a bit of `met` each, which begins with row 32 w0): a thread takes 32 rows
+// at a time.
+__device__ __forceinline__ void clear_unmet_rows(const FillArgs& f, int unit, int64_t w0, int64_t w1, const uint32_t* met, int64_t thread, int64_t threads,
+                                                 const void* zeros)
 {
-    make_zeros<kFewZeroBytes>(zeros);
-    const int64_t words = (f.rows + 31) / 32;
-    for (int64_t w = f.early / 32 + block + threadIdx.x * blocks; w < words; w += blocks * blockDim.x) {
+    for (int64_t w = w0 + thread; w < w1; w += threads) {
         const int64_t left = f.rows - w * 32;
-        uint32_t clear = ~__ldg(f.met + w) & (left < 32 ? (1u << left) - 1u : kFull);
+        uint32_t clear = ~met[w - w0] & (left < 32 ? (1u << left) - 1u : kFull);
         while (clear) {
             const int first = __ffs(clear) - 1;
             const uint32_t behind = ~(clear >> first);
@@ -291,24 +291,19 @@ __device__ __forceinline__ uint32_t shared_of(const void* p, uint32_t rank)
     return a;
 }
 
-constexpr int64_t sort_shared_bytes(int items) { return int64_t(items) * kSortThreads * 8 + kSortWarps * kMaxBins * 2 + kSortBlocks * kMaxBins * 4 + kMaxBins * 4 + 128; }
+__host__ __device__ constexpr int64_t sort_shared_bytes(int items) { return int64_t(items) * kSortThreads * 8 + kSortWarps * kMaxBins * 2 + kSortBlocks * kMaxBins * 4 + kMaxBins * 4 + 128; }
 
+// Sorts; block `mine` of `cluster` (1: alone) is left with places mine * items * 1024 on, (token << 32 | position) each, in the
+// memory that is returned, the first of `shared`.  Ends with a barrier of all.
 template <int ITEMS>
-__global__ void __launch_bounds__(kSortThreads, 1)
-sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int width, uint2* __restrict__ sorted, const FillArgs fill, int unit)
+__device__ __forceinline__ unsigned long long* sort_in_shared(const SortInput& in, int cluster, uint32_t mine, int items, int passes, int width, unsigned char* shared)
 {
-    extern __shared__ __align__(16) unsigned char sort_smem[];
-    if (blockIdx.x >= cluster) {
-        clear_rows(fill, unit, blockIdx.x - cluster, gridDim.x - cluster, sort_smem);
-        return;
-    }
-    unsigned long long* buf = reinterpret_cast<unsigned long long*>(sort_smem);
+    unsigned long long* buf = reinterpret_cast<unsigned long long*>(shared);
     unsigned short(*count)[kMaxBins] = reinterpret_cast<unsigned short(*)[kMaxBins]>(buf + ITEMS * kSortThreads);
     uint32_t(*table)[kMaxBins] = reinterpret_cast<uint32_t(*)[kMaxBins]>(count + kSortWarps);
     uint32_t* base = reinterpret_cast<uint32_t*>(table + kSortBlocks);
     uint32_t* warp_tot = base + kMaxBins;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << width;
-    const uint32_t mine = cluster > 1 ? cluster_rank() : 0u;
     const int per = items * kSortThreads;
     const int64_t first = static_cast<int64_t>(mine) * per;
     const int at = warp * (32 * items) + lane;
@@ -316,8 +311,6 @@ sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int w
         if (cluster > 1) cluster_sync();
         else __syncthreads();
     };
-    if (fill.met)
-        for (int64_t w = mine * kSortThreads + threadIdx.x; w < (fill.rows + 31) / 32; w += cluster * kSortThreads) fill.met[w] = 0u;
     if (cluster > 1) cluster_sync();      // every block has begun: its shared memory may be written
     for (int p = 0; p < passes; ++p) {
         uint32_t key[ITEMS], pos[ITEMS], rank[ITEMS];
@@ -344,11 +337,16 @@ sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int w
         __syncthreads();
         if (threadIdx.x < bins) {
             uint32_t run = 0;
-#pragma unroll 8
-            for (int w = 0; w < kSortWarps; ++w) {
-                const uint32_t c = count[w][threadIdx.x];
-                count[w][threadIdx.x] = static_cast<unsigned short>(run);
-                run += c;
+#pragma unroll
+            for (int w0 = 0; w0 < kSortWarps; w0 += 16) {      // reads first: a write between them would hold up the next
+                uint32_t c[16];
+#pragma unroll
+                for (int w = 0; w < 16; ++w) c[w] = count[w0 + w][threadIdx.x];
+#pragma unroll
+                for (int w = 0; w < 16; ++w) {
+                    count[w0 + w][threadIdx.x] = static_cast<unsigned short>(run);
+                    run += c[w];
+                }
             }
             if (cluster > 1) {
                 for (int r = 0; r < cluster; ++r)
@@ -380,6 +378,24 @@ sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int w
         }
         sync_all();
     }
+    return buf;
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kSortThreads, 1)
+sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int width, uint2* __restrict__ sorted, const FillArgs fill, int unit)
+{
+    extern __shared__ __align__(16) unsigned char sort_smem[];
+    if (blockIdx.x >= cluster) {
+        clear_rows(fill, unit, blockIdx.x - cluster, gridDim.x - cluster, sort_smem);
+        return;
+    }
+    const uint32_t mine = cluster > 1 ? cluster_rank() : 0u;
+    const int per = items * kSortThreads;
+    const int64_t first = static_cast<int64_t>(mine) * per;
+    if (fill.met)
+        for (int64_t w = mine * kSortThreads + threadIdx.x; w < (fill.rows + 31) / 32; w += cluster * kSortThreads) fill.met[w] = 0u;
+    const unsigned long long* buf = sort_in_shared<ITEMS>(in, cluster, mine, items, passes, width, sort_smem);
     for (int i = threadIdx.x; i < per && first + i < in.n; i += kSortThreads) {
         const unsigned long long both = buf[i];
         const uint32_t key = static_cast<uint32_t>(both >> 32);
@@ -574,7 +590,12 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
 {
     if (blockIdx.x < fillers) {
         __shared__ __align__(16) unsigned char zeros[INTO ? 16 : kFewZeroBytes];
-        if constexpr (!INTO) clear_unmet_rows(fill, sizeof(TO), blockIdx.x, fillers, zeros);
+        if constexpr (!INTO) {
+            make_zeros<kFewZeroBytes>(zeros);
+            const int64_t w0 = fill.early / 32;
+            clear_unmet_rows(fill, sizeof(TO), w0, (fill.rows + 31) / 32, fill.met + w0, blockIdx.x + static_cast<int64_t>(threadIdx.x) * fillers,
+                             static_cast<int64_t>(kThreads) * fillers, zeros);
+        }
         return;
     }
     const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
@@ -745,6 +766,123 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(const SumArgs a, T
     put_sum<TO, INTO>(a, out + static_cast<int64_t>(ends) * a.out_stride, add_pieces(a, tile, 0, pieces, c), c);
 }
 
+// ---- gradient of a few tokens: one launch -------------------------------------------------------------------------
+//
+// Where launches are most of the time, every block that sums sorts all tokens for itself; it takes eight lanes' columns of all
+// rows, a tile of the sorted positions to each group of eight lanes, and joins the pieces of the tiles in shared memory.  The
+// blocks behind those clear the rows that no token names, which each finds for its own rows.
+constexpr int kFewTokens = 2048, kFewItems = kFewTokens / kSortThreads;
+constexpr int kFewLanes = 8, kFewGroups = kSortThreads / kFewLanes;
+constexpr int kMostClearWords = 8 * 1024;      // of rows that one block clears
+
+template <typename T> __host__ __device__ constexpr int few_columns() { return kFewLanes * kVec<T>; }      // 128 bytes of a row
+template <typename T> __host__ __device__ constexpr int64_t few_shared_bytes() { return sort_shared_bytes(kFewItems) + int64_t(kFewGroups) * 2 * few_columns<T>() * 4; }
+
+template <typename TI, typename TO, bool ALIGNED, bool INTO>
+__global__ void __launch_bounds__(kSortThreads, 1)
+grad_of_few_kernel(const SortInput in, int passes, int width, const TI* __restrict__ grad, int64_t grad_stride, int D, float scale, TO* out, int64_t out_stride,
+                   int sum_blocks, const FillArgs fill, int64_t words_per_block)
+{
+    constexpr int VEC = kVec<TI>, kOne = ALIGNED ? VEC : 1, kRow = few_columns<TI>();
+    extern __shared__ __align__(16) unsigned char sort_smem[];
+    if (blockIdx.x >= sum_blocks) {
+        uint32_t* met = reinterpret_cast<uint32_t*>(sort_smem + kFewZeroBytes);
+        const int64_t w0 = (blockIdx.x - sum_blocks) * words_per_block, last = (fill.rows + 31) / 32, w1 = w0 + words_per_block < last ? w0 + words_per_block : last;
+        for (int64_t w = threadIdx.x; w < w1 - w0; w += kSortThreads) met[w] = 0u;
+        make_zeros<kFewZeroBytes>(sort_smem);
+        for (int i = threadIdx.x; i < in.n; i += kSortThreads) {
+            const int64_t key = token_key(in, i), w = key / 32;
+            if (key < in.num_embeddings && w >= w0 && w < w1) atomicOr(met + (w - w0), 1u << (key & 31));
+        }
+        __syncthreads();
+        clear_unmet_rows(fill, sizeof(TO), w0, w1, met, threadIdx.x, kSortThreads, sort_smem);
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        return;
+    }
+    const int n = static_cast<int>(in.n), items = (n + kSortThreads - 1) / kSortThreads;
+    const unsigned long long* sorted = sort_in_shared<kFewItems>(in, 1, 0u, items, passes, width, sort_smem);
+    float* parts = reinterpret_cast<float*>(sort_smem + sort_shared_bytes(kFewItems));
+    const uint32_t none = static_cast<uint32_t>(in.num_embeddings);
+    auto key_of = [&](int i) { return static_cast<uint32_t>(sorted[i] >> 32); };
+    const int group = threadIdx.x / kFewLanes, lane = threadIdx.x % kFewLanes;
+    const int tile_rows = (n + kFewGroups - 1) / kFewGroups, first = group * tile_rows, rows = min(tile_rows, n - first);
+    const int c = blockIdx.x * kRow + lane * VEC;
+    float acc[VEC] = {};
+    auto put_part = [&](int slot) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) parts[(group * 2 + slot) * kRow + lane * VEC + e] = acc[e];
+    };
+    auto put_row = [&](uint32_t token) {
+        TO* row = out + static_cast<int64_t>(token) * out_stride;
+#pragma unroll
+        for (int i = 0; i < VEC / kOne; ++i) {
+            if (c + i * kOne >= D) break;
+            Piece<TO, kOne> old;
+            if constexpr (INTO) load_piece<TO, kOne, false>(old, row + c + i * kOne);
+            float v[kOne];
+#pragma unroll
+            for (int e = 0; e < kOne; ++e) {
+                if constexpr (INTO) v[e] = fmaf(scale, acc[i * kOne + e], element(old, e));
+                else v[e] = scale * acc[i * kOne + e];
+            }
+            store_piece<TO, kOne>(row + c + i * kOne, v);
+        }
+    };
+    uint32_t cur = none;
+    bool onward = false;      // a token starts in this tile and goes on behind it
+    if (rows > 0) {
+        cur = key_of(first);
+        bool head = first > 0 && key_of(first - 1) == cur;
+        for (int r = 0; r < rows && cur != none; r += kAhead) {
+            Piece<TI, VEC> in_row[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                clear_piece(in_row[k]);
+                const unsigned long long both = r + k < rows ? sorted[first + r + k] : static_cast<unsigned long long>(none) << 32;
+                if (static_cast<uint32_t>(both >> 32) == none) continue;
+                const TI* row = grad + static_cast<int64_t>(static_cast<uint32_t>(both)) * grad_stride;
+                if constexpr (ALIGNED) {
+                    if (c < D) load_piece<TI, VEC>(in_row[k], row + c);
+                } else if (c < D) {
+                    SplitRow split;
+                    split.of(row, D);
+                    SplitPiece<TI, VEC> p;
+                    p.load(split, c);
+                    in_row[k] = p.piece();
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (r + k >= rows || cur == none) break;
+                const uint32_t key = key_of(first + r + k);
+                if (key != cur) {
+                    if (head) put_part(0);
+                    else put_row(cur);
+                    head = false;
+                    cur = key;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+                    if (cur == none) break;
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += element(in_row[k], e);
+            }
+        }
+        if (cur != none) {
+            const bool goes_on = first + rows < n && key_of(first + rows) == cur;
+            onward = goes_on && !head;
+            if (head || goes_on) put_part(head ? 0 : 1);
+            else put_row(cur);
+        }
+    }
+    __syncthreads();
+    if (!onward) return;
+    for (int g = group + 1; g * tile_rows < n && key_of(g * tile_rows) == cur; ++g)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += parts[g * 2 * kRow + lane * VEC + e];
+    put_row(cur);
+}
+
 int64_t align16(int64_t b) { return (b + 15) / 16 * 16; }
 
 // Where things lie in the scratch, and how the sums are cut: about as many groups of lanes as the GPU holds, each with a tile
@@ -753,6 +891,7 @@ struct GradPlan {
     int64_t sorted[2], hist, met, parts, total;
     int64_t tiles, sort_tiles;
     int tile_rows, slices, lanes_log2, padded_D;
+    bool few;      // one launch, no scratch
 };
 
 constexpr int64_t kResidentWarps = 148 * 32;
@@ -760,6 +899,9 @@ constexpr int64_t kResidentWarps = 148 * 32;
 bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
 {
     if (n < 0 || n > 0x7fffffff || num_embeddings < 1 || num_embeddings > 0x7fffffff || D < 1 || D > (1 << 20)) return false;
+    l.few = n <= kFewTokens && (num_embeddings + 31) / 32 <= int64_t(kMostClearWords) * 64;
+    l.total = 0;
+    if (l.few) return true;
     l.lanes_log2 = 2;
     while (l.lanes_log2 < 5 && (kColumns << l.lanes_log2) < D) ++l.lanes_log2;
     l.slices = static_cast<int>((D + (kColumns << l.lanes_log2) - 1) / (kColumns << l.lanes_log2));
@@ -778,6 +920,36 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
     l.parts = at; at += l.tiles * 2 * l.padded_D * 4;
     l.total = at;
     return true;
+}
+
+// Digits of equal width, at most nine bits, that cover the keys 0 .. num_embeddings.
+void digits_of(int64_t num_embeddings, int& passes, int& width)
+{
+    int bits = 1;
+    while ((num_embeddings >> bits) != 0) ++bits;
+    passes = (bits + 8) / 9;
+    width = (bits + passes - 1) / passes;
+}
+
+template <typename TI, typename TO, bool INTO>
+int launch_few(const SortInput& in, const TI* grad, int64_t grad_stride, int D, float scale, TO* out, int64_t out_stride, const FillArgs& fill, cudaStream_t s)
+{
+    constexpr int kWhole = kVec<TI>, shared = static_cast<int>(few_shared_bytes<TI>());
+    const bool aligned = D % kWhole == 0 && rows_aligned(grad, grad_stride, sizeof(TI), kWhole) && rows_aligned(out, out_stride, sizeof(TO), kWhole);
+    auto* kernel = aligned ? grad_of_few_kernel<TI, TO, true, INTO> : grad_of_few_kernel<TI, TO, false, INTO>;
+    static std::atomic<uint64_t> allowed[2] = {};
+    if (const int rc = allow_shared(reinterpret_cast<const void*>(kernel), shared, allowed[aligned])) return rc;
+    int passes, width;
+    digits_of(in.num_embeddings, passes, width);
+    const int64_t words = (fill.rows + 31) / 32, sums = (D + few_columns<TI>() - 1) / few_columns<TI>();
+    // blocks that clear: 64 KB each at least, one per multiprocessor at most
+    int64_t fillers = (fill.rows * fill.row_bytes + 65535) / 65536;
+    fillers = fillers < sm_count() ? fillers : sm_count();
+    fillers = fillers < words ? fillers : words;
+    const int64_t each = fillers ? (words + fillers - 1) / fillers : 0;
+    kernel<<<static_cast<unsigned>((in.n ? sums : 0) + fillers), kSortThreads, shared, s>>>(in, passes, width, grad, grad_stride, D, scale, out, out_stride,
+                                                                                           static_cast<int>(in.n ? sums : 0), fill, each);
+    return check_launch("grad_of_few_kernel");
 }
 
 template <int ITEMS>
@@ -811,17 +983,13 @@ int sort_and_clear(const SortInput& in, const GradPlan& l, char* scratch, const 
     // blocks that clear: 64 KB each at least, one per multiprocessor at most
     int64_t fillers = (fill.early * fill.row_bytes + 65535) / 65536;
     const int sms = sm_count();
-    if (in.n == 0 || in.n > kClusterKeys) {
-        if (fillers) {
-            clear_rows_kernel<<<static_cast<unsigned>(fillers < 4 * sms ? fillers : 4 * sms), kThreads, 0, s>>>(fill, unit);
-            if (const int rc = check_launch("clear_rows_kernel")) return rc;
-        }
-        if (in.n == 0) return TBE_B200_OK;
+    if (in.n > kClusterKeys && fillers) {
+        clear_rows_kernel<<<static_cast<unsigned>(fillers < 4 * sms ? fillers : 4 * sms), kThreads, 0, s>>>(fill, unit);
+        if (const int rc = check_launch("clear_rows_kernel")) return rc;
     }
-    // digits of equal width, at most nine bits, that cover the keys 0 .. num_embeddings
-    int bits = 1;
-    while ((in.num_embeddings >> bits) != 0) ++bits;
-    const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes, bins = 1 << width;
+    int passes, width;
+    digits_of(in.num_embeddings, passes, width);
+    const int bins = 1 << width;
     if (in.n <= kClusterKeys) {
         const int cluster = in.n <= kOneBlockKeys ? 1 : kSortBlocks;
         const int items = static_cast<int>((in.n + cluster * kSortThreads - 1) / (cluster * kSortThreads));
@@ -916,15 +1084,15 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
         return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: n and num_embeddings must be below 2^31, D at most 2^20, the last two positive");
     if (padding_idx < -1 || padding_idx >= num_embeddings) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: padding_idx %lld is no row", (long long)padding_idx);
     if (grad_stride < 0 || grad_weight_stride < D) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: bad row stride");
-    if (!grad_weight || (n > 0 && (!grad || !tokens || !scratch))) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: NULL pointer");
-    if (n > 0 && (scratch_bytes < l.total || (reinterpret_cast<uintptr_t>(scratch) & 15)))
+    if (!grad_weight || (n > 0 && (!grad || !tokens || (l.total > 0 && !scratch)))) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: NULL pointer");
+    if (l.total > 0 && (scratch_bytes < l.total || (reinterpret_cast<uintptr_t>(scratch) & 15)))
         return fail(TBE_B200_ERR_INVALID_ARGUMENT, "token_embedding_grad: scratch must be %lld bytes, 16-byte aligned", (long long)l.total);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     char* base = static_cast<char*>(scratch);
     const SortInput in{tokens, token_bits == 64, n, num_embeddings, padding_idx};
     FillArgs fill{static_cast<char*>(grad_weight), accumulate ? 0 : num_embeddings, D * ob, grad_weight_stride * ob, 0, nullptr};
     fill.early = fill.rows;
-    if (n > 0 && n <= kClusterKeys) {
+    if (!l.few && n <= kClusterKeys) {
         // Writing alone runs at 4 TB/s, beside reads at most of what a copy writes: the sums' reads cost little then.  As many rows
         // are cleared beside the sort as that takes; where little is left, all.
         const int64_t beside_sort = ((int64_t(36) << 20) + n * 1400) / fill.row_bytes / 32 * 32;
@@ -933,9 +1101,21 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
             fill.met = reinterpret_cast<uint32_t*>(base + l.met);
         }
     }
+    if (l.few) {
+        if (accumulate && n == 0) return TBE_B200_OK;
+        return with_element(grad_weight_dtype, [&](auto* to) {
+            return with_element(grad_dtype, [&](auto* ti) {
+                using TO = std::remove_pointer_t<decltype(to)>;
+                using TI = std::remove_pointer_t<decltype(ti)>;
+                const TI* g = static_cast<const TI*>(grad);
+                TO* o = static_cast<TO*>(grad_weight);
+                if (accumulate) return launch_few<TI, TO, true>(in, g, grad_stride, static_cast<int>(D), scale, o, grad_weight_stride, fill, s);
+                return launch_few<TI, TO, false>(in, g, grad_stride, static_cast<int>(D), scale, o, grad_weight_stride, fill, s);
+            });
+        });
+    }
     int half;
     if (const int rc = sort_and_clear(in, l, base, fill, ob, half, s)) return rc;
-    if (n == 0) return TBE_B200_OK;
     const SumArgs a{reinterpret_cast<const uint2*>(base + l.sorted[half]), n, static_cast<uint32_t>(num_embeddings), grad_stride, grad_weight_stride,
                     static_cast<int>(D), l.padded_D, l.tile_rows, l.slices, l.lanes_log2, l.tiles, scale, reinterpret_cast<float*>(base + l.parts)};
     return with_element(grad_weight_dtype, [&](auto* to) {

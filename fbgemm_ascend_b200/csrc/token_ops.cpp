@@ -124,7 +124,8 @@ void run_grad(const Tensor& grad, const Tensor& tokens, double scale, int64_t pa
     if (V == 0 || D == 0) return;
     const int64_t need = tbe_b200_token_embedding_grad_scratch_bytes(n, V, D);
     TORCH_CHECK(need >= 0, op, ": tokens and rows must be fewer than 2^31, D at most 2^20");
-    Tensor scratch = at::empty({need}, g.options().dtype(at::kByte));    // caching-allocator blocks are 512-byte aligned
+    Tensor scratch;
+    if (need > 0) scratch = at::empty({need}, g.options().dtype(at::kByte));    // caching-allocator blocks are 512-byte aligned
     check_status(tbe_b200_token_embedding_grad(n ? g.data_ptr() : nullptr, gt, n > 1 ? g.stride(0) : D, n ? t.data_ptr() : nullptr, bits_of(t), n, V, D,
                                                static_cast<float>(scale), padding, accumulate, into.data_ptr(), wt, row_stride(into),
                                                need ? scratch.data_ptr() : nullptr, need, current_stream()), op);
@@ -360,10 +361,11 @@ Tensor group_row_linear(const Tensor& input, const Tensor& rows, int64_t group_s
     if (m == 0 || N == 0) return out;
     const int64_t need = tbe_b200_group_row_linear_scratch_bytes(m, D, static_cast<int32_t>(group_size), it);
     TORCH_CHECK(need >= 0, op, ": at most 2^19 vectors of at most 2^20 elements");
-    Tensor scratch = at::empty({need}, x.options().dtype(at::kByte));
+    Tensor scratch;
+    if (need > 0) scratch = at::empty({need}, x.options().dtype(at::kByte));
     check_status(tbe_b200_group_row_linear(x.data_ptr(), it, row_stride(x), m, r.data_ptr<uint8_t>(), N, r.size(1), D, static_cast<int32_t>(group_size),
                                            b.defined() ? b.data_ptr() : nullptr, b.defined() ? element_type(b, op, "bias") : 0, out.data_ptr(),
-                                           static_cast<int32_t>(out_type), N, nullptr, scratch.data_ptr(), need, current_stream()), op);
+                                           static_cast<int32_t>(out_type), N, nullptr, need > 0 ? scratch.data_ptr() : nullptr, need, current_stream()), op);
     return out;
 }
 

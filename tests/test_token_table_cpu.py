@@ -25,9 +25,9 @@ def _refusals():
     assert emb(n=0) == 0 and emb(D=0) == 0
 
     need = lib.tbe_b200_token_embedding_grad_scratch_bytes
-    assert need(0, 4, 8) >= 0 and need(100, 4, 8) > 0
+    assert need(0, 4, 8) == 0 and need(100, 4, 8) == 0 and need(5000, 4, 8) > 0      # few tokens need none
     assert need(1 << 31, 4, 8) == -1 and need(4, 1 << 31, 8) == -1 and need(4, 0, 8) == -1 and need(4, 4, 0) == -1 and need(-1, 4, 8) == -1
-    grad = lambda **k: lib.tbe_b200_token_embedding_grad(k.get("g", one), k.get("gt", FP32), k.get("gs", 8), one, k.get("bits", 64), k.get("n", 2),
+    grad = lambda **k: lib.tbe_b200_token_embedding_grad(k.get("g", one), k.get("gt", FP32), k.get("gs", 8), one, k.get("bits", 64), k.get("n", 5000),
                                                          k.get("V", 4), k.get("D", 8), 1.0, k.get("pad", -1), 0, k.get("out", one), FP32,
                                                          k.get("os", 8), k.get("scratch", one), k.get("bytes", 1 << 30), None)
     assert grad(gt=INT8) == -2
@@ -36,7 +36,7 @@ def _refusals():
     assert grad(pad=-2) == -1
     assert grad(os=7) == -1 and grad(gs=-1) == -1
     assert grad(g=None) == -1 and grad(out=None) == -1 and grad(scratch=None) == -1
-    assert grad(bytes=need(2, 4, 8) - 1) == -1 and "scratch" in cabi.last_error()
+    assert grad(bytes=need(5000, 4, 8) - 1) == -1 and "scratch" in cabi.last_error()
     assert grad(scratch=8) == -1
 
     q = lambda **k: lib.tbe_b200_quantize_to_group_rows(k.get("x", one), k.get("it", FP32), 8, k.get("E", 2), k.get("D", 8), k.get("g", 32),
@@ -61,8 +61,9 @@ def _refusals():
     assert lin(x=8) == -1 and "aligned" in cabi.last_error()
     assert lin(m=2, xs=9) == -1 and lin(m=0) == 0
     need = lib.tbe_b200_group_row_linear_scratch_bytes
-    assert need(1, 8, 32, FP32) > 0 and need(-1, 8, 32, FP32) == -1 and need(1, 0, 32, FP32) == -1 and need(1, 8, 48, FP32) == -1 and need(1, 8, 32, INT8) == -1
-    assert lin(scratch=None) == -1 and lin(scratch=8) == -1 and lin(bytes=need(1, 8, 32, FP32) - 1) == -1 and "scratch" in cabi.last_error()
+    assert need(1, 8, 32, FP32) == 0 and need(17, 8, 32, FP32) > 0 and need(16, 8192, 32, FP32) > 0      # few vectors need none
+    assert need(-1, 8, 32, FP32) == -1 and need(1, 0, 32, FP32) == -1 and need(1, 8, 48, FP32) == -1 and need(1, 8, 32, INT8) == -1
+    assert lin(m=17, scratch=None) == -1 and lin(m=17, scratch=8) == -1 and lin(m=17, bytes=need(17, 8, 32, FP32) - 1) == -1 and "scratch" in cabi.last_error()
 
 
 def test_no_cpu_path():

@@ -165,7 +165,7 @@ def grad_bound(want, mass, count, dtype):
     return off + (want.abs() + off) * U[dtype] + TINY[dtype] + 2.0 ** -140
 
 
-GRAD_SIZES = [(1, 1, 8), (1, 5000, 64), (31, 7, 40), (32, 511, 1), (33, 512, 36), (64, 513, 256), (1000, 3, 8), (4095, 1000, 24), (4097, 70_000, 8),
+GRAD_SIZES = [(1, 1, 8), (1023, 1000, 128), (1025, 40, 264), (2048, 9, 7), (2049, 9, 7), (1, 5000, 64), (31, 7, 40), (32, 511, 1), (33, 512, 36), (64, 513, 256), (1000, 3, 8), (4095, 1000, 24), (4097, 70_000, 8),
               (9000, 262_143, 16), (20_001, 2, 4), (70_001, 40_000, 12), (300, 50, 1001), (257, 33, 2056)]
 
 
@@ -200,7 +200,7 @@ def test_grad_of_a_large_table(n, V, D, ti, to, kind):
     assert bool((got[(count == 0)[:, 0]] == 0).all())
 
 
-@pytest.mark.parametrize("n,V,D,stride", [(900, 60_000, 200, 264), (900, 60_000, 199, 201), (40, 77, 8, 9)])
+@pytest.mark.parametrize("n,V,D,stride", [(900, 60_000, 200, 264), (900, 60_000, 199, 201), (40, 77, 8, 9), (9000, 60_000, 200, 264), (9000, 60_000, 199, 201)])
 def test_grad_into_rows_that_lie_apart(n, V, D, stride):
     """The C entry point over a wider buffer: every row is written, nothing between the rows."""
     from fbgemm_ascend_b200 import cabi
@@ -209,7 +209,7 @@ def test_grad_into_rows_that_lie_apart(n, V, D, stride):
     dy, t = randn(g, n, D), tokens_of(g, n, V, "hot", torch.int64)
     out = torch.full((V, stride), 7.0, device="cuda")
     need = lib.tbe_b200_token_embedding_grad_scratch_bytes(n, V, D)
-    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    scratch = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
     cabi.check(lib.tbe_b200_token_embedding_grad(dy.data_ptr(), 0, D, t.data_ptr(), 64, n, V, D, 2.0, -1, 0, out.data_ptr(), 0, stride, scratch.data_ptr(),
                                                  need, torch.cuda.current_stream().cuda_stream), "grad")
     assert torch.equal(out[:, :D], ops().token_embedding_grad(dy, t, V, scale=2.0)) and bool((out[:, D:] == 7.0).all())
