@@ -195,7 +195,7 @@ struct LinearArgs {
     void* out;
     int64_t out_stride;
     int32_t* error_flag;
-    int slices_log2;                            // warps that share a row's elements
+    int slices, bands;                          // warps that share a row's elements; groups of rows
     int stages, head_bytes;                     // of a stage; of a row's scales and biases in it
     int64_t tiles;
 };
@@ -275,14 +275,14 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
 {
     constexpr int kPitch = RT * 16 + 4;         // of a state's sums in shared memory: a warp's stores meet no bank twice
     constexpr int kPart = NT * 8 * kPitch;      // one warp's sums
-    constexpr int U = units_at_once(RT), kStates = unit_bytes(NT, P, STEPS), kCodeBytes = kWarps * RT * 16 * U * (kUnit / 2);
+    constexpr int U = units_at_once(RT), kStates = unit_bytes(NT, P, STEPS);
     constexpr int kBuffers = NT == 1 ? 2 : 1;   // of the warps' sums
     constexpr bool LOCAL = !std::is_void<T>::value;
     extern __shared__ __align__(1024) unsigned char smem[];
-    const int bands = kWarps >> a.slices_log2, slices = 1 << a.slices_log2, tile_rows = bands * RT * 16;
-    const int head_bytes = tile_rows * a.head_bytes, state_bytes = LOCAL ? 0 : slices * U * kStates;
+    const int bands = a.bands, slices = a.slices, tile_rows = bands * RT * 16, boxes = (slices * U + 1) / kBoxUnits;
+    const int code_bytes = boxes * tile_rows * 128, head_bytes = tile_rows * a.head_bytes, state_bytes = LOCAL ? 0 : slices * U * kStates;
     // boxes of codes first (1024-byte aligned), then those of heads, the states, sums, barriers
-    unsigned char* heads_at = smem + a.stages * kCodeBytes;
+    unsigned char* heads_at = smem + a.stages * code_bytes;
     unsigned char* states_at = heads_at + a.stages * head_bytes;
     float* red = reinterpret_cast<float*>(states_at + a.stages * state_bytes);
     const uint32_t full = shared_address(red + kBuffers * kWarps * kPart), empty = full + 8 * kMostStages;
@@ -291,7 +291,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     int* largest = reinterpret_cast<int*>(backs + 16);
     unsigned char* local = reinterpret_cast<unsigned char*>(largest + 16);
 
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);      // known to be the same for all lanes
     const int units = (a.D + kUnit - 1) / kUnit, groups = (a.D + (1 << a.group_log2) - 1) >> a.group_log2;
     const int chunks = (units + U * slices - 1) / (U * slices);
     const int64_t m0 = static_cast<int64_t>(blockIdx.y) * (NT * 8);
@@ -300,7 +300,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) {
             barrier_init(full + 8 * i, 1);
-            barrier_init(empty + 8 * i, kWarps);
+            barrier_init(empty + 8 * i, bands * slices);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -322,11 +322,10 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
         auto fetch_rows = [&](int stage) {
             const uint32_t bar = full + 8 * stage;
             const int first = static_cast<int>(tile * tile_rows);
-            barrier_expect(bar, kCodeBytes + head_bytes + states_of(chunk));
+            barrier_expect(bar, code_bytes + head_bytes + states_of(chunk));
             // what lies outside the matrix arrives as zeros
-            const int boxes = slices * U / kBoxUnits;
             for (int k = 0; k < boxes; ++k)
-                box_copy(shared_address(smem + stage * kCodeBytes + k * (tile_rows * 128)), &code_map, (chunk * boxes + k) * 32, first, bar);
+                box_copy(shared_address(smem + stage * code_bytes + k * (tile_rows * 128)), &code_map, (chunk * slices * U + k * kBoxUnits) * (kUnit / 8), first, bar);
             const int g0 = (chunk * slices * U * kUnit) >> a.group_log2;
             box_copy(shared_address(heads_at + stage * head_bytes), &head_map, ((a.D / 2 + 4 * g0) & ~15) / 4, first, bar);
         };
@@ -398,7 +397,8 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");      // `back` is read at a tile's end
     }
-    const int g = row_of(lane >> 2), t = lane & 3, slice = warp & (slices - 1), band = warp >> a.slices_log2;
+    const int g = row_of(lane >> 2), t = lane & 3, slice = warp % slices, band = warp / slices;
+    const bool working = band < bands;          // the others only help at a tile's end
     float y[RT][NT][4];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -408,7 +408,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
             for (int e = 0; e < 4; ++e) y[i][n][e] = 0.0f;
 
     // this lane's places in a stage
-    const unsigned char* code_rows = smem + slice * U / kBoxUnits * (tile_rows * 128) + (band * RT * 16 + g) * 128;
+    const unsigned char* code_rows = smem + slice * U / kBoxUnits * (tile_rows * 128) + (band * RT * 16 + g) * 128;      // not used where band >= bands
     const int half = U == 1 ? slice & 1 : 0;
     const int row8 = 8 * a.head_bytes;
     const unsigned char* head_rows = heads_at + (band * RT * 16 + g) * a.head_bytes;
@@ -420,11 +420,11 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     int stage = 0;
     uint32_t round = 0;
     for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-        for (int c = 0; c < chunks; ++c) {
+        for (int c = working ? 0 : chunks; c < chunks; ++c) {
             if (!barrier_wait(full + 8 * stage, round & 1) && a.error_flag) atomicOr(a.error_flag, 16);
             const int g0 = (c * slices * U * kUnit) >> a.group_log2;
             const unsigned char* heads = head_rows + stage * head_bytes + ((a.D / 2 + 4 * g0) & 15) - 4 * g0;
-            const unsigned char* codes = code_rows + stage * kCodeBytes;
+            const unsigned char* codes = code_rows + stage * code_bytes;
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 const int u = U * (c * slices + slice) + k;
@@ -507,12 +507,11 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
                     y[i][n][e] = 0.0f;
                 }
         workers_sync();
-        const int rows_log2 = 31 - __clz(tile_rows);
-        for (int i = threadIdx.x; i < cols << rows_log2; i += kWorkers) {
-            const int col = i >> rows_log2, row = i & (tile_rows - 1);
+        for (int i = threadIdx.x; i < cols * tile_rows; i += kWorkers) {
+            const int col = i / tile_rows, row = i - col * tile_rows;
             const int64_t r = tile * tile_rows + row;
             if (r >= a.num_rows) continue;
-            const float* from = sums + (row / (RT * 16) << a.slices_log2) * kPart + col * kPitch + row % (RT * 16);
+            const float* from = sums + row / (RT * 16) * slices * kPart + col * kPitch + row % (RT * 16);
             float v = 0.0f;
             for (int k = 0; k < slices; ++k) v += from[k * kPart];
             v *= LOCAL ? backs[col] : __ldcg(a.back + m0 + col);
@@ -572,36 +571,43 @@ int64_t arranged_bytes(int64_t m, int64_t D, int dtype, int group_log2)
     return (m + NT * 8 - 1) / (NT * 8) * units_of(D) * unit_bytes(NT, pieces_of(dtype), steps_of(group_log2));
 }
 
-template <typename T, int RT, int NT, int P, int STEPS>
-int launch_linear(LinearArgs a, cudaStream_t s)
+// How the warps of a block share rows and elements, and what that costs.
+struct Shape {
+    int slices, bands, stages, head_bytes;
+    int64_t tiles, shared, cost;
+};
+
+// Of all shapes the one whose blocks are done first: counted in shares of a stage (4096 codes) that a warp goes through (tiles of
+// a block times chunks of a tile), twice, and one for every tile's end.  Two stages have to fit, and a box is at most 256 rows.
+Shape shape_for(const LinearArgs& a, int RT, int NT, int P, int steps, bool local)
 {
-    constexpr int U = units_at_once(RT);
-    constexpr bool LOCAL = !std::is_void<T>::value;
-    const int sms = sm_count();
+    const int U = units_at_once(RT), sms = sm_count(), shares = (a.D + U * kUnit - 1) / (U * kUnit);
     const int64_t fixed = static_cast<int64_t>(NT == 1 ? 2 : 1) * kWarps * NT * 8 * (RT * 16 + 4) * 4 + 16 * kMostStages +
-                          (LOCAL ? 128 + units_of(a.D) * local_unit_bytes(static_cast<int>(a.m), NT, P, STEPS) : 0);
-    auto stage_bytes = [&](int l) {
-        return static_cast<int64_t>(kWarps) * RT * 16 * U * (kUnit / 2) + static_cast<int64_t>(RT * 16 * (kWarps >> l)) * head_window(a.D, U << l, a.group_log2) +
-               (LOCAL ? 0 : (U << l) * unit_bytes(NT, P, STEPS));
-    };
-    // Shares of the elements: as few as keep every multiprocessor at work to the end, counted in units of time that
-    // a warp needs for its share of a stage; a tile's end is worth about half of one.  A box is at most 256 rows.
-    const int shares = (a.D + U * kUnit - 1) / (U * kUnit), fewest = RT - 1;
-    int64_t best = 0;
-    for (int l = fewest; l <= 4 && (l == fewest || ((1 << l) <= shares && fixed + 2 * stage_bytes(l) <= kMostShared)); ++l) {
-        const int64_t tiles = (a.num_rows + RT * 16 * (kWarps >> l) - 1) / (RT * 16 * (kWarps >> l));
-        const int64_t cost = ((tiles + sms - 1) / sms) * (2 * ((shares + (1 << l) - 1) / (1 << l)) + 1);
-        if (l == fewest || cost < best) {
-            best = cost;
-            a.slices_log2 = l;
-            a.tiles = tiles;
-        }
+                          (local ? 128 + units_of(a.D) * local_unit_bytes(static_cast<int>(a.m), NT, P, steps) : 0);
+    Shape best{};
+    for (int slices = kBoxUnits / U; slices <= kWarps; slices += kBoxUnits / U) {      // whole boxes
+        const int most = 256 / (RT * 16), bands = kWarps / slices < most ? kWarps / slices : most, rows = bands * RT * 16;
+        const int heads = head_window(a.D, U * slices, a.group_log2);
+        const int64_t stage = static_cast<int64_t>(rows) * (slices * U * (kUnit / 2) + heads) + (local ? 0 : slices * U * unit_bytes(NT, P, steps));
+        const int64_t stages = (kMostShared - fixed) / stage, tiles = (a.num_rows + rows - 1) / rows;
+        const int64_t cost = ((tiles + sms - 1) / sms) * (2 * ((shares + slices - 1) / slices) + 1);
+        if (best.slices && (stages < 2 || cost >= best.cost)) continue;
+        const int held = static_cast<int>(stages < kMostStages ? stages : kMostStages);
+        best = Shape{slices, bands, held, heads, tiles, fixed + held * stage, cost};
     }
-    const int tile_rows = RT * 16 * (kWarps >> a.slices_log2);
-    a.head_bytes = head_window(a.D, U << a.slices_log2, a.group_log2);
-    const int64_t stages = (kMostShared - fixed) / stage_bytes(a.slices_log2);
-    a.stages = static_cast<int>(stages < kMostStages ? stages : kMostStages);
-    const int64_t shared = fixed + a.stages * stage_bytes(a.slices_log2);
+    return best;
+}
+
+template <typename T, int RT, int NT, int P, int STEPS>
+int launch_linear(LinearArgs a, const Shape& shape, cudaStream_t s)
+{
+    constexpr bool LOCAL = !std::is_void<T>::value;
+    a.slices = shape.slices;
+    a.bands = shape.bands;
+    a.stages = shape.stages;
+    a.head_bytes = shape.head_bytes;
+    a.tiles = shape.tiles;
+    const int tile_rows = RT * 16 * a.bands, sms = sm_count();
     CUtensorMap codes, heads;
     if (!encode_rows(&codes, a, 32, tile_rows, true) || !encode_rows(&heads, a, a.head_bytes / 4, tile_rows, false))
         return fail(TBE_B200_ERR_CUDA, "group_row_linear: the rows could not be described to the copy engine");
@@ -614,7 +620,7 @@ int launch_linear(LinearArgs a, cudaStream_t s)
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(a.tiles < sms ? a.tiles : sms), static_cast<unsigned>((a.m + NT * 8 - 1) / (NT * 8)));
     config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = shared;
+    config.dynamicSmemBytes = shape.shared;
     config.stream = s;
     config.attrs = &early;
     config.numAttrs = LOCAL ? 0 : 1;
@@ -627,14 +633,18 @@ int launch_linear(LinearArgs a, cudaStream_t s)
 template <typename T, int P>
 int launch_linear(const LinearArgs& a, cudaStream_t s)
 {
-    // Rows 32 to a warp use every state twice; 16 where that leaves multiprocessors without any.
-    const bool many = a.num_rows >= static_cast<int64_t>(64) * sm_count(), two = states_per_block(a.m) == 2;
+    constexpr bool LOCAL = !std::is_void<T>::value;
+    const int NT = states_per_block(a.m), steps = steps_of(a.group_log2);
+    // 32 rows to a warp use every state twice, which makes a stage about a tenth shorter; 16 fit more numbers of rows.
+    const Shape wide = shape_for(a, 2, NT, P, steps, LOCAL), narrow = shape_for(a, 1, NT, P, steps, LOCAL);
+    const bool two = NT == 2, many = 10 * wide.cost <= 11 * narrow.cost;
     auto by_group = [&](auto rt, auto nt) {
-        constexpr int RT = decltype(rt)::value, NT = decltype(nt)::value;
-        switch (a.group_log2) {
-            case 5: return launch_linear<T, RT, NT, P, 1>(a, s);
-            case 6: return launch_linear<T, RT, NT, P, 2>(a, s);
-            default: return launch_linear<T, RT, NT, P, 4>(a, s);
+        constexpr int RT = decltype(rt)::value, N = decltype(nt)::value;
+        const Shape& shape = RT == 2 ? wide : narrow;
+        switch (steps) {
+            case 1: return launch_linear<T, RT, N, P, 1>(a, shape, s);
+            case 2: return launch_linear<T, RT, N, P, 2>(a, shape, s);
+            default: return launch_linear<T, RT, N, P, 4>(a, shape, s);
         }
     };
     const std::integral_constant<int, 1> one{};
