@@ -197,8 +197,8 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* warp_t
 // synchronisation are all that it costs beside the clearing: with nothing to clear, 16384 tokens of 131072 take LATER us.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortBlocks = 8;                       // the largest cluster that every device schedules
-constexpr int kOneBlockKeys = 4 * kSortThreads;      // so many are sorted by a block alone: barriers between blocks cost more
+constexpr int kSortBlocks = 16;                      // the largest cluster; a GPC of this GPU has as many multiprocessors
+constexpr int kOneBlockKeys = 2 * kSortThreads;      // so many are sorted by a block alone: 4096 take 16 us in one, 12 in a cluster
 constexpr int kMostItems = 16;
 constexpr int64_t kClusterKeys = int64_t(kSortBlocks) * kMostItems * kSortThreads;
 
@@ -307,6 +307,9 @@ __device__ __forceinline__ unsigned long long* sort_in_shared(const SortInput& i
     const int per = items * kSortThreads;
     const int64_t first = static_cast<int64_t>(mine) * per;
     const int at = warp * (32 * items) + lane;
+    // to / per: a quotient below 256 of numbers below 256 by one of at most 16, by its inverse in 1 / 65536
+    const uint32_t inverse = (65536u + items - 1) / items;
+    auto rank_of = [&](uint32_t to) { return ((to / kSortThreads) * inverse) >> 16; };
     auto sync_all = [&] {
         if (cluster > 1) cluster_sync();
         else __syncthreads();
@@ -372,7 +375,7 @@ __device__ __forceinline__ unsigned long long* sort_in_shared(const SortInput& i
             const uint32_t d = (key[j] >> (p * width)) & (bins - 1), to = base[d] + count[warp][d] + rank[j];
             const unsigned long long both = (static_cast<unsigned long long>(key[j]) << 32) | pos[j];
             if (cluster > 1)
-                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(shared_of(buf + to % per, to / per)), "l"(both) : "memory");
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(shared_of(buf + (to - rank_of(to) * per), rank_of(to))), "l"(both) : "memory");
             else
                 buf[to] = both;
         }
@@ -386,6 +389,7 @@ __global__ void __launch_bounds__(kSortThreads, 1)
 sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int width, uint2* __restrict__ sorted, const FillArgs fill, int unit)
 {
     extern __shared__ __align__(16) unsigned char sort_smem[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x >= cluster) {
         clear_rows(fill, unit, blockIdx.x - cluster, gridDim.x - cluster, sort_smem);
         return;
@@ -405,8 +409,8 @@ sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int w
     }
 }
 
-// ---- more tokens than a cluster holds: per digit tile histograms, one block that turns them into places (digit by digit,
-// tile by tile), and the scatter ----------------------------------------------------------------------------------
+// ---- more tokens than a cluster holds: per digit tile histograms, their running sums tile by tile, and the
+// scatter ----------------------------------------------------------------------------------
 constexpr int kWarps = kThreads / 32;
 constexpr int kSortItems = 16;
 constexpr int kSortTile = kThreads * kSortItems;
@@ -435,34 +439,34 @@ sort_histogram_kernel(const SortInput in, const uint2* __restrict__ from, int sh
     for (int b = threadIdx.x; b < bins; b += kThreads) hist[static_cast<int64_t>(b) * gridDim.x + blockIdx.x] = count[b];
 }
 
-// Exclusive running sum of `count` numbers in place, by one block.
-__global__ void __launch_bounds__(1024) sort_places_kernel(uint32_t* __restrict__ hist, int64_t count)
+// One warp per digit: the counts of its tiles become exclusive running sums, `totals` their sum.
+__global__ void __launch_bounds__(kThreads) sort_places_kernel(uint32_t* __restrict__ hist, int64_t tiles, int bins, uint32_t* __restrict__ totals)
 {
-    __shared__ uint32_t warp_tot[32];
+    const int lane = threadIdx.x & 31, bin = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (bin >= bins) return;
+    uint32_t* row = hist + bin * tiles;
     uint32_t carry = 0;
-    for (int64_t base = 0; base < count; base += 4096) {
-        const int64_t first = base + threadIdx.x * 4;
-        uint32_t v[4], mine = 0, total;
+    for (int64_t base = 0; base < tiles; base += 32) {
+        const uint32_t c = base + lane < tiles ? row[base + lane] : 0u;
+        uint32_t incl = c;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = first + j < count ? hist[first + j] : 0u;
-            mine += v[j];
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t up = __shfl_up_sync(kFull, incl, d);
+            if (lane >= d) incl += up;
         }
-        uint32_t run = carry + block_exclusive(mine, warp_tot, total);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (first + j < count) hist[first + j] = run;
-            run += v[j];
-        }
-        carry += total;
+        if (base + lane < tiles) row[base + lane] = carry + incl - c;
+        carry += __shfl_sync(kFull, incl, 31);
     }
+    if (lane == 0) totals[bin] = carry;
 }
 
 template <bool FIRST>
 __global__ void __launch_bounds__(kThreads)
-sort_scatter_kernel(const SortInput in, const uint2* __restrict__ from, int shift, int bins, const uint32_t* __restrict__ places, uint2* __restrict__ to)
+sort_scatter_kernel(const SortInput in, const uint2* __restrict__ from, int shift, int bins, const uint32_t* __restrict__ places,
+                    const uint32_t* __restrict__ totals, uint2* __restrict__ to)
 {
     __shared__ uint32_t count[kWarps][kMaxBins];
+    __shared__ uint32_t warp_tot[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int b = threadIdx.x; b < kWarps * kMaxBins; b += kThreads) (&count[0][0])[b] = 0;
     __syncthreads();
@@ -476,9 +480,24 @@ sort_scatter_kernel(const SortInput in, const uint2* __restrict__ from, int shif
     }
 #pragma unroll
     for (int j = 0; j < kSortItems; ++j) rank[j] = warp_rank((entry[j].x >> shift) & (bins - 1), base + j * 32 < in.n, count[warp]);
+    // digits of this thread: two neighbouring ones, behind all of the threads before it
+    const int b0 = 2 * threadIdx.x;
+    const uint32_t t0 = b0 < bins ? __ldg(totals + b0) : 0u, t1 = b0 + 1 < bins ? __ldg(totals + b0 + 1) : 0u;
+    uint32_t incl = t0 + t1;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t up = __shfl_up_sync(kFull, incl, d);
+        if (lane >= d) incl += up;
+    }
+    if (lane == 31) warp_tot[warp] = incl;
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += kThreads) {
-        uint32_t run = places[static_cast<int64_t>(b) * gridDim.x + blockIdx.x];
+    uint32_t smaller = incl - t0 - t1;
+    for (int w = 0; w < warp; ++w) smaller += warp_tot[w];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int b = b0 + i;
+        if (b >= bins) break;
+        uint32_t run = smaller + (i ? t0 : 0u) + places[static_cast<int64_t>(b) * gridDim.x + blockIdx.x];
         for (int w = 0; w < kWarps; ++w) {
             const uint32_t c = count[w][b];
             count[w][b] = run;
@@ -588,6 +607,8 @@ template <typename TI, typename TO, bool ALIGNED, bool INTO>
 __global__ void __launch_bounds__(kThreads)
 sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const FillArgs fill, int fillers)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x < fillers) {
         __shared__ __align__(16) unsigned char zeros[INTO ? 16 : kFewZeroBytes];
         if constexpr (!INTO) {
@@ -687,25 +708,34 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
 constexpr int kJoinColumns = 128;
 constexpr int kFewPieces = 64;
 
-// How many of the tiles t0, t0 + direction, ... begin with `key`, one after the other.
-__device__ __forceinline__ int64_t tiles_that_begin_with(const SumArgs& a, uint32_t key, int64_t t0, int direction)
+// How many of the tiles t0, t0 + direction, ... begin with `key`, one after the other.  Of the first kThreads of them this thread's
+// begins with `here`.
+__device__ __forceinline__ uint32_t begin_of(const SumArgs& a, int64_t t) { return t >= 0 && t < a.tiles ? __ldg(a.sorted + t * a.tile_rows).x : a.none; }
+__device__ __forceinline__ int64_t tiles_that_begin_with(const SumArgs& a, uint32_t key, int64_t t0, int direction, uint32_t here)
 {
     int64_t found = 0;
     for (;;) {
-        const int64_t t = t0 + direction * (found + threadIdx.x);
-        const int more = __syncthreads_count(t >= 0 && t < a.tiles && __ldg(a.sorted + t * a.tile_rows).x == key);
+        const int more = __syncthreads_count(here == key);
         found += more;
         if (more < kThreads) return found;
+        here = begin_of(a, t0 + direction * (found + threadIdx.x));
     }
 }
 
 __device__ __forceinline__ float4 add_pieces(const SumArgs& a, int64_t tile, int64_t from, int64_t to, int c)
 {
+    constexpr int kTogether = 8;      // loads in flight, whether there are as many pieces or not
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int64_t k = from; k < to; ++k) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(a.parts + ((tile + k) * 2 + (k == 0 ? 1 : 0)) * a.padded_D + c));
-        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    for (int64_t k0 = from; k0 < to; k0 += kTogether) {
+        float4 v[kTogether];
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k)
+            if (k0 + k < to) v[k] = __ldg(reinterpret_cast<const float4*>(a.parts + ((tile + k0 + k) * 2 + (k0 + k == 0 ? 1 : 0)) * a.padded_D + c));
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k)
+            if (k0 + k < to) {
+                sum.x += v[k].x; sum.y += v[k].y; sum.z += v[k].z; sum.w += v[k].w;
+            }
     }
     return sum;
 }
@@ -731,11 +761,17 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(const SumArgs a, T
     __shared__ float4 partial[kWarps][32];
     const int64_t tile = blockIdx.x, first = tile * a.tile_rows, next = first + a.tile_rows;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // everything that an ordinary tile has to know at once
     const uint32_t begins = __ldg(a.sorted + first).x, before = first > 0 ? __ldg(a.sorted + first - 1).x : a.none;
     const uint32_t ends = next < a.n ? __ldg(a.sorted + next - 1).x : a.none, after = next < a.n ? __ldg(a.sorted + next).x : a.none;
+    const uint32_t far_back = begin_of(a, tile - kFewPieces / 2), far_on = begin_of(a, tile + kFewPieces / 2),
+                   here = threadIdx.x < kFewPieces ? begin_of(a, tile + 1 + threadIdx.x) : a.none;
     const bool came_in = begins != a.none && before == begins;
-    if (came_in) {
-        const int64_t back = tiles_that_begin_with(a, begins, tile - 1, -1), reach = tiles_that_begin_with(a, begins, tile + 1, 1);
+    // more than kFewPieces pieces reach half as many tiles on one side at least
+    if (came_in && (far_back == begins || far_on == begins)) {
+        const int64_t back = tiles_that_begin_with(a, begins, tile - 1, -1, begin_of(a, tile - 1 - threadIdx.x)),
+                      reach = tiles_that_begin_with(a, begins, tile + 1, 1, begin_of(a, tile + 1 + threadIdx.x));
         // the first of the `back` tiles may be where the token starts
         const int64_t far = tile - back, lead = far > 0 && __ldg(a.sorted + far * a.tile_rows - 1).x == begins ? far - 1 : far;
         const int64_t pieces = tile + reach - lead + 1;
@@ -760,7 +796,7 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(const SumArgs a, T
         }
     }
     if (ends == a.none || after != ends || (came_in && begins == ends)) return;
-    const int64_t pieces = 1 + tiles_that_begin_with(a, ends, tile + 1, 1);
+    const int pieces = 1 + __syncthreads_count(here == ends);      // or more, where it is more than kFewPieces
     const int c = (blockIdx.y * kWarps + warp) * kJoinColumns + lane * 4;
     if (pieces > kFewPieces || c >= a.D) return;
     put_sum<TO, INTO>(a, out + static_cast<int64_t>(ends) * a.out_stride, add_pieces(a, tile, 0, pieces, c), c);
@@ -907,7 +943,7 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
     l.slices = static_cast<int>((D + (kColumns << l.lanes_log2) - 1) / (kColumns << l.lanes_log2));
     const int64_t groups = kResidentWarps << (5 - l.lanes_log2), want = (n * l.slices + groups - 1) / groups;
     // long tokens leave a piece per tile: not too many of them where rows are narrow
-    const int64_t least = n <= 8192 ? 8 : 32;
+    const int64_t least = n <= 8192 ? 8 : D <= 256 ? 64 : 32;
     l.tile_rows = static_cast<int>(want < least ? least : want > 256 ? 256 : (want + kAhead - 1) / kAhead * kAhead);
     l.tiles = (n + l.tile_rows - 1) / l.tile_rows;
     l.padded_D = static_cast<int>((D + 7) / 8 * 8);
@@ -915,7 +951,7 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
     int64_t at = 0;
     l.sorted[0] = at; at += align16(8 * n);
     l.sorted[1] = at; at += l.sort_tiles ? align16(8 * n) : 0;
-    l.hist = at; at += align16(4 * kMaxBins * l.sort_tiles);
+    l.hist = at; at += l.sort_tiles ? align16(4 * kMaxBins * (l.sort_tiles + 1)) : 0;
     l.met = at; at += align16((num_embeddings + 31) / 32 * 4);
     l.parts = at; at += l.tiles * 2 * l.padded_D * 4;
     l.total = at;
@@ -970,6 +1006,14 @@ int launch_sort(const SortInput& in, int cluster, int items, int passes, int wid
     config.stream = s;
     config.attrs = &together;
     config.numAttrs = 1;
+    static std::atomic<uint64_t> large{0};      // clusters of more than 8 blocks, once per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !(large.load(std::memory_order_relaxed) >> dev & 1)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            return fail(TBE_B200_ERR_CUDA, "sort_tokens_kernel: clusters of %d blocks are not allowed", kSortBlocks);
+        if (dev < 64) large.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    }
     const cudaError_t e = cudaLaunchKernelEx(&config, kernel, in, cluster, items, passes, width, sorted, fill, unit);
     if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "sort_tokens_kernel: %s", cudaGetErrorString(e));
     return check_launch("sort_tokens_kernel");
@@ -1002,19 +1046,37 @@ int sort_and_clear(const SortInput& in, const GradPlan& l, char* scratch, const 
         return launch_sort<kMostItems>(in, cluster, items, passes, width, sorted, fill, unit, fillers, s);
     }
     uint32_t* hist = reinterpret_cast<uint32_t*>(scratch + l.hist);
+    uint32_t* totals = hist + kMaxBins * l.sort_tiles;
     const unsigned tiles = static_cast<unsigned>(l.sort_tiles);
     for (int p = 0; p < passes; ++p) {
         const uint2* from = reinterpret_cast<const uint2*>(scratch + l.sorted[half]);
         uint2* to = reinterpret_cast<uint2*>(scratch + l.sorted[half ^ 1]);
         if (p == 0) sort_histogram_kernel<true><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist);
         else sort_histogram_kernel<false><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist);
-        sort_places_kernel<<<1, 1024, 0, s>>>(hist, static_cast<int64_t>(bins) * tiles);
-        if (p == 0) sort_scatter_kernel<true><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist, to);
-        else sort_scatter_kernel<false><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist, to);
+        sort_places_kernel<<<static_cast<unsigned>((bins + kWarps - 1) / kWarps), kThreads, 0, s>>>(hist, tiles, bins, totals);
+        if (p == 0) sort_scatter_kernel<true><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist, totals, to);
+        else sort_scatter_kernel<false><<<tiles, kThreads, 0, s>>>(in, from, p * width, bins, hist, totals, to);
         if (const int rc = check_launch("sort kernels")) return rc;
         half ^= 1;
     }
     return TBE_B200_OK;
+}
+
+// early: its blocks may come up while the kernel before it ends; they wait for it themselves.
+template <typename... Params, typename... Args>
+int launch_behind(const char* what, bool can_be_early, void (*kernel)(Params...), dim3 grid, cudaStream_t s, Args... args)
+{
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(kThreads);
+    config.stream = s;
+    config.attrs = &early;
+    config.numAttrs = can_be_early ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
+    return e == cudaSuccess ? check_launch(what) : fail(TBE_B200_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
 template <typename TI, typename TO, bool INTO>
@@ -1023,14 +1085,13 @@ int launch_sums(const SumArgs& a, const TI* grad, TO* out, const FillArgs& fill,
     const int fillers = fill.early < fill.rows ? sm_count() : 0;
     const int64_t blocks = ((a.tiles * a.slices << a.lanes_log2) + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffff - fillers) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding_grad: too many tokens");
-    const unsigned g = static_cast<unsigned>(blocks + fillers);
     constexpr int kWhole = kVec<TI>;
     const bool aligned = a.D % kWhole == 0 && rows_aligned(grad, a.grad_stride, sizeof(TI), kWhole) && rows_aligned(out, a.out_stride, sizeof(TO), kWhole);
-    if (aligned) sum_tiles_kernel<TI, TO, true, INTO><<<g, kThreads, 0, s>>>(a, grad, out, fill, fillers);
-    else sum_tiles_kernel<TI, TO, false, INTO><<<g, kThreads, 0, s>>>(a, grad, out, fill, fillers);
-    if (const int rc = check_launch("sum_tiles_kernel")) return rc;
-    join_parts_kernel<TO, INTO><<<dim3(static_cast<unsigned>(a.tiles), static_cast<unsigned>((a.D + kWarps * kJoinColumns - 1) / (kWarps * kJoinColumns))), kThreads, 0, s>>>(a, out);
-    return check_launch("join_parts_kernel");
+    auto* sums = aligned ? sum_tiles_kernel<TI, TO, true, INTO> : sum_tiles_kernel<TI, TO, false, INTO>;
+    if (const int rc = launch_behind("sum_tiles_kernel", fillers == 0, sums, dim3(static_cast<unsigned>(blocks + fillers)), s, a, grad, out, fill, fillers)) return rc;
+    // (clearing blocks that come up early would crowd on the few multiprocessors that have room: 197 instead of 161 us)
+    const dim3 grid(static_cast<unsigned>(a.tiles), static_cast<unsigned>((a.D + kWarps * kJoinColumns - 1) / (kWarps * kJoinColumns)));
+    return launch_behind("join_parts_kernel", true, join_parts_kernel<TO, INTO>, grid, s, a, out);
 }
 
 }  // namespace
@@ -1095,7 +1156,7 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
     if (!l.few && n <= kClusterKeys) {
         // Writing alone runs at 4 TB/s, beside reads at most of what a copy writes: the sums' reads cost little then.  As many rows
         // are cleared beside the sort as that takes; where little is left, all.
-        const int64_t beside_sort = ((int64_t(36) << 20) + n * 1400) / fill.row_bytes / 32 * 32;
+        const int64_t beside_sort = ((int64_t(32) << 20) + n * 1100) / fill.row_bytes / 32 * 32;
         if (beside_sort + beside_sort / 4 < fill.rows) {
             fill.early = beside_sort;
             fill.met = reinterpret_cast<uint32_t*>(base + l.met);
