@@ -50,10 +50,11 @@ __device__ __forceinline__ void clear_piece(Piece<T, VEC>& r)
     for (int i = 0; i < Piece<T, VEC>::kWords; ++i) r.w[i] = 0u;
 }
 
-// A row that starts at any element: the 16-byte border in front of it, and where it begins and ends behind that, bytes.
+// A row (of one element at least) that starts at any element: the 16-byte border in front of it, where it begins behind that, and
+// the last 16-byte word that holds some of it, bytes.
 struct SplitRow {
     const char* base;
-    int begin, end;
+    int begin, last;
 
     template <typename T>
     __device__ __forceinline__ void of(const T* row, int D)
@@ -61,12 +62,12 @@ struct SplitRow {
         const uintptr_t a = reinterpret_cast<uintptr_t>(row);
         base = reinterpret_cast<const char*>(a & ~uintptr_t(15));
         begin = static_cast<int>(a & 15);
-        end = begin + D * static_cast<int>(sizeof(T));
+        last = (begin + D * static_cast<int>(sizeof(T)) - 1) & ~15;
     }
 };
 
 // A piece of such a row, which may reach past its end: read in aligned 16-byte words, none of which lies wholly outside the
-// row, and shifted into place.  What is not the row's is left as it is there.
+// row (past the end the last one stands in), and shifted into place.  What is not the row's is whatever lies there.
 template <typename T, int VEC>
 struct SplitPiece {
     static constexpr int kBytes = Piece<T, VEC>::kBytes;
@@ -74,14 +75,13 @@ struct SplitPiece {
     uint4 q[kQuads];
     int offset;      // of the first element in the first word, bytes
 
-    // from element c on; c at most the row's number of elements
+    // from element c on
     __device__ __forceinline__ void load(const SplitRow& row, int c)
     {
-        const int at = row.begin + c * static_cast<int>(sizeof(T)), first = at & ~15, behind = at + kBytes < row.end ? at + kBytes : row.end;
+        const int at = row.begin + c * static_cast<int>(sizeof(T)), first = at & ~15;
         offset = at & 15;
-        const char* p = row.base + first;
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) q[i] = first + 16 * i < behind ? ldg16(p + 16 * i) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < kQuads; ++i) q[i] = ldg16(row.base + min(first + 16 * i, row.last));
     }
     __device__ __forceinline__ Piece<T, VEC> piece() const
     {
