@@ -166,7 +166,7 @@ def grad_bound(want, mass, count, dtype):
 
 
 GRAD_SIZES = [(1, 1, 8), (1023, 1000, 128), (1025, 40, 264), (2048, 9, 7), (2049, 9, 7), (1, 5000, 64), (31, 7, 40), (32, 511, 1), (33, 512, 36), (64, 513, 256), (1000, 3, 8), (4095, 1000, 24), (4097, 70_000, 8),
-              (9000, 262_143, 16), (20_001, 2, 4), (70_001, 40_000, 12), (300, 50, 1001), (257, 33, 2056)]
+              (9000, 262_143, 16), (20_001, 2, 4), (70_001, 40_000, 12), (140_000, 300, 8), (262_145, 70_000, 4), (300, 50, 1001), (257, 33, 2056)]
 
 
 @pytest.mark.parametrize("n,V,D", GRAD_SIZES)
@@ -446,6 +446,44 @@ def test_linear_of_shapes_and_strides():
     assert torch.equal(ops().group_row_linear(x, rows[7:20], 64), got[:, :, 7:20])
 
 
+# ---- places behind 2^31 -------------------------------------------------------------------------------------------
+
+def test_rows_far_into_a_large_table():
+    g = gen(21)
+    V, D = 140_000, 16_400
+    w = torch.zeros(V, D, device="cuda", dtype=BF16)              # 4.6 GB, 2.3 billion elements
+    t = torch.tensor([V - 1, 0, 131_071, 131_072, V - 1, -1], device="cuda")
+    w[t[:4]] = randn(g, 4, D, dtype=BF16)
+    assert torch.equal(ops().token_embedding(w, t).double(), lookup64(w, t, 1.0))
+    dy = randn(g, 6, D, dtype=BF16)
+    for again in (1, 500):                                        # a few tokens, and more of them
+        rows, tokens = dy.repeat(again, 1), t.repeat(again)
+        got = ops().token_embedding_grad(rows, tokens, V)
+        for v in (V - 1, 0, 131_071, 131_072):
+            want, mass, count = grad64(rows, (tokens == v).long() - 1, 1, 1.0)
+            within(got[v:v + 1], want, grad_bound(want, mass, count, BF16))
+        got[t[:4]] = 0
+        assert not bool(got.any())
+        del got, rows
+
+
+def test_group_rows_far_into_a_large_table():
+    import fbgemm_ascend_b200 as fa
+    g = gen(22)
+    V, D = 2_200_000, 2048
+    table = fa.GroupRowTable(V, D, 128)                           # 2.4 GB
+    last = randn(g, 5, D, std=0.1)
+    table.assign_rows_from_float(last, V - 5)
+    t = torch.tensor([V - 1, V - 5, 7, V], device="cuda")
+    want = ops().group_rows_to_float(table.rows[V - 5:], D, 128)
+    assert torch.equal(table(t).float(), torch.stack([want[4], want[0], torch.zeros_like(want[0]), torch.zeros_like(want[0])]).bfloat16().float())
+    x = randn(g, 2, D, dtype=BF16)
+    scores = table.linear(x, output_dtype=SparseType.FP32)
+    exact, off = linear_want(x, table.rows[V - 5:], D, 128, None)
+    within(scores[:, V - 5:], exact, off + (exact.abs() + off) * U[F32])
+    assert not bool(scores[:, :V - 5].any())
+
+
 # ---- together, streams, graphs ------------------------------------------------------------------------------------
 
 def test_train_publish_serve():
@@ -481,14 +519,14 @@ def test_train_publish_serve():
     within(scores, want, off + (want.abs() + off) * U[F32])
 
 
-def test_graphs_replay_with_new_inputs():
+@pytest.mark.parametrize("n,m,V,D", [(700, 3, 3000, 128), (5000, 20, 3000, 104), (20_000, 16, 200_000, 136), (270_001, 1, 3000, 16)])
+def test_graphs_replay_with_new_inputs(n, m, V, D):
     """Two captured graphs of the same calls, replayed in turn with new contents, and an eager call in between."""
     g = gen(12)
-    V, D, n = 3000, 128, 700
     held = []
     for _ in range(2):
         s = {"w": randn(g, V, D, dtype=BF16), "t": tokens_of(g, n, V, "wild", torch.int64), "dy": randn(g, n, D, dtype=BF16), "into": torch.zeros(V, D, device="cuda"),
-             "x": randn(g, 3, D, dtype=BF16)}
+             "x": randn(g, m, D, dtype=BF16)}
 
         def step(s=s):
             rows = ops().quantize_to_group_rows(s["w"], 64)
@@ -584,6 +622,8 @@ def test_refusals():
         (lambda: o.group_row_linear(w[:, :8], rows[:, :15], 64), "bytes"),
         (lambda: o.group_row_linear(w.clone().requires_grad_(), rows, 64), "no gradient"),
         (lambda: o.group_row_linear(w.long(), rows, 64), "float32, float16 or bfloat16"),
+        (lambda: o.group_row_linear(w, torch.zeros(161, dtype=torch.uint8, device="cuda")[1:].view(10, 16), 64), "16-byte aligned"),
+        (lambda: o.group_row_embedding(torch.zeros(161, dtype=torch.uint8, device="cuda")[1:].view(10, 16), t, 16, 64), "16-byte aligned"),
     ]
     for call, text in bad:
         with pytest.raises(RuntimeError, match=text):
