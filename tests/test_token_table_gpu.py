@@ -165,7 +165,7 @@ def grad_bound(want, mass, count, dtype):
     return off + (want.abs() + off) * U[dtype] + TINY[dtype] + 2.0 ** -140
 
 
-GRAD_SIZES = [(1, 1, 8), (1023, 1000, 128), (1025, 40, 264), (2048, 9, 7), (2049, 9, 7), (1, 5000, 64), (31, 7, 40), (32, 511, 1), (33, 512, 36), (64, 513, 256), (1000, 3, 8), (4095, 1000, 24), (4097, 70_000, 8),
+GRAD_SIZES = [(1, 1, 8), (1023, 1000, 128), (1025, 40, 264), (2048, 9, 7), (2049, 9, 7), (40, 30, 8193), (1, 5000, 64), (31, 7, 40), (32, 511, 1), (33, 512, 36), (64, 513, 256), (1000, 3, 8), (4095, 1000, 24), (4097, 70_000, 8),
               (9000, 262_143, 16), (20_001, 2, 4), (70_001, 40_000, 12), (140_000, 300, 8), (262_145, 70_000, 4), (300, 50, 1001), (257, 33, 2056)]
 
 
@@ -244,6 +244,13 @@ def test_grad_of_strided_broadcast_and_empty_rows():
     check(torch.ones((), device="cuda").expand(6, 10, 24))
     none = torch.empty(0, dtype=torch.int64, device="cuda")
     assert torch.equal(ops().token_embedding_grad(torch.empty(0, 24, device="cuda"), none, 5), torch.zeros(5, 24, device="cuda"))
+    for V, D in ((3, 8200), (17_000_000, 4)):                                    # tables that few tokens' own form does not take
+        junk = torch.full((V, D), float("nan"), device="cuda")
+        del junk
+        assert not bool(ops().token_embedding_grad(torch.empty(0, D, device="cuda"), none, V).any())
+        dy, one = randn(g, 1, D), torch.tensor([V - 1], device="cuda")
+        got = ops().token_embedding_grad(dy, one, V)
+        assert torch.equal(got[V - 1:], dy) and not bool(got[:V - 1].any())
     kept = randn(g, 5, 24)
     assert torch.equal(ops().token_embedding_grad_(kept.clone(), torch.empty(0, 24, device="cuda"), none), kept)
     assert ops().token_embedding_grad(randn(g, 60, 24), t.view(-1), 0).shape == (0, 24)
