@@ -196,7 +196,8 @@ struct LinearArgs {
     int64_t out_stride;
     int32_t* error_flag;
     int slices, bands;                          // warps that share a row's elements; groups of rows
-    int stages, head_bytes;                     // of a stage; of a row's scales and biases in it
+    int stages, head_bytes;                     // head_bytes: of a row's scales and biases in a stage
+    int buffers;                                // of the warps' sums, two where they do not cost a stage
     int64_t tiles;
 };
 
@@ -276,7 +277,6 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     constexpr int kPitch = RT * 16 + 4;         // of a state's sums in shared memory: a warp's stores meet no bank twice
     constexpr int kPart = NT * 8 * kPitch;      // one warp's sums
     constexpr int U = units_at_once(RT), kStates = unit_bytes(NT, P, STEPS);
-    constexpr int kBuffers = NT == 1 ? 2 : 1;   // of the warps' sums
     constexpr bool LOCAL = !std::is_void<T>::value;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int bands = a.bands, slices = a.slices, tile_rows = bands * RT * 16, boxes = (slices * U + 1) / kBoxUnits;
@@ -285,9 +285,9 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
     unsigned char* heads_at = smem + a.stages * code_bytes;
     unsigned char* states_at = heads_at + a.stages * head_bytes;
     float* red = reinterpret_cast<float*>(states_at + a.stages * state_bytes);
-    const uint32_t full = shared_address(red + kBuffers * kWarps * kPart), empty = full + 8 * kMostStages;
+    const uint32_t full = shared_address(red + a.buffers * kWarps * kPart), empty = full + 8 * kMostStages;
     // LOCAL: what undoes the states' scales, the largest of each, the states
-    float* backs = red + kBuffers * kWarps * kPart + 4 * kMostStages;
+    float* backs = red + a.buffers * kWarps * kPart + 4 * kMostStages;
     int* largest = reinterpret_cast<int*>(backs + 16);
     unsigned char* local = reinterpret_cast<unsigned char*>(largest + 16);
 
@@ -519,7 +519,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
             store_any(a.out, a.out_dtype, (m0 + col) * a.out_stride + r, v);
         }
         // the next tile's sums go to the other buffer, where there is one: its own barrier parts the two after it
-        if (kBuffers == 1) workers_sync();
+        if (a.buffers == 1) workers_sync();
         else buffer ^= 1;
     }
 }
@@ -573,7 +573,7 @@ int64_t arranged_bytes(int64_t m, int64_t D, int dtype, int group_log2)
 
 // How the warps of a block share rows and elements, and what that costs.
 struct Shape {
-    int slices, bands, stages, head_bytes;
+    int slices, bands, stages, head_bytes, buffers;
     int64_t tiles, shared, cost;
 };
 
@@ -582,18 +582,19 @@ struct Shape {
 Shape shape_for(const LinearArgs& a, int RT, int NT, int P, int steps, bool local)
 {
     const int U = units_at_once(RT), sms = sm_count(), shares = (a.D + U * kUnit - 1) / (U * kUnit);
-    const int64_t fixed = static_cast<int64_t>(NT == 1 ? 2 : 1) * kWarps * NT * 8 * (RT * 16 + 4) * 4 + 16 * kMostStages +
-                          (local ? 128 + units_of(a.D) * local_unit_bytes(static_cast<int>(a.m), NT, P, steps) : 0);
+    const int64_t sums = static_cast<int64_t>(kWarps) * NT * 8 * (RT * 16 + 4) * 4;
+    const int64_t fixed = sums + 16 * kMostStages + (local ? 128 + units_of(a.D) * local_unit_bytes(static_cast<int>(a.m), NT, P, steps) : 0);
+    auto fitting = [&](int64_t bytes, int64_t stage) { return static_cast<int>((kMostShared - bytes) / stage < kMostStages ? (kMostShared - bytes) / stage : kMostStages); };
     Shape best{};
     for (int slices = kBoxUnits / U; slices <= kWarps; slices += kBoxUnits / U) {      // whole boxes
         const int most = 256 / (RT * 16), bands = kWarps / slices < most ? kWarps / slices : most, rows = bands * RT * 16;
         const int heads = head_window(a.D, U * slices, a.group_log2);
         const int64_t stage = static_cast<int64_t>(rows) * (slices * U * (kUnit / 2) + heads) + (local ? 0 : slices * U * unit_bytes(NT, P, steps));
-        const int64_t stages = (kMostShared - fixed) / stage, tiles = (a.num_rows + rows - 1) / rows;
+        const int64_t tiles = (a.num_rows + rows - 1) / rows;
+        const int stages = fitting(fixed, stage), buffers = fitting(fixed + sums, stage) == stages ? 2 : 1;
         const int64_t cost = ((tiles + sms - 1) / sms) * (2 * ((shares + slices - 1) / slices) + 1);
         if (best.slices && (stages < 2 || cost >= best.cost)) continue;
-        const int held = static_cast<int>(stages < kMostStages ? stages : kMostStages);
-        best = Shape{slices, bands, held, heads, tiles, fixed + held * stage, cost};
+        best = Shape{slices, bands, stages, heads, buffers, tiles, fixed + (buffers - 1) * sums + stages * stage, cost};
     }
     return best;
 }
@@ -606,6 +607,7 @@ int launch_linear(LinearArgs a, const Shape& shape, cudaStream_t s)
     a.bands = shape.bands;
     a.stages = shape.stages;
     a.head_bytes = shape.head_bytes;
+    a.buffers = shape.buffers;
     a.tiles = shape.tiles;
     const int tile_rows = RT * 16 * a.bands, sms = sm_count();
     CUtensorMap codes, heads;
