@@ -33,19 +33,55 @@ __device__ __forceinline__ Piece<T, 8> load_eight(const T* p)
     return r;
 }
 
-// A warp's row and its share of it: `shares` warps to a row.
-__device__ __forceinline__ void place_of(int64_t unit, int shares, int64_t& row, int& share)
+// How warps share rows: a wide row (more than a warp's lanes hold at once) takes `shares` warps, narrow rows 1 << lanes_log2 lanes
+// each, and a warp as many of them side by side as fit, some times over.
+struct Sharing {
+    int lanes_log2, shares;
+};
+inline Sharing sharing_of(int64_t D, int per_lane, int at_once)
 {
-    row = (unit >> 32) ? unit / shares : static_cast<int64_t>(static_cast<uint32_t>(unit) / static_cast<uint32_t>(shares));
-    share = static_cast<int>(unit - row * shares);
+    Sharing s{0, 1};
+    while (s.lanes_log2 < 5 && (static_cast<int64_t>(per_lane) << s.lanes_log2) < D) ++s.lanes_log2;
+    if (D > 32 * per_lane) s.shares = static_cast<int>((D + 32 * per_lane * at_once - 1) / (32 * per_lane * at_once));
+    return s;
 }
+// Warps that rows of D elements need.
+inline int64_t warps_for(int64_t nrows, const Sharing& s, int64_t D, int per_lane, int at_once)
+{
+    const int64_t rows_per_warp = static_cast<int64_t>(32 >> s.lanes_log2) * at_once;
+    return D > 32 * per_lane ? nrows * s.shares : (nrows + rows_per_warp - 1) / rows_per_warp;
+}
+
+// The row and the first column of this lane's k-th piece.
+template <bool NARROW, int PER_LANE, int AT_ONCE>
+struct Places {
+    int64_t row;
+    int column, rows_apart;
+
+    __device__ __forceinline__ Places(int64_t unit, const Sharing& s)
+    {
+        const int lane = threadIdx.x & 31;
+        if constexpr (NARROW) {
+            rows_apart = 32 >> s.lanes_log2;
+            row = unit * (rows_apart * AT_ONCE) + (lane >> s.lanes_log2);
+            column = (lane & ((1 << s.lanes_log2) - 1)) * PER_LANE;
+        } else {
+            rows_apart = 0;
+            row = (unit >> 32) ? unit / s.shares : static_cast<int64_t>(static_cast<uint32_t>(unit) / static_cast<uint32_t>(s.shares));
+            column = static_cast<int>(unit - row * s.shares) * (32 * PER_LANE * AT_ONCE) + lane * PER_LANE;
+        }
+    }
+    __device__ __forceinline__ int64_t row_of(int k) const { return NARROW ? row + k * rows_apart : row; }
+    __device__ __forceinline__ int column_of(int k) const { return NARROW ? column : column + k * (32 * PER_LANE); }
+};
 
 // ---- quantize -------------------------------------------------------------------------------------------------------
 //
 // Bound by instructions as much as by HBM: a lane takes 16 neighbouring elements, which halves what a group costs beside its
-// elements (its two divisions, the exchange of its smallest and largest), a warp two times 512 of a row.  The ends of 16-bit
+// elements (its two divisions, the exchange of its smallest and largest), twice.  The ends of 16-bit
 // rows are found two elements at a time, and the smallest travels between lanes with the largest's negative in one word.
-constexpr int kQuantSpan = 512, kQuantAtOnce = 2;
+// 65536 rows of 4096 bf16 in groups of 128: 150 us, 4.5 TB/s (345 us with eight elements a lane).
+constexpr int kQuantLane = 16, kQuantAtOnce = 2;
 
 // The smallest and largest of the words' elements.
 template <typename T, int W>
@@ -98,20 +134,17 @@ struct Ends {
     }
 };
 
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, bool NARROW>
 __global__ void __launch_bounds__(kThreads)
-quantize_group_rows_kernel(const T* __restrict__ in, int64_t in_stride, int64_t nrows, int D, int group_log2, int shares, int64_t row_bytes,
+quantize_group_rows_kernel(const T* __restrict__ in, int64_t in_stride, int64_t nrows, int D, int group_log2, Sharing share, int64_t row_bytes,
                            uint8_t* __restrict__ rows)
 {
     constexpr int W = 2 * Piece<T, 8>::kWords;
-    const int lane = threadIdx.x & 31, sharing = 1 << (group_log2 - 4);
-    int64_t r;
-    int share;
-    place_of(static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5), shares, r, share);
-    if (r >= nrows) return;
-    const int c0 = share * (kQuantAtOnce * kQuantSpan) + lane * 16;
-    const T* from = in + r * in_stride + c0;
-    uint8_t* row = rows + r * row_bytes;
+    const int lane = threadIdx.x & 31;
+    // lanes that hold one group; a row shorter than a group is one by itself
+    const int sharing = 1 << (NARROW && share.lanes_log2 < group_log2 - 4 ? share.lanes_log2 : group_log2 - 4);
+    const Places<NARROW, kQuantLane, kQuantAtOnce> places(static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5), share);
+    if (places.row - (NARROW ? lane >> share.lanes_log2 : 0) >= nrows) return;      // the same for the whole warp
     uint32_t w[kQuantAtOnce][W];
 #pragma unroll
     for (int k = 0; k < kQuantAtOnce; ++k)
@@ -119,15 +152,18 @@ quantize_group_rows_kernel(const T* __restrict__ in, int64_t in_stride, int64_t 
         for (int h = 0; h < 2; ++h) {
             Piece<T, 8> p;
             clear_piece(p);
-            if (c0 + k * kQuantSpan + 8 * h < D) p = load_eight<T, WIDE>(from + k * kQuantSpan + 8 * h);
+            const int c = places.column_of(k) + 8 * h;
+            if (places.row_of(k) < nrows && c < D) p = load_eight<T, WIDE>(in + places.row_of(k) * in_stride + c);
 #pragma unroll
             for (int i = 0; i < W / 2; ++i) w[k][h * (W / 2) + i] = p.w[i];
         }
 #pragma unroll
     for (int k = 0; k < kQuantAtOnce; ++k) {
-        const int c = c0 + k * kQuantSpan;
-        if (c - lane * 16 >= D) break;                            // the same for the whole warp
-        const bool live = c < D, second = c + 8 < D;              // the lane has elements; it has all 16
+        const int c = places.column_of(k);
+        const int64_t r = places.row_of(k);
+        const bool live = c < D && r < nrows, second = live && c + 8 < D;      // the lane has elements; it has all 16
+        if (!__any_sync(kFull, live)) break;
+        uint8_t* row = rows + r * row_bytes;
         Ends<T, W> ends;
         ends.of(w[k], second);
         if (!live) {
@@ -184,17 +220,22 @@ quantize_group_rows_kernel(const T* __restrict__ in, int64_t in_stride, int64_t 
             *reinterpret_cast<uint32_t*>(row + D / 2 + 4 * (c >> group_log2)) =
                 static_cast<uint32_t>(__half_as_ushort(scale_h)) | (static_cast<uint32_t>(__half_as_ushort(bias_h)) << 16);
     }
-    if (share == 0) {
-        const int64_t used = D / 2 + 4 * ((D + (1 << group_log2) - 1) >> group_log2);
-        for (int64_t b = used + 4 * lane; b < row_bytes; b += 128) *reinterpret_cast<uint32_t*>(row + b) = 0u;
+    // what lies behind the groups
+    const int lanes = 1 << share.lanes_log2;
+    const int64_t used = D / 2 + 4 * ((D + (1 << group_log2) - 1) >> group_log2);
+#pragma unroll
+    for (int k = 0; k < (NARROW ? kQuantAtOnce : 1); ++k) {
+        if (places.row_of(k) >= nrows || (!NARROW && places.column >= 32 * kQuantLane)) break;
+        for (int64_t b = used + 4 * (lane & (lanes - 1)); b < row_bytes; b += 4 * lanes) *reinterpret_cast<uint32_t*>(rows + places.row_of(k) * row_bytes + b) = 0u;
     }
 }
 
 // ---- lookup ---------------------------------------------------------------------------------------------------------
 //
-// A lane takes eight elements, one word of codes, of each of four times 256 of a row: stores are whole 16-byte pieces side by
-// side.  Bound by the result's bytes (writing alone runs at 4 TB/s) and by instructions.
-constexpr int kSpan = 256, kLookupAtOnce = 4;
+// A lane takes eight elements, one word of codes, four times over: of a wide row 256 elements apart, so that stores are whole
+// 16-byte pieces side by side, or of four rows.  Bound by the result's bytes (writing alone runs at 4 TB/s) and by instructions.
+// 16384 rows of 4096 in groups of 128 as bf16: 24 us, 6.0 TB/s of what has to be moved.
+constexpr int kLookupLane = 8, kLookupAtOnce = 4;
 
 // Eight codes as numbers: a nibble or'ed into the low bits of 1024 in fp16 (16 steps apart for the upper nibble of a byte) is that
 // plus the code, and taking it off leaves the code exactly.
@@ -212,38 +253,39 @@ __device__ __forceinline__ void codes_of(uint32_t w, float (&q)[8])
     }
 }
 
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, bool NARROW>
 __global__ void __launch_bounds__(kThreads)
-group_row_embedding_kernel(const uint8_t* __restrict__ rows, int64_t num_embeddings, int64_t row_bytes, int D, int group_log2, int shares,
+group_row_embedding_kernel(const uint8_t* __restrict__ rows, int64_t num_embeddings, int64_t row_bytes, int D, int group_log2, Sharing share,
                            const void* __restrict__ tokens, int wide, int64_t n, float scale, T* __restrict__ out, int64_t out_stride,
                            int32_t* error_flag)
 {
-    const int lane = threadIdx.x & 31;
-    int64_t i;
-    int share;
-    place_of(static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5), shares, i, share);
-    if (i >= n) return;
-    int64_t t = i;
-    if (tokens) t = wide ? __ldg(reinterpret_cast<const long long*>(tokens) + i) : static_cast<int64_t>(__ldg(reinterpret_cast<const int*>(tokens) + i));
-    const bool met = t >= 0 && t < num_embeddings;
-    if (!met && t != -1 && error_flag && share == 0 && lane == 0) atomicOr(error_flag, 4);
-    const int c0 = share * (kLookupAtOnce * kSpan) + lane * 8;
-    const uint8_t* row = rows + (met ? t : 0) * row_bytes;
-    const uint8_t* words = row + c0 / 2;
-    const uint8_t* heads = row + D / 2 + 4 * (c0 >> group_log2);
+    const Places<NARROW, kLookupLane, kLookupAtOnce> places(static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5), share);
+    constexpr int kRows = NARROW ? kLookupAtOnce : 1;
+    const uint8_t* row[kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+        const int64_t i = places.row_of(k);
+        int64_t t = i;
+        if (tokens && i < n) t = wide ? __ldg(reinterpret_cast<const long long*>(tokens) + i) : static_cast<int64_t>(__ldg(reinterpret_cast<const int*>(tokens) + i));
+        const bool met = i < n && t >= 0 && t < num_embeddings;
+        if (!met && i < n && t != -1 && error_flag && places.column == 0) atomicOr(error_flag, 4);
+        row[k] = met ? rows + t * row_bytes : nullptr;
+    }
     uint32_t codes[kLookupAtOnce], head[kLookupAtOnce];
 #pragma unroll
     for (int k = 0; k < kLookupAtOnce; ++k) {
+        const uint8_t* from = row[NARROW ? k : 0];
+        const int c = places.column_of(k);
         codes[k] = head[k] = 0u;
-        if (met && c0 + k * kSpan < D) {
-            codes[k] = ldg4(words + k * (kSpan / 2));
-            head[k] = ldg4(heads + k * (4 * kSpan >> group_log2));
+        if (from && c < D) {
+            codes[k] = ldg4(from + c / 2);
+            head[k] = ldg4(from + D / 2 + 4 * (c >> group_log2));
         }
     }
-    T* to = out + i * out_stride + c0;
 #pragma unroll
     for (int k = 0; k < kLookupAtOnce; ++k) {
-        if (c0 + k * kSpan >= D) break;
+        const int c = places.column_of(k);
+        if (c >= D || places.row_of(k) >= n) break;
         // of a row that is none codes, scale and bias are 0
         const __half2 ab = *reinterpret_cast<const __half2*>(&head[k]);
         const float a = __low2float(ab), b = __high2float(ab);
@@ -251,16 +293,17 @@ group_row_embedding_kernel(const uint8_t* __restrict__ rows, int64_t num_embeddi
         codes_of(codes[k], v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], a, b);
-        if (scale != 1.0f && met) {
+        if (scale != 1.0f && row[NARROW ? k : 0]) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= scale;
         }
-        if constexpr (WIDE) store_piece<T, 8>(to + k * kSpan, v);
+        T* to = out + places.row_of(k) * out_stride + c;
+        if constexpr (WIDE) store_piece<T, 8>(to, v);
         else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float one[1] = {v[e]};
-                store_piece<T, 1>(to + k * kSpan + e, one);
+                store_piece<T, 1>(to + e, one);
             }
         }
     }
@@ -299,17 +342,17 @@ extern "C" int tbe_b200_quantize_to_group_rows(const void* input, int32_t input_
     if (input_stride < 0) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "quantize_to_group_rows: negative row stride");
     if (nrows == 0 || D == 0) return TBE_B200_OK;
     if (!input || !rows) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "quantize_to_group_rows: NULL pointer");
-    const int64_t shares = (D + kQuantAtOnce * kQuantSpan - 1) / (kQuantAtOnce * kQuantSpan), blocks = (nrows * shares + kThreads / 32 - 1) / (kThreads / 32);
+    const Sharing share = sharing_of(D, kQuantLane, kQuantAtOnce);
+    const int64_t blocks = (warps_for(nrows, share, D, kQuantLane, kQuantAtOnce) + kThreads / 32 - 1) / (kThreads / 32);
     if (blocks > 0x7fffffff) return fail(TBE_B200_ERR_UNSUPPORTED, "quantize_to_group_rows: too many rows");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return with_element(input_dtype, [&](auto* ti) {
         using T = std::remove_pointer_t<decltype(ti)>;
         const T* in = static_cast<const T*>(input);
-        const int g = group_log2_of(group_size);
-        if (rows_aligned(in, input_stride, ib, 8))
-            quantize_group_rows_kernel<T, true><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(in, input_stride, nrows, static_cast<int>(D), g, static_cast<int>(shares), row_bytes, rows);
-        else
-            quantize_group_rows_kernel<T, false><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(in, input_stride, nrows, static_cast<int>(D), g, static_cast<int>(shares), row_bytes, rows);
+        const bool wide = rows_aligned(in, input_stride, ib, 8), narrow = D <= 32 * kQuantLane;
+        auto* kernel = wide ? (narrow ? quantize_group_rows_kernel<T, true, true> : quantize_group_rows_kernel<T, true, false>)
+                            : (narrow ? quantize_group_rows_kernel<T, false, true> : quantize_group_rows_kernel<T, false, false>);
+        kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(in, input_stride, nrows, static_cast<int>(D), group_log2_of(group_size), share, row_bytes, rows);
         return check_launch("quantize_group_rows_kernel");
     });
 }
@@ -326,19 +369,18 @@ extern "C" int tbe_b200_group_row_embedding(const uint8_t* rows, int64_t num_emb
     if (!tokens && n > num_embeddings) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "group_row_embedding: %lld rows wanted of %lld", (long long)n, (long long)num_embeddings);
     if (n == 0 || D == 0) return TBE_B200_OK;
     if (!output || (num_embeddings > 0 && !rows)) return fail(TBE_B200_ERR_INVALID_ARGUMENT, "group_row_embedding: NULL pointer");
-    const int64_t shares = (D + kLookupAtOnce * kSpan - 1) / (kLookupAtOnce * kSpan), blocks = (n * shares + kThreads / 32 - 1) / (kThreads / 32);
+    const Sharing share = sharing_of(D, kLookupLane, kLookupAtOnce);
+    const int64_t blocks = (warps_for(n, share, D, kLookupLane, kLookupAtOnce) + kThreads / 32 - 1) / (kThreads / 32);
     if (blocks > 0x7fffffff) return fail(TBE_B200_ERR_UNSUPPORTED, "group_row_embedding: too many tokens");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return with_element(output_dtype, [&](auto* to) {
         using T = std::remove_pointer_t<decltype(to)>;
         T* o = static_cast<T*>(output);
-        const int g = group_log2_of(group_size);
-        if (rows_aligned(o, output_stride, ob, 8))
-            group_row_embedding_kernel<T, true><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(
-                rows, num_embeddings, row_bytes, static_cast<int>(D), g, static_cast<int>(shares), tokens, token_bits == 64, n, scale, o, output_stride, error_flag);
-        else
-            group_row_embedding_kernel<T, false><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(
-                rows, num_embeddings, row_bytes, static_cast<int>(D), g, static_cast<int>(shares), tokens, token_bits == 64, n, scale, o, output_stride, error_flag);
+        const bool whole = rows_aligned(o, output_stride, ob, 8), narrow = D <= 32 * kLookupLane;
+        auto* kernel = whole ? (narrow ? group_row_embedding_kernel<T, true, true> : group_row_embedding_kernel<T, true, false>)
+                             : (narrow ? group_row_embedding_kernel<T, false, true> : group_row_embedding_kernel<T, false, false>);
+        kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(rows, num_embeddings, row_bytes, static_cast<int>(D), group_log2_of(group_size), share, tokens,
+                                                                  token_bits == 64, n, scale, o, output_stride, error_flag);
         return check_launch("group_row_embedding_kernel");
     });
 }

@@ -228,7 +228,7 @@ __device__ __forceinline__ void clear_run(char* p, int64_t bytes, int64_t thread
                      "r"(run) : "memory");
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
-    const int64_t edge = (bytes - body) / unit;
+    const int64_t edge = (bytes - body) >> (unit == 4 ? 2 : 1);
     for (int64_t i = thread; i < edge; i += threads) {
         char* q = i * unit < head ? p + i * unit : p + body + i * unit;
         if (unit == 4) *reinterpret_cast<uint32_t*>(q) = 0u;
@@ -707,8 +707,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
 }
 
 // A token that starts in tile t and goes on: its piece in slot 1 of t and slot 0 of the tiles that it reaches, added in order.
-// A block looks at a tile and 128 columns for each of its warps, which add up a token of up to kFewPieces pieces alone.  A longer
-// one occupies as many tiles, whose blocks have nothing else to do: each takes 128 columns in turn, with its warps' sums of
+// A warp looks at a tile and 128 columns, and adds up a token of up to kFewPieces pieces alone.  A longer one occupies as many tiles, whose blocks have nothing else to do: each takes 128 columns in turn, with its warps' sums of
 // equal runs of the pieces added in order.
 constexpr int kJoinColumns = 128;
 constexpr int kFewPieces = 64;
@@ -760,72 +759,86 @@ __device__ __forceinline__ void put_sum(const SumArgs& a, TO* row, float4 sum, i
     }
 }
 
+// `share_log2`: log2 of the warps that share a tile's columns; a block looks at as many tiles as its warps allow.
 template <typename TO, bool INTO>
-__global__ void __launch_bounds__(kThreads) join_parts_kernel(const SumArgs a, TO* out)
+__global__ void __launch_bounds__(kThreads, 4) join_parts_kernel(const SumArgs a, TO* out, int share_log2)
 {
     __shared__ float4 partial[kWarps][32];
-    const int64_t tile = blockIdx.x, first = tile * a.tile_rows, next = first + a.tile_rows;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ int is_long[kWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, here_tiles = kWarps >> share_log2;
+    const int64_t first_tile = static_cast<int64_t>(blockIdx.x) * here_tiles, tile = first_tile + (warp >> share_log2);
+    const int64_t first = tile * a.tile_rows, next = first + a.tile_rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // everything that an ordinary tile has to know at once
-    const uint32_t begins = __ldg(a.sorted + first).x, before = first > 0 ? __ldg(a.sorted + first - 1).x : a.none;
-    const uint32_t ends = next < a.n ? __ldg(a.sorted + next - 1).x : a.none, after = next < a.n ? __ldg(a.sorted + next).x : a.none;
-    const uint32_t far_back = begin_of(a, tile - kFewPieces / 2), far_on = begin_of(a, tile + kFewPieces / 2),
-                   here = threadIdx.x < kFewPieces ? begin_of(a, tile + 1 + threadIdx.x) : a.none;
+    auto key_at = [&](int64_t i) { return i >= 0 && i < a.n ? __ldg(a.sorted + i).x : a.none; };
+    const uint32_t begins = key_at(first), before = key_at(first - 1), ends = key_at(next - 1), after = key_at(next);
+    const uint32_t far_back = begin_of(a, tile - kFewPieces / 2), far_on = begin_of(a, tile + kFewPieces / 2);
+    const uint32_t here0 = begin_of(a, tile + 1 + lane), here1 = begin_of(a, tile + 33 + lane);
     const bool came_in = begins != a.none && before == begins;
     // more than kFewPieces pieces reach half as many tiles on one side at least
-    if (came_in && (far_back == begins || far_on == begins)) {
-        const int64_t back = tiles_that_begin_with(a, begins, tile - 1, -1, begin_of(a, tile - 1 - threadIdx.x)),
-                      reach = tiles_that_begin_with(a, begins, tile + 1, 1, begin_of(a, tile + 1 + threadIdx.x));
-        // the first of the `back` tiles may be where the token starts
-        const int64_t far = tile - back, lead = far > 0 && __ldg(a.sorted + far * a.tile_rows - 1).x == begins ? far - 1 : far;
-        const int64_t pieces = tile + reach - lead + 1;
-        if (pieces > kFewPieces) {
-            const int64_t run = (pieces + kWarps - 1) / kWarps, from = warp * run < pieces ? warp * run : pieces, to = from + run < pieces ? from + run : pieces;
-            // the tile where it starts has blocks of its own only if it begins with it; the others share the columns
-            const int64_t helpers = (pieces - 1) * gridDim.y, me = (tile - lead - 1) * gridDim.y + blockIdx.y;
-            for (int64_t chunk = me; chunk * kJoinColumns < a.D; chunk += helpers) {
-                const int c = static_cast<int>(chunk) * kJoinColumns + lane * 4;
-                partial[warp][lane] = c < a.D ? add_pieces(a, lead, from, to, c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                __syncthreads();
-                if (warp == 0 && c < a.D) {
-                    float4 sum = partial[0][lane];
-                    for (int w = 1; w < kWarps; ++w) {
-                        const float4 v = partial[w][lane];
-                        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-                    }
-                    put_sum<TO, INTO>(a, out + static_cast<int64_t>(begins) * a.out_stride, sum, c);
+    if (lane == 0) is_long[warp] = came_in && (far_back == begins || far_on == begins);
+    const bool onward = next < a.n && ends != a.none && after == ends && !(came_in && begins == ends);
+    if (onward) {
+        const int pieces = 1 + __popc(__ballot_sync(kFull, here0 == ends)) + __popc(__ballot_sync(kFull, here1 == ends));      // or more than kFewPieces
+        const int c = ((static_cast<int>(blockIdx.y) << share_log2) + (warp & ((1 << share_log2) - 1))) * kJoinColumns + lane * 4;
+        if (pieces <= kFewPieces && c < a.D) put_sum<TO, INTO>(a, out + static_cast<int64_t>(ends) * a.out_stride, add_pieces(a, tile, 0, pieces, c), c);
+    }
+    __syncthreads();
+    uint32_t key = a.none;      // neighbouring tiles mostly belong to one long token: it is measured once
+    int64_t lead = 0, pieces = 0;
+    for (int i = 0; i < here_tiles; ++i) {
+        if (!is_long[i << share_log2]) continue;
+        const int64_t t = first_tile + i;
+        const uint32_t begins_here = key_at(t * a.tile_rows);
+        if (begins_here != key) {
+            key = begins_here;
+            const int64_t back = tiles_that_begin_with(a, key, t - 1, -1, begin_of(a, t - 1 - threadIdx.x)),
+                          reach = tiles_that_begin_with(a, key, t + 1, 1, begin_of(a, t + 1 + threadIdx.x));
+            // the first of the `back` tiles may be where the token starts
+            const int64_t far = t - back;
+            lead = key_at(far * a.tile_rows - 1) == key ? far - 1 : far;
+            pieces = t + reach - lead + 1;
+        }
+        if (pieces <= kFewPieces) continue;
+        const int64_t run = (pieces + kWarps - 1) / kWarps, from = warp * run < pieces ? warp * run : pieces, to = from + run < pieces ? from + run : pieces;
+        // the tile where it starts has blocks of its own only if it begins with it; the others share the columns
+        const int64_t helpers = (pieces - 1) * gridDim.y, me = (t - lead - 1) * gridDim.y + blockIdx.y;
+        for (int64_t chunk = me; chunk * kJoinColumns < a.D; chunk += helpers) {
+            const int c = static_cast<int>(chunk) * kJoinColumns + lane * 4;
+            partial[warp][lane] = c < a.D ? add_pieces(a, lead, from, to, c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            __syncthreads();
+            if (warp == 0 && c < a.D) {
+                float4 sum = partial[0][lane];
+                for (int w = 1; w < kWarps; ++w) {
+                    const float4 v = partial[w][lane];
+                    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
                 }
-                __syncthreads();
+                put_sum<TO, INTO>(a, out + static_cast<int64_t>(key) * a.out_stride, sum, c);
             }
+            __syncthreads();
         }
     }
-    if (ends == a.none || after != ends || (came_in && begins == ends)) return;
-    const int pieces = 1 + __syncthreads_count(here == ends);      // or more, where it is more than kFewPieces
-    const int c = (blockIdx.y * kWarps + warp) * kJoinColumns + lane * 4;
-    if (pieces > kFewPieces || c >= a.D) return;
-    put_sum<TO, INTO>(a, out + static_cast<int64_t>(ends) * a.out_stride, add_pieces(a, tile, 0, pieces, c), c);
 }
 
 // ---- gradient of a few tokens: one launch -------------------------------------------------------------------------
 //
-// Where launches are most of the time, every block that sums sorts all tokens for itself; it takes eight lanes' columns of all
-// rows, a tile of the sorted positions to each group of eight lanes, and joins the pieces of the tiles in shared memory.  The
+// Where launches are most of the time, every block that sums sorts all tokens for itself; it takes two to eight lanes' columns of
+// all rows, a tile of the sorted positions to each group of lanes, and joins the pieces of the tiles in shared memory.  The
 // blocks behind those clear the rows that no token names, which each finds for its own rows.
 constexpr int kFewTokens = 2048, kFewItems = kFewTokens / kSortThreads;
-constexpr int kFewLanes = 8, kFewGroups = kSortThreads / kFewLanes;
 constexpr int kMostClearWords = 8 * 1024;      // of rows that one block clears
 constexpr int kMostFewColumns = 8192;
 
-template <typename T> __host__ __device__ constexpr int few_columns() { return kFewLanes * kVec<T>; }      // 128 bytes of a row
-template <typename T> __host__ __device__ constexpr int64_t few_shared_bytes() { return sort_shared_bytes(kFewItems) + int64_t(kFewGroups) * 2 * few_columns<T>() * 4; }
+// two pieces, of every lane's columns
+template <typename T> __host__ __device__ constexpr int64_t few_shared_bytes() { return sort_shared_bytes(kFewItems) + int64_t(kSortThreads) * 2 * kVec<T> * 4; }
 
 template <typename TI, typename TO, bool ALIGNED, bool INTO>
 __global__ void __launch_bounds__(kSortThreads, 1)
 grad_of_few_kernel(const SortInput in, int passes, int width, const TI* __restrict__ grad, int64_t grad_stride, int D, float scale, TO* out, int64_t out_stride,
-                   int sum_blocks, const FillArgs fill, int64_t words_per_block)
+                   int lanes_log2, int sum_blocks, const FillArgs fill, int64_t words_per_block)
 {
-    constexpr int VEC = kVec<TI>, kOne = ALIGNED ? VEC : 1, kRow = few_columns<TI>();
+    constexpr int VEC = kVec<TI>, kOne = ALIGNED ? VEC : 1;
+    const int lanes = 1 << lanes_log2, groups = kSortThreads >> lanes_log2, row_floats = VEC << lanes_log2;
     extern __shared__ __align__(16) unsigned char sort_smem[];
     if (blockIdx.x >= sum_blocks) {
         uint32_t* met = reinterpret_cast<uint32_t*>(sort_smem + kFewZeroBytes);
@@ -846,25 +859,29 @@ grad_of_few_kernel(const SortInput in, int passes, int width, const TI* __restri
     float* parts = reinterpret_cast<float*>(sort_smem + sort_shared_bytes(kFewItems));
     const uint32_t none = static_cast<uint32_t>(in.num_embeddings);
     auto key_of = [&](int i) { return static_cast<uint32_t>(sorted[i] >> 32); };
-    const int group = threadIdx.x / kFewLanes, lane = threadIdx.x % kFewLanes;
-    const int tile_rows = (n + kFewGroups - 1) / kFewGroups, first = group * tile_rows, rows = min(tile_rows, n - first);
-    const int c = blockIdx.x * kRow + lane * VEC;
+    const int group = threadIdx.x >> lanes_log2, lane = threadIdx.x & (lanes - 1);
+    const int tile_rows = (n + groups - 1) / groups, first = group * tile_rows, rows = min(tile_rows, n - first);
+    const int c = blockIdx.x * row_floats + lane * VEC;
     float acc[VEC] = {};
     auto put_part = [&](int slot) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) parts[(group * 2 + slot) * kRow + lane * VEC + e] = acc[e];
+        for (int e = 0; e < VEC; ++e) parts[(group * 2 + slot) * row_floats + lane * VEC + e] = acc[e];
     };
     auto put_row = [&](uint32_t token) {
         TO* row = out + static_cast<int64_t>(token) * out_stride;
+        Piece<TO, kOne> old[INTO ? VEC / kOne : 1];
+        if constexpr (INTO) {
+#pragma unroll
+            for (int i = 0; i < VEC / kOne; ++i)
+                if (c + i * kOne < D) load_piece<TO, kOne, false>(old[i], row + c + i * kOne);
+        }
 #pragma unroll
         for (int i = 0; i < VEC / kOne; ++i) {
             if (c + i * kOne >= D) break;
-            Piece<TO, kOne> old;
-            if constexpr (INTO) load_piece<TO, kOne, false>(old, row + c + i * kOne);
             float v[kOne];
 #pragma unroll
             for (int e = 0; e < kOne; ++e) {
-                if constexpr (INTO) v[e] = fmaf(scale, acc[i * kOne + e], element(old, e));
+                if constexpr (INTO) v[e] = fmaf(scale, acc[i * kOne + e], element(old[i], e));
                 else v[e] = scale * acc[i * kOne + e];
             }
             store_piece<TO, kOne>(row + c + i * kOne, v);
@@ -876,21 +893,18 @@ grad_of_few_kernel(const SortInput in, int passes, int width, const TI* __restri
         cur = key_of(first);
         bool head = first > 0 && key_of(first - 1) == cur;
         for (int r = 0; r < rows && cur != none; r += kAhead) {
-            Piece<TI, VEC> in_row[kAhead];
+            typename std::conditional<ALIGNED, Piece<TI, VEC>, SplitPiece<TI, VEC>>::type in_row[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                clear_piece(in_row[k]);
                 const unsigned long long both = r + k < rows ? sorted[first + r + k] : static_cast<unsigned long long>(none) << 32;
-                if (static_cast<uint32_t>(both >> 32) == none) continue;
+                if (static_cast<uint32_t>(both >> 32) == none || c >= D) continue;
                 const TI* row = grad + static_cast<int64_t>(static_cast<uint32_t>(both)) * grad_stride;
                 if constexpr (ALIGNED) {
-                    if (c < D) load_piece<TI, VEC>(in_row[k], row + c);
-                } else if (c < D) {
+                    load_piece<TI, VEC>(in_row[k], row + c);
+                } else {
                     SplitRow split;
                     split.of(row, D);
-                    SplitPiece<TI, VEC> p;
-                    p.load(split, c);
-                    in_row[k] = p.piece();
+                    in_row[k].load(split, c);
                 }
             }
 #pragma unroll
@@ -906,8 +920,11 @@ grad_of_few_kernel(const SortInput in, int passes, int width, const TI* __restri
                     for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
                     if (cur == none) break;
                 }
+                Piece<TI, VEC> one;
+                if constexpr (ALIGNED) one = in_row[k];
+                else one = in_row[k].piece();
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) acc[e] += element(in_row[k], e);
+                for (int e = 0; e < VEC; ++e) acc[e] += element(one, e);
             }
         }
         if (cur != none) {
@@ -921,7 +938,7 @@ grad_of_few_kernel(const SortInput in, int passes, int width, const TI* __restri
     if (!onward) return;
     for (int g = group + 1; g * tile_rows < n && key_of(g * tile_rows) == cur; ++g)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += parts[g * 2 * kRow + lane * VEC + e];
+        for (int e = 0; e < VEC; ++e) acc[e] += parts[g * 2 * row_floats + lane * VEC + e];
     put_row(cur);
 }
 
@@ -949,8 +966,8 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
     while (l.lanes_log2 < 5 && (kColumns << l.lanes_log2) < D) ++l.lanes_log2;
     l.slices = static_cast<int>((D + (kColumns << l.lanes_log2) - 1) / (kColumns << l.lanes_log2));
     const int64_t groups = kResidentWarps << (5 - l.lanes_log2), want = (n * l.slices + groups - 1) / groups;
-    // long tokens leave a piece per tile: not too many of them where rows are narrow
-    const int64_t least = n <= 8192 ? 8 : D <= 256 ? 64 : 32;
+    // Short tiles for few tokens, whose rows come one after the other; long tokens leave a piece per tile: not too many of them.
+    const int64_t least = n <= 8192 ? 8 : n <= 49152 ? 16 : D <= 256 ? 64 : 32;
     l.tile_rows = static_cast<int>(want < least ? least : want > 256 ? 256 : (want + kAhead - 1) / kAhead * kAhead);
     l.tiles = (n + l.tile_rows - 1) / l.tile_rows;
     l.padded_D = static_cast<int>((D + 7) / 8 * 8);
@@ -984,14 +1001,18 @@ int launch_few(const SortInput& in, const TI* grad, int64_t grad_stride, int D, 
     if (const int rc = allow_shared(reinterpret_cast<const void*>(kernel), shared, allowed[aligned])) return rc;
     int passes, width;
     digits_of(in.num_embeddings, passes, width);
-    const int64_t words = (fill.rows + 31) / 32, sums = (D + few_columns<TI>() - 1) / few_columns<TI>();
+    // as many lanes to a row, up to eight, as leave every second multiprocessor a block
+    int lanes_log2 = 1;
+    auto blocks_of = [&](int l) { return (D + (kWhole << l) - 1) / (kWhole << l); };
+    while (lanes_log2 < 3 && 2 * blocks_of(lanes_log2) > sm_count()) ++lanes_log2;
+    const int64_t words = (fill.rows + 31) / 32, sums = blocks_of(lanes_log2);
     // blocks that clear: 64 KB each at least, one per multiprocessor at most
     int64_t fillers = (fill.rows * fill.row_bytes + 65535) / 65536;
     fillers = fillers < sm_count() ? fillers : sm_count();
     fillers = fillers < words ? fillers : words;
     const int64_t each = fillers ? (words + fillers - 1) / fillers : 0;
     kernel<<<static_cast<unsigned>((in.n ? sums : 0) + fillers), kSortThreads, shared, s>>>(in, passes, width, grad, grad_stride, D, scale, out, out_stride,
-                                                                                           static_cast<int>(in.n ? sums : 0), fill, each);
+                                                                                           lanes_log2, static_cast<int>(in.n ? sums : 0), fill, each);
     return check_launch("grad_of_few_kernel");
 }
 
@@ -1098,8 +1119,11 @@ int launch_sums(const SumArgs& a, const TI* grad, TO* out, const FillArgs& fill,
     auto* sums = aligned ? sum_tiles_kernel<TI, TO, true, INTO> : sum_tiles_kernel<TI, TO, false, INTO>;
     if (const int rc = launch_behind("sum_tiles_kernel", fillers == 0, sums, dim3(static_cast<unsigned>(blocks + fillers)), s, a, grad, out, fill, fillers)) return rc;
     // (clearing blocks that come up early would crowd on the few multiprocessors that have room: 197 instead of 161 us)
-    const dim3 grid(static_cast<unsigned>(a.tiles), static_cast<unsigned>((a.D + kWarps * kJoinColumns - 1) / (kWarps * kJoinColumns)));
-    return launch_behind("join_parts_kernel", true, join_parts_kernel<TO, INTO>, grid, s, a, out);
+    int share_log2 = 0;
+    while ((kJoinColumns << share_log2) < a.D && (1 << share_log2) < kWarps) ++share_log2;
+    const int64_t here = kWarps >> share_log2, columns = kJoinColumns << share_log2;
+    const dim3 grid(static_cast<unsigned>((a.tiles + here - 1) / here), static_cast<unsigned>((a.D + columns - 1) / columns));
+    return launch_behind("join_parts_kernel", true, join_parts_kernel<TO, INTO>, grid, s, a, out, share_log2);
 }
 
 }  // namespace
