@@ -577,11 +577,11 @@ struct Columns {
     }
 };
 
-// The same columns (those of rows of TI) of a row of another type.
-template <typename TI, typename TO, bool ALIGNED>
+// The same columns (those of rows of TI) of a row of another type, kOne at a time.
+template <typename TI, typename TO, int kOne>
 __device__ __forceinline__ void load_row(float (&v)[kColumns], const TO* row, int column, int step, int D)
 {
-    constexpr int VEC = kVec<TI>, kOne = ALIGNED ? VEC : 1;
+    constexpr int VEC = kVec<TI>;
 #pragma unroll
     for (int i = 0; i < kColumns / kOne; ++i) {
         const int c = column + (i * kOne / VEC) * step + (i * kOne) % VEC;
@@ -593,10 +593,10 @@ __device__ __forceinline__ void load_row(float (&v)[kColumns], const TO* row, in
     }
 }
 
-template <typename TI, typename TO, bool ALIGNED>
+template <typename TI, typename TO, int kOne>
 __device__ __forceinline__ void store_row(TO* row, const float (&v)[kColumns], int column, int step, int D)
 {
-    constexpr int VEC = kVec<TI>, kOne = ALIGNED ? VEC : 1;
+    constexpr int VEC = kVec<TI>;
 #pragma unroll
     for (int i = 0; i < kColumns / kOne; ++i) {
         const int c = column + (i * kOne / VEC) * step + (i * kOne) % VEC;
@@ -607,8 +607,9 @@ __device__ __forceinline__ void store_row(TO* row, const float (&v)[kColumns], i
     }
 }
 
-// (Rows that are not aligned, added into others, are 15 % faster with all the registers that one block leaves them.)
-template <typename TI, typename TO, bool ALIGNED, bool INTO>
+// ALIGNED: rows of `grad` are; OUT: elements of a row of the gradient that can be moved together.  (Rows that are not aligned,
+// added into others, are 15 % faster with all the registers that one block leaves them.)
+template <typename TI, typename TO, bool ALIGNED, int OUT, bool INTO>
 __global__ void __launch_bounds__(kThreads, !ALIGNED && INTO ? 1 : 0)
 sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const FillArgs fill, int fillers)
 {
@@ -639,13 +640,13 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
     float acc[kColumns] = {}, kept[kColumns] = {};
     auto put_part = [&](int slot) {
         float* part = a.parts + (tile * 2 + slot) * a.padded_D;
-        store_row<TI, float, true>(part, acc, column, step, a.padded_D);
+        store_row<TI, float, VEC>(part, acc, column, step, a.padded_D);
     };
     auto put_row = [&] {
         float v[kColumns];
 #pragma unroll
         for (int e = 0; e < kColumns; ++e) v[e] = INTO ? fmaf(a.scale, acc[e], kept[e]) : a.scale * acc[e];
-        store_row<TI, TO, ALIGNED>(out + static_cast<int64_t>(cur) * a.out_stride, v, column, step, D);
+        store_row<TI, TO, OUT>(out + static_cast<int64_t>(cur) * a.out_stride, v, column, step, D);
     };
     bool fresh = !head;        // the row in the buffer has still to be fetched
     uint2 next[kAhead];
@@ -663,7 +664,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
             if constexpr (INTO) {
                 const uint32_t before = k == 0 ? cur : now[k == 0 ? 0 : k - 1].x;
                 if (now[k].x != a.none && (now[k].x != before || (r + k == 0 && fresh)))
-                    load_row<TI, TO, ALIGNED>(old[k], out + static_cast<int64_t>(now[k].x) * a.out_stride, column, step, D);
+                    load_row<TI, TO, OUT>(old[k], out + static_cast<int64_t>(now[k].x) * a.out_stride, column, step, D);
             }
         }
 #pragma unroll
@@ -1001,14 +1002,15 @@ int launch_few(const SortInput& in, const TI* grad, int64_t grad_stride, int D, 
     if (const int rc = allow_shared(reinterpret_cast<const void*>(kernel), shared, allowed[aligned])) return rc;
     int passes, width;
     digits_of(in.num_embeddings, passes, width);
-    // as many lanes to a row, up to eight, as leave every second multiprocessor a block
+    // as many lanes to a row, up to eight, as leave every second multiprocessor a block and a tile four rows
     int lanes_log2 = 1;
     auto blocks_of = [&](int l) { return (D + (kWhole << l) - 1) / (kWhole << l); };
-    while (lanes_log2 < 3 && 2 * blocks_of(lanes_log2) > sm_count()) ++lanes_log2;
+    while (lanes_log2 < 3 && (2 * blocks_of(lanes_log2) > sm_count() || (in.n << lanes_log2) < 4 * kSortThreads)) ++lanes_log2;
     const int64_t words = (fill.rows + 31) / 32, sums = blocks_of(lanes_log2);
-    // blocks that clear: 64 KB each at least, one per multiprocessor at most
+    // blocks that clear: 64 KB each at least, one per multiprocessor that sums leave free at most, and half of all at least
+    const int64_t room = sums < sm_count() / 2 ? sm_count() - sums : sm_count() / 2;
     int64_t fillers = (fill.rows * fill.row_bytes + 65535) / 65536;
-    fillers = fillers < sm_count() ? fillers : sm_count();
+    fillers = fillers < room ? fillers : room;
     fillers = fillers < words ? fillers : words;
     const int64_t each = fillers ? (words + fillers - 1) / fillers : 0;
     kernel<<<static_cast<unsigned>((in.n ? sums : 0) + fillers), kSortThreads, shared, s>>>(in, passes, width, grad, grad_stride, D, scale, out, out_stride,
@@ -1116,7 +1118,8 @@ int launch_sums(const SumArgs& a, const TI* grad, TO* out, const FillArgs& fill,
     if (blocks > 0x7fffffff - fillers) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding_grad: too many tokens");
     constexpr int kWhole = kVec<TI>;
     const bool aligned = a.D % kWhole == 0 && rows_aligned(grad, a.grad_stride, sizeof(TI), kWhole) && rows_aligned(out, a.out_stride, sizeof(TO), kWhole);
-    auto* sums = aligned ? sum_tiles_kernel<TI, TO, true, INTO> : sum_tiles_kernel<TI, TO, false, INTO>;
+    const bool fours = a.D % 4 == 0 && rows_aligned(out, a.out_stride, sizeof(TO), 4);
+    auto* sums = aligned ? sum_tiles_kernel<TI, TO, true, kWhole, INTO> : fours ? sum_tiles_kernel<TI, TO, false, 4, INTO> : sum_tiles_kernel<TI, TO, false, 1, INTO>;
     if (const int rc = launch_behind("sum_tiles_kernel", fillers == 0, sums, dim3(static_cast<unsigned>(blocks + fillers)), s, a, grad, out, fill, fillers)) return rc;
     // (clearing blocks that come up early would crowd on the few multiprocessors that have room: 197 instead of 161 us)
     int share_log2 = 0;
