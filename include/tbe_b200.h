@@ -285,8 +285,8 @@ int tbe_b200_token_embedding(const void* weight, int32_t weight_dtype, int64_t n
  * in fp32 and rounded once.  accumulate 0: every row is written, zeros where no token names it; 1: only rows that
  * tokens name are read and written.  Tokens equal to padding_idx (-1: none) take part in no gradient.
  * scratch: tbe_b200_token_embedding_grad_scratch_bytes(n, num_embeddings, D) bytes of device memory, 16-byte aligned,
- * overwritten by the call; two calls that may overlap need separate scratch.  The function returns -1 for sizes that
- * the call refuses.  n and num_embeddings are below 2^31. */
+ * overwritten by the call (0 for few tokens: scratch may be NULL then); two calls that may overlap need separate scratch.
+ * The function returns -1 for sizes that the call refuses.  n and num_embeddings are below 2^31. */
 int64_t tbe_b200_token_embedding_grad_scratch_bytes(int64_t n, int64_t num_embeddings, int64_t D);
 int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtype, int64_t grad_stride, const void* tokens, int32_t token_bits,
                                   int64_t n, int64_t num_embeddings, int64_t D, float scale, int64_t padding_idx,
@@ -309,12 +309,13 @@ int tbe_b200_group_row_embedding(const uint8_t* rows, int64_t num_embeddings, in
                                  int64_t output_stride, int32_t* error_flag, tbe_b200_stream_t stream);
 
 /* Products of a few vectors with every row: output[i, r] = sum over c of input[i, c] * (number c of row r) + bias[r], for
- * m vectors of D elements and num_rows rows; fp32 accumulation, one rounding.  A vector with a non-finite element gets no finite result.  bias (num_rows entries) may be NULL.
+ * m vectors of D elements and num_rows rows; fp32 accumulation, one rounding.  A vector with a non-finite element gets no
+ * finite result (infinities or NaN, not told apart).  bias (num_rows entries) may be NULL.
  * `input` is 16-byte aligned and its rows 16-byte apart in whole pieces; D is at most 2^20.  Made for m up to 16 (a decoding
  * step's states): every 16 vectors read the rows once more.  Waits inside the kernel are bounded; one that ran out would set
  * bit 16 of *error_flag (if given).  scratch: tbe_b200_group_row_linear_scratch_bytes(m, D, group_size, input_dtype) bytes of
- * device memory, 16-byte aligned, overwritten by the call; two calls that may overlap need separate scratch.  The
- * function returns -1 for sizes that the call refuses. */
+ * device memory, 16-byte aligned, overwritten by the call (0 for few and short vectors: scratch may be NULL then); two calls
+ * that may overlap need separate scratch.  The function returns -1 for sizes that the call refuses. */
 int64_t tbe_b200_group_row_linear_scratch_bytes(int64_t m, int64_t D, int32_t group_size, int32_t input_dtype);
 int tbe_b200_group_row_linear(const void* input, int32_t input_dtype, int64_t input_stride, int64_t m, const uint8_t* rows,
                               int64_t num_rows, int64_t row_bytes, int64_t D, int32_t group_size, const void* bias,
