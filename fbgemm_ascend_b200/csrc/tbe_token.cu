@@ -529,6 +529,8 @@ __global__ void __launch_bounds__(kThreads) clear_rows_kernel(const FillArgs fil
 constexpr int kColumns = 8;                 // per lane
 constexpr int kAhead = 4;                   // rows whose loads are in flight together
 
+// What the kernel before writes, `sorted` and `parts`, is read by plain loads: a block may have begun before that kernel ended,
+// and the read-only path may be taken before the wait for it.
 struct SumArgs {
     const uint2* sorted;
     int64_t n;
@@ -635,8 +637,8 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
     const int64_t first = tile * a.tile_rows;
     const int rows = static_cast<int>(a.n - first < a.tile_rows ? a.n - first : a.tile_rows);
     const uint2* entries = a.sorted + first;
-    uint32_t cur = __ldg(entries).x;
-    bool head = first > 0 && __ldg(entries - 1).x == cur;
+    uint32_t cur = entries[0].x;
+    bool head = first > 0 && entries[-1].x == cur;
     float acc[kColumns] = {}, kept[kColumns] = {};
     auto put_part = [&](int slot) {
         float* part = a.parts + (tile * 2 + slot) * a.padded_D;
@@ -651,7 +653,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
     bool fresh = !head;        // the row in the buffer has still to be fetched
     uint2 next[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) next[k] = k < rows ? __ldg(entries + k) : make_uint2(a.none, 0u);
+    for (int k = 0; k < kAhead; ++k) next[k] = k < rows ? entries[k] : make_uint2(a.none, 0u);
     bool over = false;
     for (int r = 0; r < rows && !over; r += kAhead) {
         uint2 now[kAhead];
@@ -668,7 +670,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
             }
         }
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) next[k] = r + kAhead + k < rows ? __ldg(entries + r + kAhead + k) : make_uint2(a.none, 0u);
+        for (int k = 0; k < kAhead; ++k) next[k] = r + kAhead + k < rows ? entries[r + kAhead + k] : make_uint2(a.none, 0u);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             if (over) continue;
@@ -702,20 +704,21 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
         }
     }
     if (cur == a.none) return;
-    const bool goes_on = first + rows < a.n && __ldg(entries + rows).x == cur;
+    const bool goes_on = first + rows < a.n && entries[rows].x == cur;
     if (head || goes_on) put_part(head ? 0 : 1);
     else put_row();
 }
 
 // A token that starts in tile t and goes on: its piece in slot 1 of t and slot 0 of the tiles that it reaches, added in order.
-// A warp looks at a tile and 128 columns, and adds up a token of up to kFewPieces pieces alone.  A longer one occupies as many tiles, whose blocks have nothing else to do: each takes 128 columns in turn, with its warps' sums of
-// equal runs of the pieces added in order.
+// A warp looks at a tile and 128 columns, and adds up a token of up to kFewPieces pieces alone.  A longer one occupies as many
+// tiles, whose blocks have nothing else to do: each takes 128 columns in turn, with its warps' sums of equal runs of the pieces
+// added in order.
 constexpr int kJoinColumns = 128;
 constexpr int kFewPieces = 64;
 
 // How many of the tiles t0, t0 + direction, ... begin with `key`, one after the other.  Of the first kThreads of them this thread's
 // begins with `here`.
-__device__ __forceinline__ uint32_t begin_of(const SumArgs& a, int64_t t) { return t >= 0 && t < a.tiles ? __ldg(a.sorted + t * a.tile_rows).x : a.none; }
+__device__ __forceinline__ uint32_t begin_of(const SumArgs& a, int64_t t) { return t >= 0 && t < a.tiles ? a.sorted[t * a.tile_rows].x : a.none; }
 __device__ __forceinline__ int64_t tiles_that_begin_with(const SumArgs& a, uint32_t key, int64_t t0, int direction, uint32_t here)
 {
     int64_t found = 0;
@@ -735,7 +738,7 @@ __device__ __forceinline__ float4 add_pieces(const SumArgs& a, int64_t tile, int
         float4 v[kTogether];
 #pragma unroll
         for (int k = 0; k < kTogether; ++k)
-            if (k0 + k < to) v[k] = __ldg(reinterpret_cast<const float4*>(a.parts + ((tile + k0 + k) * 2 + (k0 + k == 0 ? 1 : 0)) * a.padded_D + c));
+            if (k0 + k < to) v[k] = *reinterpret_cast<const float4*>(a.parts + ((tile + k0 + k) * 2 + (k0 + k == 0 ? 1 : 0)) * a.padded_D + c);
 #pragma unroll
         for (int k = 0; k < kTogether; ++k)
             if (k0 + k < to) {
@@ -771,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 4) join_parts_kernel(const SumArgs a
     const int64_t first = tile * a.tile_rows, next = first + a.tile_rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // everything that an ordinary tile has to know at once
-    auto key_at = [&](int64_t i) { return i >= 0 && i < a.n ? __ldg(a.sorted + i).x : a.none; };
+    auto key_at = [&](int64_t i) { return i >= 0 && i < a.n ? a.sorted[i].x : a.none; };
     const uint32_t begins = key_at(first), before = key_at(first - 1), ends = key_at(next - 1), after = key_at(next);
     const uint32_t far_back = begin_of(a, tile - kFewPieces / 2), far_on = begin_of(a, tile + kFewPieces / 2);
     const uint32_t here0 = begin_of(a, tile + 1 + lane), here1 = begin_of(a, tile + 33 + lane);
@@ -1007,11 +1010,14 @@ int launch_few(const SortInput& in, const TI* grad, int64_t grad_stride, int D, 
     auto blocks_of = [&](int l) { return (D + (kWhole << l) - 1) / (kWhole << l); };
     while (lanes_log2 < 3 && (2 * blocks_of(lanes_log2) > sm_count() || (in.n << lanes_log2) < 4 * kSortThreads)) ++lanes_log2;
     const int64_t words = (fill.rows + 31) / 32, sums = blocks_of(lanes_log2);
-    // blocks that clear: 64 KB each at least, one per multiprocessor that sums leave free at most, and half of all at least
+    // blocks that clear: 64 KB each at least, one per multiprocessor that sums leave free at most (half of all, if
+    // those are fewer), and as many as their bits of rows take
     const int64_t room = sums < sm_count() / 2 ? sm_count() - sums : sm_count() / 2;
     int64_t fillers = (fill.rows * fill.row_bytes + 65535) / 65536;
     fillers = fillers < room ? fillers : room;
     fillers = fillers < words ? fillers : words;
+    const int64_t least = (words + kMostClearWords - 1) / kMostClearWords;
+    fillers = fillers > least ? fillers : least;
     const int64_t each = fillers ? (words + fillers - 1) / fillers : 0;
     kernel<<<static_cast<unsigned>((in.n ? sums : 0) + fillers), kSortThreads, shared, s>>>(in, passes, width, grad, grad_stride, D, scale, out, out_stride,
                                                                                            lanes_log2, static_cast<int>(in.n ? sums : 0), fill, each);
