@@ -543,50 +543,96 @@ struct SumArgs {
     float* parts;
 };
 
-// A lane's eight columns lie in pieces of 16 bytes, `lanes` pieces apart.
+// Such a load that stays behind the wait (volatile), but that the stores of sums do not hold up, as they would one that may alias.
+__device__ __forceinline__ uint2 entry(const uint2* p)
+{
+    uint2 v;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+
+// A lane's eight columns lie in runs of kRun neighbours, `lanes` runs apart: of 16 bytes where rows are aligned, else of 4, so that
+// the lanes' loads and stores lie side by side wherever a row begins.  (With 16 bytes to a lane there too, read in two aligned words
+// each and shifted, and stored element by element, the gradient of 65537 tokens of 1001 fp16 takes 100 us, not 90.)
 template <typename T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+template <typename T, bool ALIGNED> constexpr int kRun = (ALIGNED ? 16 : 4) / static_cast<int>(sizeof(T));
 
 template <typename T, bool ALIGNED>
 struct Columns {
     static constexpr int VEC = kVec<T>, kPieces = kColumns / VEC;
-    typename std::conditional<ALIGNED, Piece<T, VEC>, SplitPiece<T, VEC>>::type p[kPieces];
+    Piece<T, VEC> p[kPieces];
 
     __device__ __forceinline__ void load(const T* row, int column, int step, int D)
     {
-        SplitRow split;
-        if constexpr (!ALIGNED) split.of(row, D);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int c = column + i * step;
-            if constexpr (ALIGNED) {
-                if (c < D) load_piece<T, VEC>(p[i], row + c);
-                else clear_piece(p[i]);
-            } else {
-                p[i].load(split, c);
-            }
+            if (column + i * step < D) load_piece<T, VEC>(p[i], row + column + i * step);
+            else clear_piece(p[i]);
+        }
+    }
+    __device__ __forceinline__ void add_to(float (&acc)[kColumns]) const
+    {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[i * VEC + e] += element(p[i], e);
+    }
+};
+
+template <>
+struct Columns<float, false> {
+    float v[kColumns];
+
+    __device__ __forceinline__ void load(const float* row, int column, int step, int D)
+    {
+#pragma unroll
+        for (int i = 0; i < kColumns; ++i) v[i] = column + i * step < D ? __ldg(row + column + i * step) : 0.0f;
+    }
+    __device__ __forceinline__ void add_to(float (&acc)[kColumns]) const
+    {
+#pragma unroll
+        for (int i = 0; i < kColumns; ++i) acc[i] += v[i];
+    }
+};
+
+// Two 16-bit elements of a row that starts between the words lie in two: the word that holds the first, and the one that holds
+// the second.  No word is read that holds nothing of the row.
+template <typename T>
+struct Columns<T, false> {
+    static constexpr int kPieces = kColumns / 2;
+    uint32_t first[kPieces], second[kPieces], off;      // off: bits in front of the first element
+
+    __device__ __forceinline__ void load(const T* row, int column, int step, int D)
+    {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row + column);
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+        const uint32_t* q = reinterpret_cast<const uint32_t*>((at + 2) & ~uintptr_t(3));
+        off = static_cast<uint32_t>(at & 2) * 8;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            first[i] = column + i * step < D ? __ldg(p + i * (step / 2)) : 0u;
+            second[i] = column + i * step + 1 < D ? __ldg(q + i * (step / 2)) : 0u;
         }
     }
     __device__ __forceinline__ void add_to(float (&acc)[kColumns]) const
     {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            Piece<T, VEC> r;
-            if constexpr (ALIGNED) r = p[i];
-            else r = p[i].piece();
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[i * VEC + e] += element(r, e);
+            Piece<T, 2> r;
+            r.w[0] = __funnelshift_r(first[i], second[i], off);
+            acc[2 * i] += element(r, 0);
+            acc[2 * i + 1] += element(r, 1);
         }
     }
 };
 
-// The same columns (those of rows of TI) of a row of another type, kOne at a time.
-template <typename TI, typename TO, int kOne>
+// The same columns, in runs of RUN, of a row of another type, kOne at a time.
+template <int RUN, typename TO, int kOne>
 __device__ __forceinline__ void load_row(float (&v)[kColumns], const TO* row, int column, int step, int D)
 {
-    constexpr int VEC = kVec<TI>;
 #pragma unroll
     for (int i = 0; i < kColumns / kOne; ++i) {
-        const int c = column + (i * kOne / VEC) * step + (i * kOne) % VEC;
+        const int c = column + (i * kOne / RUN) * step + (i * kOne) % RUN;
         Piece<TO, kOne> p;
         if (c < D) load_piece<TO, kOne, false>(p, row + c);
         else clear_piece(p);
@@ -595,13 +641,12 @@ __device__ __forceinline__ void load_row(float (&v)[kColumns], const TO* row, in
     }
 }
 
-template <typename TI, typename TO, int kOne>
+template <int RUN, typename TO, int kOne>
 __device__ __forceinline__ void store_row(TO* row, const float (&v)[kColumns], int column, int step, int D)
 {
-    constexpr int VEC = kVec<TI>;
 #pragma unroll
     for (int i = 0; i < kColumns / kOne; ++i) {
-        const int c = column + (i * kOne / VEC) * step + (i * kOne) % VEC;
+        const int c = column + (i * kOne / RUN) * step + (i * kOne) % RUN;
         float one[kOne];
 #pragma unroll
         for (int e = 0; e < kOne; ++e) one[e] = v[i * kOne + e];
@@ -609,10 +654,15 @@ __device__ __forceinline__ void store_row(TO* row, const float (&v)[kColumns], i
     }
 }
 
-// ALIGNED: rows of `grad` are; OUT: elements of a row of the gradient that can be moved together.  (Rows that are not aligned,
-// added into others, are 15 % faster with all the registers that one block leaves them.)
+// ALIGNED: rows of `grad` are; OUT: elements of a row of the gradient that can be moved together.
+// Blocks per multiprocessor: 16-bit rows that are aligned need the loads that four have in flight (101589 tokens of 528 fp16: 74 us,
+// 84 with three); else two, whose registers let the loads of four rows go out together (65537 tokens of 1001 fp16: 90 us, 95 with
+// three); one where old rows are moved element by element as well (16384 tokens into 50000 x 1001 fp32: 54 us, 56 with two).
+template <typename TI, bool ALIGNED, int OUT, bool INTO>
+constexpr int kSumBlocks = ALIGNED && !INTO && sizeof(TI) == 2 ? 4 : !ALIGNED && INTO && OUT == 1 ? 1 : 2;
+
 template <typename TI, typename TO, bool ALIGNED, int OUT, bool INTO>
-__global__ void __launch_bounds__(kThreads, !ALIGNED && INTO ? 1 : 0)
+__global__ void __launch_bounds__(kThreads, (kSumBlocks<TI, ALIGNED, OUT, INTO>))
 sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const FillArgs fill, int fillers)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -632,28 +682,29 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
     const int64_t tile = group / a.slices;
     const int slice = static_cast<int>(group - tile * a.slices);
     if (tile >= a.tiles) return;
-    constexpr int VEC = kVec<TI>;
-    const int step = lanes * VEC, column = slice * (lanes * kColumns) + lane * VEC, D = a.D;
+    constexpr int RUN = kRun<TI, ALIGNED>;
+    const int step = lanes * RUN, column = slice * (lanes * kColumns) + lane * RUN, D = a.D;
     const int64_t first = tile * a.tile_rows;
     const int rows = static_cast<int>(a.n - first < a.tile_rows ? a.n - first : a.tile_rows);
     const uint2* entries = a.sorted + first;
-    uint32_t cur = entries[0].x;
-    bool head = first > 0 && entries[-1].x == cur;
+    uint32_t cur = entry(entries).x;
+    bool head = first > 0 && entry(entries - 1).x == cur;
     float acc[kColumns] = {}, kept[kColumns] = {};
     auto put_part = [&](int slot) {
         float* part = a.parts + (tile * 2 + slot) * a.padded_D;
-        store_row<TI, float, VEC>(part, acc, column, step, a.padded_D);
+        store_row<RUN, float, RUN>(part, acc, column, step, a.padded_D);
     };
     auto put_row = [&] {
         float v[kColumns];
 #pragma unroll
         for (int e = 0; e < kColumns; ++e) v[e] = INTO ? fmaf(a.scale, acc[e], kept[e]) : a.scale * acc[e];
-        store_row<TI, TO, OUT>(out + static_cast<int64_t>(cur) * a.out_stride, v, column, step, D);
+        TO* row = out + static_cast<int64_t>(cur) * a.out_stride;
+        store_row<RUN, TO, OUT>(row, v, column, step, D);
     };
     bool fresh = !head;        // the row in the buffer has still to be fetched
     uint2 next[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) next[k] = k < rows ? entries[k] : make_uint2(a.none, 0u);
+    for (int k = 0; k < kAhead; ++k) next[k] = k < rows ? entry(entries + k) : make_uint2(a.none, 0u);
     bool over = false;
     for (int r = 0; r < rows && !over; r += kAhead) {
         uint2 now[kAhead];
@@ -666,11 +717,11 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
             if constexpr (INTO) {
                 const uint32_t before = k == 0 ? cur : now[k == 0 ? 0 : k - 1].x;
                 if (now[k].x != a.none && (now[k].x != before || (r + k == 0 && fresh)))
-                    load_row<TI, TO, OUT>(old[k], out + static_cast<int64_t>(now[k].x) * a.out_stride, column, step, D);
+                    load_row<RUN, TO, OUT>(old[k], out + static_cast<int64_t>(now[k].x) * a.out_stride, column, step, D);
             }
         }
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) next[k] = r + kAhead + k < rows ? entries[r + kAhead + k] : make_uint2(a.none, 0u);
+        for (int k = 0; k < kAhead; ++k) next[k] = r + kAhead + k < rows ? entry(entries + r + kAhead + k) : make_uint2(a.none, 0u);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             if (over) continue;
@@ -704,7 +755,7 @@ sum_tiles_kernel(const SumArgs a, const TI* __restrict__ grad, TO* out, const Fi
         }
     }
     if (cur == a.none) return;
-    const bool goes_on = first + rows < a.n && entries[rows].x == cur;
+    const bool goes_on = first + rows < a.n && entry(entries + rows).x == cur;
     if (head || goes_on) put_part(head ? 0 : 1);
     else put_row();
 }
@@ -1124,8 +1175,12 @@ int launch_sums(const SumArgs& a, const TI* grad, TO* out, const FillArgs& fill,
     if (blocks > 0x7fffffff - fillers) return fail(TBE_B200_ERR_UNSUPPORTED, "token_embedding_grad: too many tokens");
     constexpr int kWhole = kVec<TI>;
     const bool aligned = a.D % kWhole == 0 && rows_aligned(grad, a.grad_stride, sizeof(TI), kWhole) && rows_aligned(out, a.out_stride, sizeof(TO), kWhole);
-    const bool fours = a.D % 4 == 0 && rows_aligned(out, a.out_stride, sizeof(TO), 4);
-    auto* sums = aligned ? sum_tiles_kernel<TI, TO, true, kWhole, INTO> : fours ? sum_tiles_kernel<TI, TO, false, 4, INTO> : sum_tiles_kernel<TI, TO, false, 1, INTO>;
+    auto* sums = sum_tiles_kernel<TI, TO, true, kWhole, INTO>;
+    if (!aligned) {
+        sums = sum_tiles_kernel<TI, TO, false, 1, INTO>;
+        if constexpr (sizeof(TI) == 2)
+            if (a.D % 2 == 0 && rows_aligned(out, a.out_stride, sizeof(TO), 2)) sums = sum_tiles_kernel<TI, TO, false, 2, INTO>;
+    }
     if (const int rc = launch_behind("sum_tiles_kernel", fillers == 0, sums, dim3(static_cast<unsigned>(blocks + fillers)), s, a, grad, out, fill, fillers)) return rc;
     // (clearing blocks that come up early would crowd on the few multiprocessors that have room: 197 instead of 161 us)
     int share_log2 = 0;
