@@ -234,6 +234,29 @@ def test_grad_into_a_buffer(n, V, D, kind, ti, to):
     assert torch.equal(into[untouched], old[untouched]) and torch.equal(wide[:, D:], beside)
 
 
+@pytest.mark.parametrize("D", [1, 2, 6, 31, 34, 66, 126, 130, 255, 258, 1030])
+@pytest.mark.parametrize("ti,to", [(BF16, F32), (F16, F16), (F32, F32), (F32, BF16)])
+def test_grad_of_rows_that_begin_anywhere(D, ti, to):
+    """More tokens than one launch takes; rows of both matrices 1, 2 or 3 elements behind a border, or alternating."""
+    n, V = 2300, 90
+    g = gen(D)
+    t = tokens_of(g, n, V, "wild", torch.int64)
+    for first, gap in ((0, 0), (1, 1), (2, 2), (3, 5), (1, 0)):
+        wide = randn(g, n * (D + gap) + first, dtype=ti, std=0.01)
+        dy = wide[first:].view(n, D + gap)[:, :D]
+        want, mass, count = grad64(dy, t, V, 0.5)
+        got = ops().token_embedding_grad(dy, t, V, scale=0.5, output_dtype=CODE[to])
+        within(got, want, grad_bound(want, mass, count, to))
+        buffer = randn(g, V * (D + gap) + first + 9, dtype=to, std=0.01)
+        was = buffer.clone()
+        view = lambda b: b[first:first + V * (D + gap)].view(V, D + gap)
+        ops().token_embedding_grad_(view(buffer)[:, :D], dy, t, scale=0.5)
+        total = want + view(was)[:, :D].double()
+        off = (count + 2) * 2.0 ** -24 * mass + 2.0 ** -24 * total.abs()
+        within(view(buffer)[:, :D], total, off + (total.abs() + off) * U[to] + TINY[to])
+        assert torch.equal(view(buffer)[:, D:], view(was)[:, D:]) and torch.equal(buffer[:first], was[:first]) and torch.equal(buffer[-9:], was[-9:])
+
+
 def test_grad_of_strided_broadcast_and_empty_rows():
     g = gen(3)
     t = tokens_of(g, 60, 11, "uniform", torch.int64).view(6, 10)
