@@ -476,6 +476,68 @@ def test_linear_of_shapes_and_strides():
     assert torch.equal(ops().group_row_linear(x, rows[7:20], 64), got[:, :, 7:20])
 
 
+def exact_linear(x, rows, D, group, bias=None):
+    """(products, bound) in 64 bits, from the codes themselves: a code of 0 leaves nothing but the group's bias.
+
+    An element stands for code * scale + bias, so its terms are |x| * (code |scale| + |bias|).  A term passes up to 32 matrix
+    instructions of a group (sums are cut off, 2^-23; 21 additions for the sum of the states), two FMAs a group, 16 shares and the
+    bias: 64 + 2 G roundings.  bf16 and fp32 states are held to 2^-23 of an element or 2^-39 of the state's largest one.
+    """
+    G = -(-D // group)
+    code = torch.stack([rows[:, :D // 2] & 15, rows[:, :D // 2] >> 4], 2).view(-1, D).double()
+    head = rows[:, D // 2:D // 2 + 4 * G].contiguous().view(torch.float16).double().view(-1, G, 2).repeat_interleave(group, 1)[:, :D]
+    number, term = code * head[..., 0] + head[..., 1], code * head[..., 0].abs() + head[..., 1].abs()
+    x64 = x.double()
+    held = torch.zeros_like(x64) if x.dtype == F16 else torch.maximum(2.0 ** -39 * x64.abs().amax(1, keepdim=True), (2.0 ** -23 if x.dtype == F32 else 0.0) * x64.abs())
+    want, mass = x64 @ number.t(), (x64.abs() + held) @ term.t()
+    off = held @ number.abs().t()
+    if bias is not None:
+        want, mass = want + bias.double(), mass + bias.double().abs()
+    return want, off + (64 + 2 * G) * 2.0 ** -23 * mass
+
+
+@pytest.mark.parametrize("m,D,group", [(1, 4096, 128), (3, 1000, 32), (8, 520, 64), (9, 2048, 256), (16, 264, 32), (17, 776, 128), (2, 16_400, 64)])
+@pytest.mark.parametrize("ti", [F32, F16, BF16])
+def test_linear_of_rows_without_a_span(m, D, group, ti):
+    """Groups whose elements are all alike, or nearly: the quantizer gives them scale 1 and codes 0, or a scale far below the bias."""
+    g = gen(D + m)
+    values = [0.0, -0.0, 1e-3, 1e-4, 1e-5, -1e-6, 1e-7, 0.37, -250.0, 3e-5, 6e-8]
+    x = torch.zeros(len(values) + 5, D, device="cuda")
+    for r, v in enumerate(values):
+        x[r] = v
+    few = x[len(values):]
+    few[0] = 1e-3 + 3e-7 * torch.rand(D, device="cuda", generator=g)          # a span of a few steps of the scale's smallest number
+    few[1] = randn(g, D, std=1e-3)
+    few[1, :group] = 0.0                                                      # a group of zeros among small ones
+    few[2] = randn(g, D, std=1e-6)
+    few[2, -8:] = 1e-6
+    few[3] = randn(g, D, std=1e-7)
+    few[4] = randn(g, D, std=0.05)
+    few[4, group:2 * group] = 2e-6
+    rows = ops().quantize_to_group_rows(x, group)
+    states = randn(g, m, D, dtype=ti)
+    for bias in (None, randn(g, x.shape[0], std=1e-6)):
+        got = ops().group_row_linear(states, rows, group, bias=bias, output_dtype=CODE[F32])
+        want, off = exact_linear(states, rows, D, group, bias)
+        within(got, want, off + (want.abs() + off) * U[F32] + TINY[F32])
+        if bias is None:
+            assert not bool(got[:, :2].any())                                 # zeros score zero
+
+
+@pytest.mark.parametrize("dtype,span", [(F32, 60), (BF16, 60), (F16, 20)])
+@pytest.mark.parametrize("m", [3, 20])
+def test_linear_of_states_with_elements_far_apart(dtype, span, m):
+    """Elements of one state over `span` powers of two, and rows from 1e-7 to 1e3."""
+    g = gen(span + m)
+    for D, group in ((512, 64), (1000, 32), (4096, 128)):
+        size = 10.0 ** torch.linspace(-7, 3, 48, device="cuda")
+        rows = ops().quantize_to_group_rows(randn(g, 48, D) * size[:, None], group)
+        x = (randn(g, m, D) * 2.0 ** (-span * torch.rand(m, D, device="cuda", generator=g))).to(dtype)
+        got = ops().group_row_linear(x, rows, group, output_dtype=CODE[F32])
+        want, off = exact_linear(x, rows, D, group)
+        within(got, want, off + (want.abs() + off) * U[F32] + TINY[F32])
+
+
 # ---- places behind 2^31 -------------------------------------------------------------------------------------------
 
 def test_rows_far_into_a_large_table():
