@@ -61,7 +61,8 @@ def _run(cmd, verbose):
 def build_cabi(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
-    headers = [os.path.join(CSRC, "tbe_common.cuh"), os.path.join(CSRC, "tbe_elements.cuh"), os.path.join(INCLUDE, "tbe_b200.h")]
+    headers = [os.path.join(CSRC, "tbe_common.cuh"), os.path.join(CSRC, "tbe_elements.cuh"), os.path.join(CSRC, "tbe_token_plan.h"),
+               os.path.join(INCLUDE, "tbe_b200.h")]
     nvcc = _nvcc()
     jobs, objs = [], []
     for src in CUDA_SOURCES:

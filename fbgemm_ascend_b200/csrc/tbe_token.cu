@@ -7,6 +7,7 @@
 // writing alone (a plain fill: 3.9), which is what the whole gradient of a large table mostly is.  No counterparts in the
 // reference.
 #include "tbe_elements.cuh"
+#include "tbe_token_plan.h"
 
 namespace tbe {
 namespace {
@@ -199,12 +200,7 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* warp_t
 // between the blocks, then every key straight to its place in whichever block's shared memory that is.  Bound by latency: the
 // barriers, and a warp's ranks one after the other.  13 us for 8192 tokens of 128000 (two digits), 17 us for 32768, 24 us for
 // 65537; clusters of eight blocks took 21 and 37 us, three kernels per digit through global memory 27 us for 8192.
-constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortBlocks = 16;                      // the largest cluster; a GPC of this GPU has as many multiprocessors
-constexpr int kOneBlockKeys = 2 * kSortThreads;      // so many are sorted by a block alone: 4096 take 16 us in one, 12 in a cluster
-constexpr int kMostItems = 16;
-constexpr int64_t kClusterKeys = int64_t(kSortBlocks) * kMostItems * kSortThreads;
 
 struct FillArgs {
     char* out;
@@ -413,7 +409,7 @@ sort_tokens_kernel(const SortInput in, int cluster, int items, int passes, int w
     }
 }
 
-// ---- more tokens than a cluster holds: per digit tile histograms, their running sums tile by tile, and the
+// ---- more tokens than a cluster holds, or no cluster to be had: per digit tile histograms, their running sums tile by tile, and the
 // scatter ----------------------------------------------------------------------------------
 constexpr int kWarps = kThreads / 32;
 constexpr int kSortItems = 16;
@@ -1026,7 +1022,7 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
     l.tile_rows = static_cast<int>(want < least ? least : want > 256 ? 256 : (want + kAhead - 1) / kAhead * kAhead);
     l.tiles = (n + l.tile_rows - 1) / l.tile_rows;
     l.padded_D = static_cast<int>((D + 7) / 8 * 8);
-    l.sort_tiles = n > kClusterKeys ? (n + kSortTile - 1) / kSortTile : 0;
+    l.sort_tiles = sort_form(n, false) == SortForm::kTiles ? (n + kSortTile - 1) / kSortTile : 0;      // whether the device needs it or not
     int64_t at = 0;
     l.sorted[0] = at; at += align16(8 * n);
     l.sorted[1] = at; at += l.sort_tiles ? align16(8 * n) : 0;
@@ -1075,18 +1071,19 @@ int launch_few(const SortInput& in, const TI* grad, int64_t grad_stride, int D, 
     return check_launch("grad_of_few_kernel");
 }
 
+// A launch of the sort by clusters of `cluster` blocks; `together` has to outlive it.
 template <int ITEMS>
-int launch_sort(const SortInput& in, int cluster, int items, int passes, int width, uint2* sorted, const FillArgs& fill, int unit, int64_t fillers, cudaStream_t s)
+int sort_config(int cluster, int64_t fillers, cudaStream_t s, cudaLaunchAttribute& together, cudaLaunchConfig_t& config)
 {
     auto* kernel = sort_tokens_kernel<ITEMS>;
     const int shared = static_cast<int>(sort_shared_bytes(ITEMS));
     static std::atomic<uint64_t> allowed{0};
     if (const int rc = allow_shared(reinterpret_cast<const void*>(kernel), shared, allowed)) return rc;
-    cudaLaunchAttribute together{};
+    together = {};
     together.id = cudaLaunchAttributeClusterDimension;
     together.val.clusterDim.x = cluster;
     together.val.clusterDim.y = together.val.clusterDim.z = 1;
-    cudaLaunchConfig_t config{};
+    config = {};
     config.gridDim = dim3(static_cast<unsigned>(cluster + fillers));
     config.blockDim = dim3(kSortThreads);
     config.dynamicSmemBytes = shared;
@@ -1101,6 +1098,37 @@ int launch_sort(const SortInput& in, int cluster, int items, int passes, int wid
             return fail(TBE_B200_ERR_CUDA, "sort_tokens_kernel: clusters of %d blocks are not allowed", kSortBlocks);
         if (dev < 64) large.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
     }
+    return TBE_B200_OK;
+}
+
+// Whether the current device can hold a cluster that sorts; the driver is asked once per device.
+bool sort_cluster_fits()
+{
+    static std::atomic<uint64_t> asked{0}, fits{0};
+    int dev = 0;
+    const bool kept = cudaGetDevice(&dev) == cudaSuccess && dev < 64;
+    const uint64_t bit = kept ? uint64_t(1) << dev : 0;
+    if (asked.load(std::memory_order_acquire) & bit) return fits.load(std::memory_order_relaxed) & bit;
+    cudaLaunchAttribute together;
+    cudaLaunchConfig_t config;
+    int clusters = 0;
+    if (sort_config<kMostItems>(kSortBlocks, 0, nullptr, together, config) != TBE_B200_OK ||
+        cudaOccupancyMaxActiveClusters(&clusters, sort_tokens_kernel<kMostItems>, &config) != cudaSuccess) {
+        cudaGetLastError();      // an answer, not a failure
+        clusters = 0;
+    }
+    if (clusters > 0) fits.fetch_or(bit, std::memory_order_relaxed);
+    asked.fetch_or(bit, std::memory_order_release);
+    return clusters > 0;
+}
+
+template <int ITEMS>
+int launch_sort(const SortInput& in, int cluster, int items, int passes, int width, uint2* sorted, const FillArgs& fill, int unit, int64_t fillers, cudaStream_t s)
+{
+    auto* kernel = sort_tokens_kernel<ITEMS>;
+    cudaLaunchAttribute together;
+    cudaLaunchConfig_t config;
+    if (const int rc = sort_config<ITEMS>(cluster, fillers, s, together, config)) return rc;
     const cudaError_t e = cudaLaunchKernelEx(&config, kernel, in, cluster, items, passes, width, sorted, fill, unit);
     if (e != cudaSuccess) return fail(TBE_B200_ERR_CUDA, "sort_tokens_kernel: %s", cudaGetErrorString(e));
     return check_launch("sort_tokens_kernel");
@@ -1108,26 +1136,23 @@ int launch_sort(const SortInput& in, int cluster, int items, int passes, int wid
 
 // Sorted (token, position) pairs into one of the two halves of the scratch, whose number is returned in `half`; the
 // gradient cleared on the way.
-int sort_and_clear(const SortInput& in, const GradPlan& l, char* scratch, const FillArgs& fill, int unit, int& half, cudaStream_t s)
+int sort_and_clear(const SortInput& in, SortForm form, const GradPlan& l, char* scratch, const FillArgs& fill, int unit, int& half, cudaStream_t s)
 {
     half = 0;
-    // blocks that clear: 64 KB each at least, one per multiprocessor at most
-    int64_t fillers = (fill.early * fill.row_bytes + 65535) / 65536;
-    const int sms = sm_count();
-    if ((in.n == 0 || in.n > kClusterKeys) && fillers) {
-        clear_rows_kernel<<<static_cast<unsigned>(fillers < 4 * sms ? fillers : 4 * sms), kThreads, 0, s>>>(fill, unit);
+    const int sms = sm_count(), cluster = form == SortForm::kBlock ? 1 : kSortBlocks;
+    const int64_t bytes = fill.early * fill.row_bytes;
+    const int64_t fillers = in.n == 0 || form == SortForm::kTiles ? 0 : clearing_blocks(bytes, sms, cluster);
+    if (bytes && !fillers) {
+        const int64_t blocks = (bytes + 65535) / 65536;
+        clear_rows_kernel<<<static_cast<unsigned>(blocks < 4 * sms ? blocks : 4 * sms), kThreads, 0, s>>>(fill, unit);
         if (const int rc = check_launch("clear_rows_kernel")) return rc;
     }
     if (in.n == 0) return TBE_B200_OK;
     int passes, width;
     digits_of(in.num_embeddings, passes, width);
     const int bins = 1 << width;
-    if (in.n <= kClusterKeys) {
-        const int cluster = in.n <= kOneBlockKeys ? 1 : kSortBlocks;
+    if (form != SortForm::kTiles) {
         const int items = static_cast<int>((in.n + cluster * kSortThreads - 1) / (cluster * kSortThreads));
-        fillers = fillers < sms - cluster ? fillers : sms - cluster;
-        fillers = (fillers + cluster - 1) / cluster * cluster;
-        if (cluster + fillers > sms) fillers -= cluster;
         uint2* sorted = reinterpret_cast<uint2*>(scratch + l.sorted[0]);
         if (items <= 2) return launch_sort<2>(in, cluster, items, passes, width, sorted, fill, unit, fillers, s);
         if (items <= 6) return launch_sort<6>(in, cluster, items, passes, width, sorted, fill, unit, fillers, s);
@@ -1249,7 +1274,8 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
     const SortInput in{tokens, token_bits == 64, n, num_embeddings, padding_idx};
     FillArgs fill{static_cast<char*>(grad_weight), accumulate ? 0 : num_embeddings, D * ob, grad_weight_stride * ob, 0, nullptr};
     fill.early = fill.rows;
-    if (!l.few && n > 0 && n <= kClusterKeys) {
+    const SortForm form = sort_form(n, n > kOneBlockKeys && !l.few && sort_cluster_fits());
+    if (!l.few && n > 0 && form != SortForm::kTiles) {
         // Writing alone runs at 4 TB/s, beside reads at most of what a copy writes: the sums' reads cost little then.  As many rows
         // are cleared beside the sort as that takes; where little is left, all.
         const int64_t beside_sort = ((int64_t(32) << 20) + n * 1100) / fill.row_bytes / 32 * 32;
@@ -1272,7 +1298,7 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
         });
     }
     int half;
-    if (const int rc = sort_and_clear(in, l, base, fill, ob, half, s)) return rc;
+    if (const int rc = sort_and_clear(in, form, l, base, fill, ob, half, s)) return rc;
     if (n == 0) return TBE_B200_OK;
     const SumArgs a{reinterpret_cast<const uint2*>(base + l.sorted[half]), n, static_cast<uint32_t>(num_embeddings), grad_stride, grad_weight_stride,
                     static_cast<int>(D), l.padded_D, l.tile_rows, l.slices, l.lanes_log2, l.tiles, scale, reinterpret_cast<float*>(base + l.parts)};

@@ -83,3 +83,38 @@ def test_no_cpu_path():
 def test_group_row_bytes():
     from fbgemm_ascend_b200.types import group_row_bytes
     assert [group_row_bytes(d, g) for d, g in ((8, 32), (32, 32), (64, 32), (4096, 128), (5000, 32), (1000, 256))] == [16, 32, 48, 2176, 3136, 528]
+
+
+_PLAN = """
+#include "tbe_token_plan.h"
+#include <stdio.h>
+int main() {
+    long long n, bytes; int fits, sms, cluster;
+    while (scanf("%lld %d %lld %d %d", &n, &fits, &bytes, &sms, &cluster) == 5)
+        printf("%d %lld\\n", static_cast<int>(tbe::sort_form(n, fits)), static_cast<long long>(tbe::clearing_blocks(bytes, sms, cluster)));
+}
+"""
+
+
+def test_plan_of_a_gradient_on_few_multiprocessors(tmp_path):
+    """Blocks that clear beside a sort come in whole clusters and never crowd one out; where none has room, the count says so."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fbgemm_ascend_b200", "csrc")
+    src, exe = tmp_path / "plan.cpp", tmp_path / "plan"
+    src.write_text(_PLAN)
+    subprocess.run(["g++", "-std=c++17", "-I" + csrc, str(src), "-o", str(exe)], check=True)
+
+    def ask(rows):
+        r = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, q)) for q in rows), capture_output=True, text=True, check=True)
+        return [tuple(map(int, line.split())) for line in r.stdout.splitlines()]
+
+    BLOCK, CLUSTER, TILES = 0, 1, 2
+    forms = [(1, 1, BLOCK), (2048, 0, BLOCK), (2049, 1, CLUSTER), (2049, 0, TILES), (262_144, 1, CLUSTER), (262_144, 0, TILES), (262_145, 1, TILES)]
+    assert [f for f, _ in ask([(n, fits, 0, 148, 16) for n, fits, _ in forms])] == [f for _, _, f in forms]
+    asked = [(5000, 1, b, sms, c) for b in (0, 1, 65_536, 65_537, 10 << 20, 1 << 40) for sms in (1, 2, 15, 16, 17, 31, 32, 33, 47, 64, 132, 147, 148, 160) for c in (1, 16)]
+    for (_, _, b, sms, c), (_, got) in zip(asked, ask(asked)):
+        assert got % c == 0 and got >= 0 and (got == 0 or got + c <= sms), (b, sms, c, got)
+        assert (got > 0) == (b > 0 and sms >= 2 * c), (b, sms, c, got)
+        assert got * 65_536 < b + c * 65_536, (b, sms, c, got)
+    assert [g for _, g in ask([(5000, 1, 1 << 30, sms, 16) for sms in (16, 17, 31, 32, 148)])] == [0, 0, 0, 16, 128]
