@@ -4,6 +4,7 @@
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -86,6 +87,25 @@ int64_t padding_row(std::optional<int64_t> padding_idx, int64_t rows, const char
     return *padding_idx < 0 ? *padding_idx + rows : *padding_idx;
 }
 
+// The operator of that name from the keys below autograd on, for tensors that are wrapped, or made of zeros alone, too.
+template <typename Signature, typename... Args>
+auto call_below(const c10::TypedOperatorHandle<Signature>& op, Args&&... args)
+{
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(std::forward<Args>(args)...);
+}
+
+template <typename Signature>
+c10::TypedOperatorHandle<Signature> operator_of(const char* name, Signature*)
+{
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+
+// Whether forward-mode differentiation goes through `t`.
+bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+
+bool differentiated(const Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || has_tangent(t); }
+
 // ---- lookup and gradient ----------------------------------------------------------------------------------------
 
 Tensor token_embedding_cuda(const Tensor& weight, const Tensor& tokens, double scale, std::optional<int64_t> padding_idx,
@@ -155,8 +175,6 @@ Tensor& token_embedding_grad_into_cuda(Tensor& grad_weight, const Tensor& grad, 
     check_tokens(tokens, grad_weight, op);
     TORCH_CHECK(grad.device() == grad_weight.device(), op, ": grad is on ", grad.device(), ", grad_weight on ", grad_weight.device());
     TORCH_CHECK(grad_weight.dim() == 2, op, ": grad_weight must be a matrix [num_embeddings, D]");
-    TORCH_CHECK(!(at::GradMode::is_enabled() && (grad_weight.requires_grad() || grad.requires_grad())), op,
-                ": adds in place without a graph; call it under torch.no_grad() or with detached tensors");
     TORCH_CHECK((grad_weight.size(1) <= 1 || grad_weight.stride(1) == 1) && row_stride(grad_weight) >= grad_weight.size(1), op,
                 ": rows of grad_weight must lie apart and their elements next to one another");
     at::assert_no_overlap(grad_weight, grad);
@@ -167,7 +185,17 @@ Tensor& token_embedding_grad_into_cuda(Tensor& grad_weight, const Tensor& grad, 
     return grad_weight;
 }
 
-// The lookup is linear in the table and its gradient linear in the rows: each is the other's backward, any number of times.
+Tensor& token_embedding_grad_into_autograd(Tensor& grad_weight, const Tensor& grad, const Tensor& tokens, double scale, std::optional<int64_t> padding_idx)
+{
+    TORCH_CHECK(!differentiated(grad_weight) && !differentiated(grad),
+                "token_embedding_grad_: adds in place without a graph; call it with detached tensors, or under torch.no_grad() without tangents");
+    static const auto op = operator_of("tbe_b200::token_embedding_grad_", token_embedding_grad_into_cuda);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(grad_weight, grad, tokens, scale, padding_idx);
+}
+
+// The lookup is linear in the table and its gradient linear in the rows: each is the other's backward, any number of times, and
+// a tangent goes through them as the values do.
 Tensor token_embedding_autograd(const Tensor& weight, const Tensor& tokens, double scale, std::optional<int64_t> padding_idx,
                                 std::optional<int64_t> output_dtype);
 Tensor token_embedding_grad_autograd(const Tensor& grad, const Tensor& tokens, int64_t num_embeddings, double scale,
@@ -242,10 +270,13 @@ void check_capture(const Tensor& t, const char* op)
 Tensor token_embedding_autograd(const Tensor& weight, const Tensor& tokens, double scale, std::optional<int64_t> padding_idx,
                                 std::optional<int64_t> output_dtype)
 {
-    if (!(at::GradMode::is_enabled() && weight.requires_grad())) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        return token_embedding_cuda(weight, tokens, scale, padding_idx, output_dtype);
+    static const auto op = operator_of("tbe_b200::token_embedding", token_embedding_cuda);
+    if (has_tangent(weight)) {
+        Tensor out = token_embedding_autograd(weight._fw_primal(0), tokens, scale, padding_idx, output_dtype);
+        out._set_fw_grad(op.call(weight._fw_grad(0), tokens, scale, padding_idx, type_number(out)), /*level=*/0, /*is_inplace_op=*/false);
+        return out;
     }
+    if (!(at::GradMode::is_enabled() && weight.requires_grad())) return call_below(op, weight, tokens, scale, padding_idx, output_dtype);
     check_capture(weight, "token_embedding");
     return TokenEmbeddingFunction::apply(weight, tokens, scale, padding_idx, output_dtype);
 }
@@ -253,10 +284,13 @@ Tensor token_embedding_autograd(const Tensor& weight, const Tensor& tokens, doub
 Tensor token_embedding_grad_autograd(const Tensor& grad, const Tensor& tokens, int64_t num_embeddings, double scale,
                                      std::optional<int64_t> padding_idx, std::optional<int64_t> output_dtype)
 {
-    if (!(at::GradMode::is_enabled() && grad.requires_grad())) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        return token_embedding_grad_cuda(grad, tokens, num_embeddings, scale, padding_idx, output_dtype);
+    static const auto op = operator_of("tbe_b200::token_embedding_grad", token_embedding_grad_cuda);
+    if (has_tangent(grad)) {
+        Tensor out = token_embedding_grad_autograd(grad._fw_primal(0), tokens, num_embeddings, scale, padding_idx, output_dtype);
+        out._set_fw_grad(op.call(grad._fw_grad(0), tokens, num_embeddings, scale, padding_idx, type_number(out)), /*level=*/0, /*is_inplace_op=*/false);
+        return out;
     }
+    if (!(at::GradMode::is_enabled() && grad.requires_grad())) return call_below(op, grad, tokens, num_embeddings, scale, padding_idx, output_dtype);
     check_capture(grad, "token_embedding_grad");
     return TokenEmbeddingGradFunction::apply(grad, tokens, num_embeddings, scale, padding_idx, output_dtype);
 }
@@ -283,7 +317,7 @@ Tensor checked_rows(const Tensor& rows, int64_t D, int64_t group_size, const cha
 
 void check_no_grad(const Tensor& t, const char* op, const char* name)
 {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), op, ": has no gradient; call it under torch.no_grad() or with a detached ", name);
+    TORCH_CHECK(!differentiated(t), op, ": has no gradient; call it with a detached ", name, ", or under torch.no_grad() without tangents");
 }
 
 Tensor quantize_to_group_rows(const Tensor& input, int64_t group_size)
@@ -293,7 +327,6 @@ Tensor quantize_to_group_rows(const Tensor& input, int64_t group_size)
     TORCH_CHECK(input.dim() == 2, op, ": input must be a matrix");
     const int it = element_type(input, op, "input");
     check_group(op, input.size(1), group_size);
-    check_no_grad(input, op, "input");
     const c10::cuda::CUDAGuard guard(input.device());
     const Tensor x = as_matrix(input);
     const int64_t D = x.size(1), bytes = row_bytes_of(D, group_size);
@@ -301,6 +334,13 @@ Tensor quantize_to_group_rows(const Tensor& input, int64_t group_size)
     check_status(tbe_b200_quantize_to_group_rows(x.data_ptr(), it, row_stride(x), x.size(0), D, static_cast<int32_t>(group_size), bytes,
                                                  out.data_ptr<uint8_t>(), current_stream()), op);
     return out;
+}
+
+Tensor quantize_to_group_rows_autograd(const Tensor& input, int64_t group_size)
+{
+    check_no_grad(input, "quantize_to_group_rows", "input");
+    static const auto op = operator_of("tbe_b200::quantize_to_group_rows", quantize_to_group_rows);
+    return call_below(op, input, group_size);
 }
 
 Tensor read_group_rows(const Tensor& rows, const Tensor* tokens, int64_t D, int64_t group_size, double scale, int64_t output_dtype, const char* op)
@@ -340,7 +380,6 @@ Tensor group_row_linear(const Tensor& input, const Tensor& rows, int64_t group_s
     const int it = element_type(input, op, "input");
     const Tensor r = checked_rows(rows, D, group_size, op);
     TORCH_CHECK(rows.device() == input.device(), op, ": input is on ", input.device(), ", the rows on ", rows.device());
-    check_no_grad(input, op, "input");
     const int64_t N = r.size(0), out_type = output_dtype.value_or(it);
     const at::ScalarType type = scalar_type_of(out_type, op);
     const c10::cuda::CUDAGuard guard(input.device());
@@ -349,7 +388,6 @@ Tensor group_row_linear(const Tensor& input, const Tensor& rows, int64_t group_s
         check_cuda(*bias, op, "bias");
         element_type(*bias, op, "bias");
         TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N && bias->device() == input.device(), op, ": bias must have one entry per row, on the rows' device");
-        check_no_grad(*bias, op, "bias");
         b = bias->contiguous();
     }
     Tensor x = as_matrix(input.reshape({D ? input.numel() / D : 0, D}));
@@ -367,6 +405,15 @@ Tensor group_row_linear(const Tensor& input, const Tensor& rows, int64_t group_s
                                            b.defined() ? b.data_ptr() : nullptr, b.defined() ? element_type(b, op, "bias") : 0, out.data_ptr(),
                                            static_cast<int32_t>(out_type), N, nullptr, need > 0 ? scratch.data_ptr() : nullptr, need, current_stream()), op);
     return out;
+}
+
+Tensor group_row_linear_autograd(const Tensor& input, const Tensor& rows, int64_t group_size, const std::optional<Tensor>& bias,
+                                 std::optional<int64_t> output_dtype)
+{
+    check_no_grad(input, "group_row_linear", "input");
+    if (bias && bias->defined()) check_no_grad(*bias, "group_row_linear", "bias");
+    static const auto op = operator_of("tbe_b200::group_row_linear", group_row_linear);
+    return call_below(op, input, rows, group_size, bias, output_dtype);
 }
 
 }  // namespace
@@ -398,4 +445,7 @@ TORCH_LIBRARY_IMPL(tbe_b200, AutogradCUDA, m)
 {
     m.impl("token_embedding", TORCH_FN(token_embedding_autograd));
     m.impl("token_embedding_grad", TORCH_FN(token_embedding_grad_autograd));
+    m.impl("token_embedding_grad_", TORCH_FN(token_embedding_grad_into_autograd));
+    m.impl("quantize_to_group_rows", TORCH_FN(quantize_to_group_rows_autograd));
+    m.impl("group_row_linear", TORCH_FN(group_row_linear_autograd));
 }

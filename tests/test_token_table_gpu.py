@@ -333,6 +333,62 @@ def test_gradient_against_differences_and_of_the_gradient():
     within(second, want, (count + 40) * 2.0 ** -24 * (mass + 1e-3))
 
 
+@pytest.mark.parametrize("ti,to", [(F32, F32), (BF16, F32), (F16, BF16)])
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode(ti, to, needs_grad):
+    """The lookup and its gradient are linear: a tangent goes through them as the values do."""
+    import torch.autograd.forward_ad as fwd
+    g = gen(14)
+    V, D = 40, 24
+    t = tokens_of(g, 3 * 25, V, "wild", torch.int64).view(3, 25)
+    w, dw, dy, ddy = randn(g, V, D, dtype=ti), randn(g, V, D, dtype=ti), randn(g, 3, 25, D, dtype=ti), randn(g, 3, 25, D, dtype=ti)
+    look = lambda w: ops().token_embedding(w, t, scale=0.5, padding_idx=3, output_dtype=CODE[to])
+    back = lambda dy: ops().token_embedding_grad(dy, t, V, scale=0.5, padding_idx=3, output_dtype=CODE[to])
+    for f, x, dx in ((look, w, dw), (back, dy, ddy)):
+        value, tangent = f(x), f(dx)
+        with fwd.dual_level():
+            got = fwd.unpack_dual(f(fwd.make_dual(x.clone().requires_grad_(needs_grad), dx)))
+            assert torch.equal(got.primal, value) and got.tangent is not None and torch.equal(got.tangent, tangent)
+            assert got.primal.requires_grad == needs_grad
+            assert fwd.unpack_dual(f(x)).tangent is None
+        value2, tangent2 = torch.func.jvp(f, (x,), (dx,))
+        assert torch.equal(value2, value) and torch.equal(tangent2, tangent)
+
+
+def test_forward_mode_over_reverse():
+    """The derivative of a gradient along a direction, which takes both."""
+    import torch.autograd.forward_ad as fwd
+    g = gen(15)
+    w, e, t = randn(g, 20, 12), randn(g, 20, 12), tokens_of(g, 50, 20, "uniform", torch.int64)
+    with fwd.dual_level():
+        dual = fwd.make_dual(w.clone().requires_grad_(), e)
+        (grad,) = torch.autograd.grad((ops().token_embedding(dual, t, scale=0.5) ** 2).sum(), dual, create_graph=True)
+        got = fwd.unpack_dual(grad).tangent
+    want, mass, count = grad64(2 * lookup64(e, t, 0.5).float(), t, 20, 0.5)
+    within(got, want, (count + 8) * 2.0 ** -24 * mass + 2.0 ** -140)
+
+
+def test_forward_mode_is_refused_where_there_is_no_derivative():
+    import torch.autograd.forward_ad as fwd
+    w, t, dy = torch.ones(10, 16, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda"), torch.ones(4, 16, device="cuda")
+    rows, b = ops().quantize_to_group_rows(w, 32), torch.ones(10, device="cuda")
+    calls = [(lambda x: ops().quantize_to_group_rows(x, 32), w), (lambda x: ops().group_row_linear(x, rows, 32), w),
+             (lambda x: ops().group_row_linear(w, rows, 32, bias=x), b), (lambda x: ops().token_embedding_grad_(w.clone(), x, t), dy),
+             (lambda x: ops().token_embedding_grad_(x, dy, t), w)]
+    for f, x in calls:
+        with fwd.dual_level():
+            dual = fwd.make_dual(x.clone(), torch.ones_like(x))
+            with pytest.raises(RuntimeError, match="gradient|graph"):
+                f(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="gradient|graph"):
+                f(dual)
+            f(dual.detach())
+        with pytest.raises(RuntimeError, match="gradient|graph"):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))
+        with pytest.raises(RuntimeError, match="gradient|graph"):
+            torch.func.grad(lambda x: f(x).float().sum())(x)
+
+
 # ---- 4-bit rows with group scales --------------------------------------------------------------------------------
 
 def rows_by_oracle(x, group):
