@@ -58,6 +58,8 @@ EXPORTS = {
     "tbe_b200_group_row_linear_scratch_bytes": (_i64, [_i64, _i64, _i32, _i32]),
     "tbe_b200_group_row_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _i32, _i64, _vp, _vp, _i64,
                                          _vp]),
+    "tbe_b200_group_row_linear_bounded": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _i32, _i64, _vp, _vp,
+                                                 _i64, _i64, _vp]),
     "tbe_b200_last_error": (C.c_char_p, []),
     "tbe_b200_version": (_i32, []),
 }

@@ -312,8 +312,8 @@ int tbe_b200_group_row_embedding(const uint8_t* rows, int64_t num_embeddings, in
  * m vectors of D elements and num_rows rows; fp32 accumulation, one rounding.  A vector with a non-finite element gets no
  * finite result (infinities or NaN, not told apart).  bias (num_rows entries) may be NULL.
  * `input` is 16-byte aligned and its rows 16-byte apart in whole pieces; D is at most 2^20.  Made for m up to 16 (a decoding
- * step's states): every 16 vectors read the rows once more.  Waits inside the kernel are bounded; one that ran out would set
- * bit 16 of *error_flag (if given).  scratch: tbe_b200_group_row_linear_scratch_bytes(m, D, group_size, input_dtype) bytes of
+ * step's states): every 16 vectors read the rows once more.  Waits inside the kernel are bounded: outputs whose rows did not
+ * arrive are NaN, and bit 16 of *error_flag (if given) is set.  scratch: tbe_b200_group_row_linear_scratch_bytes(m, D, group_size, input_dtype) bytes of
  * device memory, 16-byte aligned, overwritten by the call (0 for few and short vectors: scratch may be NULL then); two calls
  * that may overlap need separate scratch.  The function returns -1 for sizes that the call refuses. */
 int64_t tbe_b200_group_row_linear_scratch_bytes(int64_t m, int64_t D, int32_t group_size, int32_t input_dtype);
@@ -321,6 +321,12 @@ int tbe_b200_group_row_linear(const void* input, int32_t input_dtype, int64_t in
                               int64_t num_rows, int64_t row_bytes, int64_t D, int32_t group_size, const void* bias,
                               int32_t bias_dtype, void* output, int32_t output_dtype, int64_t output_stride,
                               int32_t* error_flag, void* scratch, int64_t scratch_bytes, tbe_b200_stream_t stream);
+/* The same with the limit of each wait, in polls (the call above: 2^20).  0 gives every wait up, so that all outputs are NaN. */
+int tbe_b200_group_row_linear_bounded(const void* input, int32_t input_dtype, int64_t input_stride, int64_t m, const uint8_t* rows,
+                                      int64_t num_rows, int64_t row_bytes, int64_t D, int32_t group_size, const void* bias,
+                                      int32_t bias_dtype, void* output, int32_t output_dtype, int64_t output_stride,
+                                      int32_t* error_flag, void* scratch, int64_t scratch_bytes, int64_t max_polls,
+                                      tbe_b200_stream_t stream);
 
 /* Message of the last failure on the calling thread ("" if none).  Host pointer,
  * valid until the next failing call on the same thread. */

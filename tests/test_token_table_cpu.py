@@ -66,6 +66,18 @@ def _refusals():
     assert lin(m=17, scratch=None) == -1 and lin(m=17, scratch=8) == -1 and lin(m=17, bytes=need(17, 8, 32, FP32) - 1) == -1 and "scratch" in cabi.last_error()
 
 
+def test_c_entry_point_of_bounded_products_refuses():
+    ThreadPoolExecutor(1).submit(_bounded_refusals).result()
+
+
+def _bounded_refusals():
+    from fbgemm_ascend_b200 import cabi
+    lib = cabi.lib()
+    call = lambda m, polls: lib.tbe_b200_group_row_linear_bounded(16, 0, 8, m, 16, 4, 16, 8, 32, None, 0, 16, 0, 4, None, 16, 1 << 30, polls, None)
+    assert call(1, -1) == -1 and "max_polls" in cabi.last_error()
+    assert call(0, 0) == 0 and call(0, 1 << 40) == 0
+
+
 def test_no_cpu_path():
     import fbgemm_ascend_b200 as fa
     ops = torch.ops.tbe_b200

@@ -594,6 +594,32 @@ def test_linear_of_states_with_elements_far_apart(dtype, span, m):
         within(got, want, off + (want.abs() + off) * U[F32] + TINY[F32])
 
 
+@pytest.mark.parametrize("m,N,D,group,ti", [(1, 40, 512, 128, BF16), (16, 5000, 1000, 32, F32), (8, 70_000, 264, 64, F16), (17, 300, 776, 256, BF16), (3, 20_000, 16_400, 128, F32)])
+def test_linear_whose_waits_run_out(m, N, D, group, ti):
+    """Rows that do not arrive in time leave NaN and a word for the host, and the next call is as ever."""
+    from fbgemm_ascend_b200 import cabi
+    lib, g = cabi.lib(), gen(m + D)
+    rows, x = ops().quantize_to_group_rows(randn(g, N, D, std=0.05), group), randn(g, m, D, dtype=ti)
+    need = lib.tbe_b200_group_row_linear_scratch_bytes(m, D, group, CODE[ti])
+    scratch = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+
+    def call(polls, to, flag):
+        out = torch.zeros(m, N, device="cuda", dtype=to)
+        cabi.check(lib.tbe_b200_group_row_linear_bounded(x.data_ptr(), CODE[ti], D, m, rows.data_ptr(), N, rows.shape[1], D, group, None, 0, out.data_ptr(), CODE[to], N,
+                                                         None if flag is None else flag.data_ptr(), scratch.data_ptr(), need, polls,
+                                                         torch.cuda.current_stream().cuda_stream), "linear")
+        return out
+
+    want = ops().group_row_linear(x, rows, group, output_dtype=CODE[F32])
+    for to in (F32, BF16):
+        flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+        assert bool(call(0, to, flag).isnan().all()) and int(flag) == 16
+        assert bool(call(0, to, None).isnan().all())
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert torch.equal(call(1 << 20, F32, flag), want) and int(flag) == 0
+    assert torch.equal(ops().group_row_linear(x, rows, group, output_dtype=CODE[F32]), want)
+
+
 # ---- places behind 2^31 -------------------------------------------------------------------------------------------
 
 def test_rows_far_into_a_large_table():
