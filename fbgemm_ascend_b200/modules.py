@@ -197,6 +197,7 @@ class GroupRowTable:
         self.num_embeddings, self.embedding_dim, self.group_size = int(num_embeddings), int(embedding_dim), int(group_size)
         self.output_dtype = int(output_dtype)
         self.rows = torch.zeros(self.num_embeddings, group_row_bytes(self.embedding_dim, self.group_size), dtype=torch.uint8, device=self.device)
+        self.device = self.rows.device      # with its number: another device may be current later
 
     def assign_rows_from_float(self, x: torch.Tensor, row_start: int = 0) -> None:
         """Quantize fp32, fp16 or bf16 ``x`` [n, D] into rows ``row_start .. row_start + n``."""

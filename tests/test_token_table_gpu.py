@@ -807,3 +807,12 @@ def test_refusals():
                  lambda: fa.GroupRowTable(4, 8, 48), lambda: fa.GroupRowTable(4, 12)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_group_row_table_keeps_to_the_device_of_its_rows():
+    """A device without a number is the one that is current when the table is made, whichever is later."""
+    import fbgemm_ascend_b200 as fa
+    table = fa.GroupRowTable(10, 16, 64, device="cuda")
+    assert table.device == table.rows.device and table.device.index is not None
+    table.assign_rows_from_float(torch.ones(10, 16))             # of another device
+    assert torch.equal(table.to_float(), torch.ones(10, 16, device="cuda"))
