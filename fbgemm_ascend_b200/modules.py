@@ -201,10 +201,12 @@ class GroupRowTable:
 
     def assign_rows_from_float(self, x: torch.Tensor, row_start: int = 0) -> None:
         """Quantize fp32, fp16 or bf16 ``x`` [n, D] into rows ``row_start .. row_start + n``."""
-        n = x.shape[0]
+        n = x.shape[0] if x.dim() else 0
         if x.dim() != 2 or x.shape[1] != self.embedding_dim or row_start < 0 or row_start + n > self.num_embeddings:
             raise ValueError(f"rows {row_start} .. {row_start + n} of {tuple(x.shape)} do not fit a table of "
                              f"[{self.num_embeddings}, {self.embedding_dim}]")
+        if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise ValueError(f"rows must be float32, float16 or bfloat16, got {x.dtype}")
         with torch.cuda.device(self.device):
             cabi.quantize_to_group_rows(x.detach().to(self.device).contiguous(), self.group_size, self.rows[row_start:row_start + n])
 

@@ -816,3 +816,13 @@ def test_group_row_table_keeps_to_the_device_of_its_rows():
     assert table.device == table.rows.device and table.device.index is not None
     table.assign_rows_from_float(torch.ones(10, 16))             # of another device
     assert torch.equal(table.to_float(), torch.ones(10, 16, device="cuda"))
+
+
+def test_group_row_table_names_what_it_cannot_take():
+    import fbgemm_ascend_b200 as fa
+    table = fa.GroupRowTable(10, 16, 64)
+    for bad, text in ((torch.zeros(3, 16, dtype=torch.float64, device="cuda"), "float32, float16 or bfloat16"), (torch.zeros(3, 16, dtype=torch.int64), "float32, float16 or bfloat16"),
+                      (torch.zeros((), device="cuda"), "do not fit"), (torch.zeros(16, device="cuda"), "do not fit"), (torch.zeros(1, 3, 16, device="cuda"), "do not fit")):
+        with pytest.raises(ValueError, match=text):
+            table.assign_rows_from_float(bad)
+    assert not bool(table.rows.any())
