@@ -148,6 +148,31 @@ __device__ __forceinline__ void store_piece(T* p, const float (&v)[VEC])
     }
 }
 
+// (v & mask) | bits in one instruction; written out with two constants it becomes two.
+__device__ __forceinline__ uint32_t mask_or(uint32_t v, uint32_t mask, uint32_t bits)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
+    return r;
+}
+
+// One word of 4-bit codes (elements 0 .. 7, low nibble first) as four pairs (0,4) (1,5) (2,6) (3,7) of fp16 numbers.  A nibble
+// or'ed into the low bits of 1024 (16 steps apart for the upper nibble of a byte) makes that number plus the code; what is
+// taken off again leaves it exact.
+__device__ __forceinline__ void decode_codes(uint32_t w, uint32_t (&p)[4])
+{
+    const uint32_t v = w >> 8;
+    const uint32_t in[4] = {mask_or(w, 0x000f000fu, 0x64006400u), mask_or(w, 0x00f000f0u, 0x64006400u), mask_or(v, 0x000f000fu, 0x64006400u),
+                            mask_or(v, 0x00f000f0u, 0x64006400u)};
+    const __half2 even = __float2half2_rn(1024.0f), sixteenth = __float2half2_rn(0.0625f), odd = __float2half2_rn(-64.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = *reinterpret_cast<const __half2*>(&in[i]);
+        const __half2 r = (i & 1) ? __hfma2(h, sixteenth, odd) : __hsub2(h, even);
+        p[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
 inline int element_bytes(int dtype) { return dtype == TBE_B200_FP32 ? 4 : (dtype == TBE_B200_FP16 || dtype == TBE_B200_BF16) ? 2 : 0; }
 
 // Whether rows that start at p, stride elements apart, can be moved in pieces of vec elements.

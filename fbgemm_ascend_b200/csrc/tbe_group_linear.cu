@@ -54,31 +54,6 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// (v & mask) | bits in one instruction; written out with two constants it becomes two.
-__device__ __forceinline__ uint32_t mask_or(uint32_t v, uint32_t mask, uint32_t bits)
-{
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
-    return r;
-}
-
-// One word of codes (elements 0 .. 7, low nibble first) as four pairs (0,4) (1,5) (2,6) (3,7) of codes in fp16.  A nibble
-// or'ed into the low bits of 1024 (16 steps apart for the upper nibble of a byte) makes that number plus the code; what is
-// taken off again leaves it exact.
-__device__ __forceinline__ void decode(uint32_t w, uint32_t (&p)[4])
-{
-    const uint32_t v = w >> 8;
-    const uint32_t in[4] = {mask_or(w, 0x000f000fu, 0x64006400u), mask_or(w, 0x00f000f0u, 0x64006400u), mask_or(v, 0x000f000fu, 0x64006400u),
-                            mask_or(v, 0x00f000f0u, 0x64006400u)};
-    const __half2 even = __float2half2_rn(1024.0f), sixteenth = __float2half2_rn(0.0625f), odd = __float2half2_rn(-64.0f);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 h = *reinterpret_cast<const __half2*>(&in[i]);
-        const __half2 r = (i & 1) ? __hfma2(h, sixteenth, odd) : __hsub2(h, even);
-        p[i] = *reinterpret_cast<const uint32_t*>(&r);
-    }
-}
-
 // c = a * b, or c += a * b.
 template <bool FIRST>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -493,7 +468,7 @@ group_row_linear_kernel(const LinearArgs a, const __grid_constant__ CUtensorMap 
 #pragma unroll
                     for (int i = 0; i < RT; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) decode(s == 0 ? w[i][j].x : s == 1 ? w[i][j].y : s == 2 ? w[i][j].z : w[i][j].w, p[i][j]);
+                        for (int j = 0; j < 2; ++j) decode_codes(s == 0 ? w[i][j].x : s == 1 ? w[i][j].y : s == 2 ? w[i][j].z : w[i][j].w, p[i][j]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -237,17 +237,13 @@ quantize_group_rows_kernel(const T* __restrict__ in, int64_t in_stride, int64_t 
 // 16384 rows of 4096 in groups of 128 as bf16: 24 us, 6.0 TB/s of what has to be moved.
 constexpr int kLookupLane = 8, kLookupAtOnce = 4;
 
-// Eight codes as numbers: a nibble or'ed into the low bits of 1024 in fp16 (16 steps apart for the upper nibble of a byte) is that
-// plus the code, and taking it off leaves the code exactly.
 __device__ __forceinline__ void codes_of(uint32_t w, float (&q)[8])
 {
-    const __half2 even = __float2half2_rn(1024.0f), sixteenth = __float2half2_rn(0.0625f), odd = __float2half2_rn(-64.0f);
+    uint32_t p[4];
+    decode_codes(w, p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        uint32_t bits;
-        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(bits) : "r"(i < 2 ? w : w >> 8), "r"((i & 1) ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
-        const __half2 h = *reinterpret_cast<const __half2*>(&bits);
-        const float2 f = __half22float2((i & 1) ? __hfma2(h, sixteenth, odd) : __hsub2(h, even));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
         q[i] = f.x;
         q[i + 4] = f.y;
     }
