@@ -69,8 +69,9 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 // ---- the states, in the order that the matrix instructions take them --------------------------------------------
 //
 // A state's elements become fp16: as they are, or times the power of two that brings the state's largest into 2^14 .. 2^15
-// (bf16 keeps its 8 bits then, but for elements below 2^-28 of the largest, which are off by 2^-40 of it at most); fp32 in
-// two pieces, 22 bits and a sign, off by 2^-23 at most.  The sums are scaled back.
+// (bf16 keeps its 8 bits then down to 2^-31 of the largest; elements below that are off by 2^-39 of the largest at most); fp32
+// in two pieces, off by 2^-23 of the element down to 2^-16 of the largest, below that by 2^-39 of the largest, since the second
+// piece is subnormal there.  (A state below 2^-112 is brought up by 2^126, and off by 2^-151.)  The sums are scaled back.
 //
 // For a unit of 128 elements: four steps, in each 64 bytes per state and piece, 16 to each of four lanes; then the sums of the
 // states over every group of the unit.  A block that arranges the states itself (LOCAL) keeps only those that there are; else
@@ -656,7 +657,10 @@ int launch_linear(const LinearArgs& a, cudaStream_t s)
 {
     constexpr bool LOCAL = !std::is_void<T>::value;
     const int NT = states_per_block(a.m), steps = steps_of(a.group_log2);
-    // 32 rows to a warp use every state twice, which makes a stage about a tenth shorter; 16 fit more numbers of rows.
+    // 32 rows to a warp use every state twice, which makes a stage about a tenth shorter; 16 fit more numbers of rows.  Measured over
+    // 1024 to 131072 rows of 1024 to 8192 by 1, 8 and 16 states (us, 32 / 16): at equal cost 61.5 / 65.5 (8 states by 131072 x 4096) and
+    // 28.2 / 30.6 (1 by 28672 x 5000), seldom behind; at a cost 1.13 times as high 10.7 / 10.0 (1 by 5000 x 8192) and 38.4 / 34.8 (16 by
+    // 20000 x 8192).
     const Shape wide = shape_for(a, 2, NT, P, steps, LOCAL), narrow = shape_for(a, 1, NT, P, steps, LOCAL);
     const bool two = NT == 2, many = 10 * wide.cost <= 11 * narrow.cost;
     auto by_group = [&](auto rt, auto nt) {

@@ -274,7 +274,9 @@ int tbe_b200_wait_flags(const int64_t* flags, int32_t world, int64_t value, int6
  * outside [0, num_embeddings) names no row: it looks up zeros and takes part in no gradient; entries other than -1 that
  * do so set bit 4 of *error_flag (if given), like an index past its table's end in the lookup above. */
 
-/* output[i, :] = scale * weight[tokens[i], :], the product rounded once to the output's type. */
+/* output[i, :] = scale * weight[tokens[i], :], the product in fp32, rounded to the output's type.
+ * Rows that do not begin at 16-byte borders are read in the aligned 16-byte words that hold them, here and in the gradient: up
+ * to 15 bytes in front of a row and behind it, in the same words as its ends, are read and not used. */
 int tbe_b200_token_embedding(const void* weight, int32_t weight_dtype, int64_t num_embeddings, int64_t D, int64_t weight_stride,
                              const void* tokens, int32_t token_bits, int64_t n, float scale, void* output, int32_t output_dtype,
                              int64_t output_stride, int32_t* error_flag, tbe_b200_stream_t stream);
@@ -282,7 +284,7 @@ int tbe_b200_token_embedding(const void* weight, int32_t weight_dtype, int64_t n
 /* The gradient of tbe_b200_token_embedding by its table:
  *   grad_weight[v, :] = [grad_weight[v, :] if accumulate] + scale * sum of grad[i, :] over the i with tokens[i] == v
  * Tokens are sorted first, so every row's sum has one fixed order: a call gives the same bits every time.  Sums are held
- * in fp32 and rounded once.  accumulate 0: every row is written, zeros where no token names it; 1: only rows that
+ * in fp32, scaled there and rounded to the buffer's type.  accumulate 0: every row is written, zeros where no token names it; 1: only rows that
  * tokens name are read and written.  Tokens equal to padding_idx (-1: none) take part in no gradient.
  * scratch: tbe_b200_token_embedding_grad_scratch_bytes(n, num_embeddings, D) bytes of device memory, 16-byte aligned,
  * overwritten by the call (0 for few tokens: scratch may be NULL then); two calls that may overlap need separate scratch.
@@ -302,14 +304,17 @@ int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtype, int64_t 
 int tbe_b200_quantize_to_group_rows(const void* input, int32_t input_dtype, int64_t input_stride, int64_t nrows, int64_t D,
                                     int32_t group_size, int64_t row_bytes, uint8_t* rows, tbe_b200_stream_t stream);
 
-/* output[i, :] = scale * the numbers of row tokens[i], rounded once (num_embeddings rows).  tokens NULL: row i itself
+/* output[i, :] = scale * the numbers of row tokens[i] (num_embeddings rows): code * scale + bias rounded to fp32, the product with
+ * a scale other than 1 again, the result to the output's type.  tokens NULL: row i itself
  * (n <= num_embeddings), which reads a table back. */
 int tbe_b200_group_row_embedding(const uint8_t* rows, int64_t num_embeddings, int64_t row_bytes, int64_t D, int32_t group_size,
                                  const void* tokens, int32_t token_bits, int64_t n, float scale, void* output, int32_t output_dtype,
                                  int64_t output_stride, int32_t* error_flag, tbe_b200_stream_t stream);
 
 /* Products of a few vectors with every row: output[i, r] = sum over c of input[i, c] * (number c of row r) + bias[r], for
- * m vectors of D elements and num_rows rows; fp32 accumulation, one rounding.  A vector with a non-finite element gets no
+ * m vectors of D elements and num_rows rows; fp32 accumulation, one rounding to the output's type.  fp16 vectors are taken as they
+ * are, bf16 and fp32 elements are held to 2^-23 of themselves or 2^-39 of their vector's largest element, whichever is more (bf16
+ * exactly down to 2^-31 of the largest).  A vector with a non-finite element gets no
  * finite result (infinities or NaN, not told apart).  bias (num_rows entries) may be NULL.
  * `input` is 16-byte aligned and its rows 16-byte apart in whole pieces; D is at most 2^20.  Made for m up to 16 (a decoding
  * step's states): every 16 vectors read the rows once more.  Waits inside the kernel are bounded: outputs whose rows did not
