@@ -1004,6 +1004,7 @@ struct GradPlan {
     bool few;      // one launch, no scratch
 };
 
+// Of a whole GPU, whatever part of it there is: how sums are cut, and so their bits and the scratch, is the same on any.
 constexpr int64_t kResidentWarps = 148 * 32;
 
 bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
@@ -1018,7 +1019,11 @@ bool plan_grad(int64_t n, int64_t num_embeddings, int64_t D, GradPlan& l)
     l.slices = static_cast<int>((D + (kColumns << l.lanes_log2) - 1) / (kColumns << l.lanes_log2));
     const int64_t groups = kResidentWarps << (5 - l.lanes_log2), want = (n * l.slices + groups - 1) / groups;
     // Short tiles for few tokens, whose rows come one after the other; long tokens leave a piece per tile: not too many of them.
-    const int64_t least = n <= 8192 ? 8 : n <= 49152 ? 16 : D <= 256 ? 64 : 32;
+    // Where rows are wide `want` decides.  Measured over tables of 32000 bf16 rows (us a gradient, with tiles of 8 / 16 / 32 / 64):
+    // 2500 tokens of 128 17.5 / 17.9 / 20.7 / 27.2, 12000 of 256 with a hot token 26.2 / 24.3 / 23.5 / 30.7, 32768 of 128 29.5 / 27.5 /
+    // 30.5 / 35.6, 49152 of 128 37.3 / 32.8 / 32.9 / 39.0, 65537 of 128 47.8 / 42.1 / 41.5 / 46.1, 131072 of 256 with a hot token
+    // 85.5 / 85.5 / 90.2 / 82.7, 300000 of 64 92.6 / 92.6 / 77.2 / 76.8.
+    const int64_t least = n <= 8192 ? 8 : n <= 49152 ? 16 : n < 131072 ? 32 : 64;
     l.tile_rows = static_cast<int>(want < least ? least : want > 256 ? 256 : (want + kAhead - 1) / kAhead * kAhead);
     l.tiles = (n + l.tile_rows - 1) / l.tile_rows;
     l.padded_D = static_cast<int>((D + 7) / 8 * 8);
@@ -1277,7 +1282,9 @@ extern "C" int tbe_b200_token_embedding_grad(const void* grad, int32_t grad_dtyp
     const SortForm form = sort_form(n, n > kOneBlockKeys && !l.few && sort_cluster_fits());
     if (!l.few && n > 0 && form != SortForm::kTiles) {
         // Writing alone runs at 4 TB/s, beside reads at most of what a copy writes: the sums' reads cost little then.  As many rows
-        // are cleared beside the sort as that takes; where little is left, all.
+        // are cleared beside the sort as that takes; where little is left, all.  Measured (us, 16384 tokens into 131072 x 2048 bf16 /
+        // 131072 tokens into 500000 x 512): this rule 158 / 173, without its 32 MB 162 / 184, with 128 MB 162 / 168, with 32 MB however
+        // many tokens there are 155 / 204, everything beside the sort 172 / 184.
         const int64_t beside_sort = ((int64_t(32) << 20) + n * 1100) / fill.row_bytes / 32 * 32;
         if (beside_sort + beside_sort / 4 < fill.rows) {
             fill.early = beside_sort;
