@@ -9,17 +9,20 @@
 //
 // A decoding step's states times a weight matrix or a token table.  No counterpart in the reference.
 //
-// Bounded by the rows' bytes where the rows are wide in groups of 128 and 256 and there are up to eight states, by the issue of
-// instructions elsewhere.  Each row is read once for up to 16 states, by copies into shared memory that a warp of its own issues
-// some stages ahead, and only the codes (exact in fp16) meet the tensor core: what a group's scale and bias multiply are sums
-// over the group.  The matrix instruction is the warp's (16 rows by 8 states by 16 elements, one per 8 clocks and SM quarter):
-// operands must come out of registers, where codes become numbers, and at 16 states or fewer its rate is no limit (24 % of it is
-// used at eight).  What the codes cost is decoding: four masks and four subtractions for eight of them, and the loads; 274 warp
-// instructions per 4096 codes in all.
+// The rows' bytes are the floor.  Each row is read once for up to 16 states, by copies into shared memory that a warp of its own
+// issues some stages ahead, and only the codes (exact in fp16) meet the tensor core: what a group's scale and bias multiply are
+// sums over the group.  The matrix instruction is the warp's (16 rows by 8 states by 16 elements, one per 8 clocks and SM quarter):
+// operands must come out of registers, where codes become numbers, and at 16 states or fewer its rate is no limit (26 % of it is
+// used at eight).  What the codes cost is decoding: four masks and four subtractions for eight of them, and the loads; 315 warp
+// instructions per 4096 codes in all, at eight states by groups of 128.
+//
+// Large tables: no unit is saturated (8 states by 131072 x 4096: 64 % of the issue slots, 54 % of the DRAM peak); four working warps
+// to a scheduler do not hide the chain from a code to the scaled sum.  Layers: what every block does once, arranging all states
+// before its first product and a tile's end.
 //
 // Measured, bf16 states, rows of 4096 in groups of 128, within a graph: 131072 rows (285 MB) by one state 53 us, 5.4 TB/s; by
-// eight 62 us, 4.6 TB/s; by 16 80 us, 3.6 TB/s; groups of 32, whose sums are scaled four times as often, by eight 82 us (336 MB,
-// 4.1 TB/s).  4096 rows by one state 5.2 us, of which the launch and the first stage's way are the most.
+// eight 61 us, 4.7 TB/s; by 16 80 us, 3.6 TB/s; groups of 32, whose sums are scaled four times as often, by eight 77 us (336 MB,
+// 4.4 TB/s).  16384 rows by one state 10.7 us, 3.3 TB/s; 4096 rows 5.1 us, of which the launch and the first stage's way are the most.
 #include <cuda.h>
 
 #include <atomic>
